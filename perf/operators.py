@@ -151,7 +151,7 @@ def _quantize(x, group):
     """f32 [..., dim] -> codes as int64 [..., dim], params f16 [..., dim / group, 2], by the definition above."""
     g = x.unflatten(-1, (-1, group))
     lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
-    s, m = ((hi - lo) / 15).half(), lo.half()
+    s, m = ((hi - lo) / torch.full_like(hi, 15)).half(), lo.half()          # a true division: by a Python number it is a product with 1 / 15
     c = torch.where(s > 0, torch.round((g - m.float()) / s.float()).clamp(0, 15), 0.0)
     return c.flatten(-2).to(torch.uint8), torch.cat([s, m], -1)
 
@@ -362,7 +362,7 @@ def exact(case, seed):
         for x in (s["k"], s["v"]):
             x = x.double().clamp(-65504, 65504).unflatten(-1, (-1, group))
             low, high = x.min(-1).values[..., None], x.max(-1).values[..., None]
-            step, low = ((high - low).float() / 15).half().double(), low.half().double()
+            step, low = ((high - low) / torch.full_like(high, 15)).float().half().double(), low.half().double()
             level = torch.where(step > 0, ((x - low) / step).round().clamp(0, 15), 0.0)
             out.append((low + level * step).flatten(-2))
         return tuple(out)
