@@ -441,6 +441,87 @@ OXQ_API int32_t oxq_gptq_quantize_layer(oxq_handle* h, const float* weights_dev,
                                 int bits, int symmetric, double percdamp, int32_t* quantized_dev, float* scales_dev,
                                 int32_t* zero_points_dev, int32_t* info_dev, void* workspace_dev, size_t workspace_bytes);
 
+/* ---- residual, norm and quantizer between two blocks ---------------------------------------------------------------
+ * The seam of a decoder layer around RmsNorm::forward (crates/oxicuda-lm/src/layer/norm.rs:73-95), one pass over the rows:
+ *   t  = y, or rms(y; post_weight) when post_weight is not NULL;  t *= gate when gate is not NULL
+ *   r' = residual + alpha * t                                     -> residual_out (may be residual itself)
+ *   h  = rms(r'; weight) -> out in the type of y / E4M3 of h / scale[0] (RNE, saturating, the input of oxq_gemm_fp8) /
+ *                           INT8 per row as oxq_int8_quant_rows (half to even, the input of oxq_gemm_w8a8)
+ * with rms(x; w) = x / sqrt(mean(x^2) + eps) * w.  f32 arithmetic throughout; r' is normed before it is rounded.  y, gate
+ * and out have `dtype` (OXQ_F32 / OXQ_BF16 / OXQ_F16), residual and residual_out `residual_dtype`: the same, or OXQ_F32.
+ * Rows are `*_ld` elements apart (multiples of 8, at least cols; gate_ld 0: one gate row for all); out, q and the codes are
+ * dense.  cols % 8 == 0, cols <= 16384; pointers 16-byte aligned (q: 8).  Apart from residual_out == residual (with the
+ * same leading dimension) no output may overlap an input.  A row with a NaN or an infinity gives NaNs in that row only. */
+typedef struct oxq_residual_norm {
+    const void* y; int64_t y_ld; int32_t dtype;
+    const void* residual; int64_t residual_ld; int32_t residual_dtype;
+    const void* gate; int64_t gate_ld;
+    const float* post_weight; const float* weight;
+    float alpha, eps;
+    void* residual_out; int64_t residual_out_ld;
+} oxq_residual_norm;
+OXQ_API int32_t oxq_residual_rmsnorm(oxq_handle* h, const oxq_residual_norm* args, int64_t rows, int64_t cols, void* out_dev);
+OXQ_API int32_t oxq_residual_rmsnorm_fp8(oxq_handle* h, const oxq_residual_norm* args, int64_t rows, int64_t cols, const float* scale_dev, uint8_t* q_dev);
+OXQ_API int32_t oxq_residual_rmsnorm_int8_rows(oxq_handle* h, const oxq_residual_norm* args, int64_t rows, int64_t cols, int8_t* q_dev, float* scales_dev);
+
+/* ---- 4-bit key / value cache, and attention over it ----------------------------------------------------------------
+ * The per-group affine quantizer (MinMaxQuantizer's int4_per_group, crates/oxicuda-quant/src/scheme/minmax.rs:146-167,
+ * :226-232) applied to keys and values as they enter a paged cache, and the attention entry of the reference's backend
+ * trait (crates/oxicuda-backend/src/lib.rs:198-409) over what the cache holds.
+ *
+ * The pool: `pages` pages of `page_size` tokens (a power of two, 16 to 4096) of `heads` kv heads of `dim` (64 or 128)
+ * elements, head-major: codes [pages][heads][page_size][dim / 2] bytes, params [pages][heads][page_size][dim / group] pairs of
+ * f16 (s, m), group 64 or 128, not above dim.  A group stands for c * s + m with s = f16((max - min) / 15), m = f16(min),
+ * c = clamp(rint((x - m) / s), 0, 15), 0 where s is 0.  x is held to +-65504 (s and m are f16) and a NaN is stored as 0.
+ * Eight codes a 32-bit word, element e of a word at bits [4 e, 4 e + 4); the words of a row are transposed in it: word
+ * 4 i + c of a key row lies at place c * (dim / 32) + i, word 8 i + c of a value row at place c * (dim / 64) + i.
+ *
+ * The batch: sequence b owns the call's tokens cu_tokens[b] .. cu_tokens[b + 1] (not decreasing; seqs + 1 offsets), and they
+ * are its last ones: with them it has seq_lens[b] tokens, the last at position seq_lens[b] - 1.  Position p lives in page
+ * block_table[b][p / page_size].  All three arrays are device memory and are read when the kernels run; `tokens` is the number
+ * of rows of the token arrays.  Rows behind the last sequence are not read, and left as they were.  Two sequences may
+ * share pages that are only read; two tokens of one append must not share a place (its contents are then unspecified).  A
+ * table entry that names no page of the pool, or a position behind the table's end, is never followed: an append skips the
+ * token, a read gives zeros, attention leaves the keys out, and oxq_device_status() then returns
+ * OXQ_ERR_INVALID_ARGUMENT.  A token before position 0 (more tokens than seq_lens) is skipped, reads as zeros, sees no key.
+ *
+ * oxq_kv4_append  keys and values [tokens][heads][dim] of `dtype` with any token and head strides (in elements; elements of a
+ *                 row are adjacent): the columns of a fused projection need no copy.
+ * oxq_kv4_read    the same tokens back as dense [tokens][heads][dim] of `dtype`.
+ * oxq_kv4_attention  q [tokens][q_heads][dim] (bf16 or f16), q_heads a multiple of heads; query head i reads kv head
+ *                 i / (q_heads / heads).  o = softmax(scale * q . k) v over the keys that the query sees: with `causal` those up
+ *                 to its own position, and with window > 0 of them the last `window`; without, all of the sequence.
+ *                 A query that sees no key gives zeros.  lse (f32 [tokens][q_heads], may be NULL) receives
+ *                 ln(sum(exp(scale * q . k))), -inf where nothing is seen.  max_tokens: the most tokens that a sequence has in
+ *                 this call (0: not known); it chooses kernels and sizes the workspace, results are right whatever it says.
+ *                 Out rows have strides like q's and are 4-byte aligned.  Scores, the softmax's statistics and the sums
+ *                 are f32.  The workspace (oxq_kv4_attention_workspace_bytes for dim and max_tokens * q_heads / heads; 16-byte
+ *                 aligned) needs no initial value and holds nothing between calls; calls that may overlap need one each. */
+typedef struct oxq_kv4_cache {
+    void* k_codes; void* k_params; void* v_codes; void* v_params;
+    int64_t pages;
+    int32_t page_size, heads, dim, group;
+} oxq_kv4_cache;
+typedef struct oxq_kv4_batch {
+    const int32_t* block_table; int64_t table_width;
+    const int32_t* seq_lens; const int32_t* cu_tokens;
+    int64_t seqs, tokens;
+} oxq_kv4_batch;
+typedef struct oxq_kv4_attention_args {
+    const void* q; int64_t q_token_stride, q_head_stride;
+    void* out; int64_t out_token_stride, out_head_stride;
+    float* lse;
+    int64_t q_heads, max_tokens, window;
+    float scale;
+    int32_t causal, dtype;
+} oxq_kv4_attention_args;
+OXQ_API int32_t oxq_kv4_append(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_kv4_batch* batch, const void* k_dev, int64_t k_token_stride,
+                       int64_t k_head_stride, const void* v_dev, int64_t v_token_stride, int64_t v_head_stride, int dtype);
+OXQ_API int32_t oxq_kv4_read(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_kv4_batch* batch, void* k_dev, void* v_dev, int dtype);
+OXQ_API int32_t oxq_kv4_attention_workspace_bytes(oxq_handle* h, int64_t dim, int64_t max_rows, size_t* bytes_out);
+OXQ_API int32_t oxq_kv4_attention(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_kv4_batch* batch, const oxq_kv4_attention_args* args,
+                          void* workspace_dev, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -60,6 +60,18 @@ struct OxqPerDevice {
     void set(int device, int value) { if ((unsigned)device < (unsigned)OXQ_MAX_DEVICES) v[device].store(value, std::memory_order_release); }
 };
 
+// Makes the handle's device current for the length of a call (a stream belongs to its device) and puts the caller's back.
+struct OxqDeviceGuard {
+    int prev = -1;
+    explicit OxqDeviceGuard(int device) {
+        int cur = -1;
+        if (cudaGetDevice(&cur) == cudaSuccess && cur != device && cudaSetDevice(device) == cudaSuccess) prev = cur;
+    }
+    ~OxqDeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
+    OxqDeviceGuard(const OxqDeviceGuard&) = delete;
+    OxqDeviceGuard& operator=(const OxqDeviceGuard&) = delete;
+};
+
 // Refuses to launch on anything but a compute-capability 10.x device: there is no fallback path.
 int32_t oxq_require_sm100(oxq_handle* h);
 

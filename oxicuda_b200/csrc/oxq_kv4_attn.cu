@@ -1,0 +1,597 @@
+// Attention of query tokens over the paged 4-bit cache (layout: oxq_kv4.cuh), for few query rows per kv head.
+//
+// The mathematics.  With k^ = c s + m per group, the score of a query row q (in units of log2) is
+//     x = scale log2(e) * sum over groups ( s * (q . c)_group + m * (sum of q)_group ),
+// so the product runs on the codes themselves and scale and offset are applied to its result in f32: the keys are never
+// rounded.  Likewise o = sum p v^ = sum (p s) c + sum p m: the second product's left factor is w = p s, its right factor
+// the codes; the offsets' sum is kept beside it in f32.  A code is used as the f16 number with those bits, the subnormal
+// c * 2^-24 (16 c * 2^-24 for a nibble that is left where it lies): one AND per two codes, exact, and the power of two is
+// taken out again in f32.  q enters as f16 scaled per row by a power of two, so that the row's largest element lies in
+// [2^11, 2^12): exact for f16 and bf16 values down to 2^-25 of the row's largest.
+// The running reference M of a row is the maximum over its keys of x + log2(largest s of the key's value row, rounded
+// down), so that w stays in f16's range whatever the scales are; it moves only when a key exceeds it by 2^8 (w <= 2^9),
+// which one vote per 16 keys finds out.  l = sum p, the offsets' sum and all accumulators are f32.
+// f16 outputs are finer than one f16 rounding of w; for them w is split into two f16 terms (two products).
+//
+// The shape.  mma.sync m16n8k16 with the keys as the 16 rows and 8 query rows as the columns (a kv head's query heads, and
+// the tokens of a run): S^T = K Q^T, then O^T = V^T P^T; P^T moves from accumulator to operand layout by movmatrix.
+// Eight warps of a CTA take 16 keys each of a tile of 128; all tiles of all (sequence, kv head, block of query rows) items
+// lie on one line, which the CTAs cut into equal parts (lengths are known on the device only).  An item that lies inside
+// one part is finished there; of a cut one every CTA leaves o, M and l in the workspace and a second kernel joins them, in
+// the order of the keys, so results do not depend on timing.
+#include "oxq_kv4_attn.cuh"
+
+namespace oxq {
+namespace kv4 {
+
+constexpr int TILE = 128;               // keys per tile: 8 warps x 16
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float lo_f32(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v & 0xFFFFu))); }
+__device__ __forceinline__ float hi_f32(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
+// floor(log2(s)) of a non-negative f16 number as a float, not below -24 (the smallest s there is; also for s = 0)
+__device__ __forceinline__ float log2_floor(float s) { return fmaxf((float)((int)(__float_as_uint(s) >> 23) - 127), -24.0f); }
+template <int N> __device__ __forceinline__ void load_words(uint32_t (&r)[N], const void* p) {
+    if constexpr (N == 4) { const uint4 v = __ldg(reinterpret_cast<const uint4*>(p)); r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
+    else if constexpr (N == 2) { const uint2 v = __ldg(reinterpret_cast<const uint2*>(p)); r[0] = v.x; r[1] = v.y; }
+    else r[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+}
+
+// The tiles of all items of one sequence, and of one item (row block rt).
+struct Span { int first, tiles; int lo, hi; };          // first tile, how many (at least one), visible positions [lo, hi)
+__device__ __forceinline__ Span item_span(const AttnParams& p, const SeqInfo& q, int rt, int nr) {
+    Span s;
+    const int j0 = (rt * nr) / p.per, j1 = min(q.n, (min((rt + 1) * nr, q.n * p.per) - 1) / p.per + 1) - 1;
+    s.hi = p.causal ? min(q.len, q.len - q.asked + j1 + 1) : q.len;
+    s.lo = p.window > 0 ? max(0, q.len - q.asked + j0 + 1 - p.window) : 0;
+    s.hi = max(s.hi, 0);
+    s.first = min(s.lo, s.hi) / TILE;
+    s.tiles = max(1, (s.hi + TILE - 1) / TILE - s.first);
+    return s;
+}
+__device__ __forceinline__ int row_blocks(const AttnParams& p, const SeqInfo& q, int nr) { return (q.n * p.per + nr - 1) / nr; }
+__device__ __forceinline__ int64_t head_tiles(const AttnParams& p, const SeqInfo& q, int nr) {
+    int64_t t = 0;
+    for (int rt = 0, e = row_blocks(p, q, nr); rt < e; rt++) t += item_span(p, q, rt, nr).tiles;
+    return t;
+}
+// Rows of this kernel: those of sequences with at most row_limit of them (0: all); the other kernel takes the rest.
+__device__ __forceinline__ SeqInfo small_seq(const AttnParams& p, int b) {
+    SeqInfo q = seq_info(p, b);
+    if (p.row_limit > 0 && (int64_t)q.n * p.per > p.row_limit) q.n = 0;
+    return q;
+}
+
+struct Where { int b; int64_t at; };    // sequence, and the line's position of its first tile
+// Sum of all sequences' tiles; every thread of the CTA gets it.  256 threads.
+__device__ __forceinline__ int64_t total_tiles(const AttnParams& p, int nr, int64_t* red) {
+    int64_t t = 0;
+    for (int b = threadIdx.x; b < p.s.seqs; b += 256) t += head_tiles(p, small_seq(p, b), nr) * p.c.heads;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = t;
+    __syncthreads();
+    t = 0;
+#pragma unroll
+    for (int w = 0; w < 8; w++) t += red[w];
+    __syncthreads();
+    return t;
+}
+// The sequence that holds tile `want` of the line (want < total).
+__device__ __forceinline__ Where find_tile(const AttnParams& p, int nr, int64_t want, int64_t* red, Where* found) {
+    int64_t base = 0;
+    for (int b0 = 0; b0 < p.s.seqs; b0 += 256) {
+        const int b = b0 + threadIdx.x;
+        const int64_t mine = b < p.s.seqs ? head_tiles(p, small_seq(p, b), nr) * p.c.heads : 0;
+        int64_t x = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if ((threadIdx.x & 31) >= o) x += y;
+        }
+        if ((threadIdx.x & 31) == 31) red[threadIdx.x >> 5] = x;
+        __syncthreads();
+        int64_t before = base, all = base;
+#pragma unroll
+        for (int w = 0; w < 8; w++) {
+            if (w < (int)(threadIdx.x >> 5)) before += red[w];
+            all += red[w];
+        }
+        const int64_t start = before + x - mine;
+        if (mine > 0 && start <= want && want < start + mine) { found->b = b; found->at = start; }
+        __syncthreads();
+        base = all;
+        if (want < base) break;
+    }
+    return *found;
+}
+
+// An item of a sequence: which one holds tile `in_seq` of the sequence's own line.
+struct Item { int head, rt; int64_t start; Span span; };
+__device__ __forceinline__ Item find_item(const AttnParams& p, const SeqInfo& q, int nr, int64_t in_seq) {
+    Item it;
+    const int64_t per_head = head_tiles(p, q, nr);
+    it.head = (int)(in_seq / per_head);
+    it.start = it.head * per_head;
+    for (it.rt = 0;; it.rt++) {
+        it.span = item_span(p, q, it.rt, nr);
+        if (in_seq < it.start + it.span.tiles) return it;
+        it.start += it.span.tiles;
+    }
+}
+
+template <int NT> struct Slot {         // what a cut item's CTA leaves: o [rows][D], then M, l
+    static constexpr int ROWS = NT * 8;
+    __host__ __device__ static constexpr int floats(int d) { return ROWS * (d + 2); }
+};
+
+template <typename T, int D, int NG, int NT>
+struct Smem {
+    static constexpr int ROWS = NT * 8, QPAD = D + 8;
+    __half q[ROWS * QPAD];              // per eight elements in the order 0 4 1 5 2 6 3 7, the odd ones / 16
+    float slab[8][ROWS * (D + 8)];
+    float a[ROWS], bsum[ROWS][NG];      // scale log2(e) 2^(24 + e - 11), scale log2(e) * sum of q
+    float m[8][ROWS], l[8][ROWS];
+    int64_t red[8];
+    Where found;
+};
+
+template <typename T, int D, int NG, int NT>
+__global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(AttnParams p) {
+    constexpr bool SPLIT = sizeof(T) == 2 && Elem<T>::kDtype == OXQ_F16;
+    constexpr int ROWS = NT * 8, NB = D / 32, NS = D / 64, QPAD = D + 8, OPAD = D + 8;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    Smem<T, D, NG, NT>& sm = *reinterpret_cast<Smem<T, D, NG, NT>*>(smem_raw);
+    pdl_trigger();
+    pdl_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
+
+    const int64_t total = total_tiles(p, ROWS, sm.red);
+    const int64_t parts = min((int64_t)gridDim.x, total);
+    if (blockIdx.x >= parts) return;
+    int64_t at = total * blockIdx.x / parts;
+    const int64_t begin = at, end = total * (blockIdx.x + 1) / parts;
+    Where w = find_tile(p, ROWS, at, sm.red, &sm.found);
+    SeqInfo seq = small_seq(p, w.b);
+    int64_t seq_tiles = head_tiles(p, seq, ROWS) * p.c.heads;
+
+    while (at < end) {
+        while (at >= w.at + seq_tiles) {                              // on to the next sequence that has tiles
+            w.at += seq_tiles;
+            w.b++;
+            if (w.b >= p.s.seqs) return;                              // cannot happen: `end` is within the line
+            seq = small_seq(p, w.b);
+            seq_tiles = head_tiles(p, seq, ROWS) * p.c.heads;
+        }
+        const Item it = find_item(p, seq, ROWS, at - w.at);
+        const int ta = (int)(at - w.at - it.start);
+        const int tb = (int)min((int64_t)it.span.tiles, (int64_t)ta + (end - at));
+        const bool whole = ta == 0 && tb == it.span.tiles;
+        const int row0 = it.rt * ROWS, rows = min(ROWS, seq.n * p.per - row0);
+
+        // ---- the query rows: D / 8 threads a row
+        __syncthreads();
+        for (int i = tid; i < ROWS * (D / 8); i += 256) {
+            const int row = i / (D / 8), g = i % (D / 8);
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] = 0.0f;
+            if (row < rows) {
+                const int j = (row0 + row) / p.per, qh = it.head * p.per + (row0 + row) % p.per;
+                const T* src = (const T*)p.q + (int64_t)(seq.start + j) * p.q_ts + (int64_t)qh * p.q_hs + g * 8;
+                if (p.q_vec) {
+                    const Vec16<T> v = ld16(src);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) f[e] = Elem<T>::to_f32(v.v[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) f[e] = Elem<T>::to_f32(src[e]);
+                }
+            }
+            float top = 0.0f, sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) { top = fmaxf(top, fabsf(f[e])); sum += f[e]; }
+#pragma unroll
+            for (int o = 1; o < D / 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+            for (int o = 1; o < D / 8 / NG; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const int ex = max((int)(__float_as_uint(top) >> 23) - 127, -100);
+            const float up = pow2_of(max(11 - ex, -126));
+            uint4 o;
+            o.x = pack_f16(f[0] * up, f[4] * up); o.y = pack_f16(f[1] * up * 0.0625f, f[5] * up * 0.0625f);
+            o.z = pack_f16(f[2] * up, f[6] * up); o.w = pack_f16(f[3] * up * 0.0625f, f[7] * up * 0.0625f);
+            *reinterpret_cast<uint4*>(&sm.q[row * QPAD + g * 8]) = o;
+            if (g == 0) sm.a[row] = p.scale_log2 * pow2_of(min(24 - 11 + ex, 127));
+            if (g % (D / 8 / NG) == 0) sm.bsum[row][g / (D / 8 / NG)] = p.scale_log2 * sum;
+        }
+        __syncthreads();
+
+        // ---- this warp's constants and accumulators; columns 2 c and 2 c + 1 of each block of eight rows are this lane's
+        float qa[NT][2], qb[NT][2][NG], M[NT][2], l[NT][2], po[NT][2][NG];
+        int vlo[NT][2], vhi[NT][2];
+        float acc[NS * 4][NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int row = nt * 8 + 2 * c + e;
+                qa[nt][e] = sm.a[row];
+                M[nt][e] = -1e30f; l[nt][e] = 0.0f;
+#pragma unroll
+                for (int g = 0; g < NG; g++) { qb[nt][e][g] = sm.bsum[row][g]; po[nt][e][g] = 0.0f; }
+                const int pos = seq.len - seq.asked + (row0 + row) / p.per;        // the row's own position
+                vhi[nt][e] = p.causal ? min(seq.len, pos + 1) : seq.len;
+                vlo[nt][e] = p.window > 0 ? pos + 1 - p.window : 0;
+            }
+#pragma unroll
+        for (int i = 0; i < NS * 4; i++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[i][nt][e] = 0.0f;
+        // keys that every row of the block sees need no mask
+        const int pos0 = seq.len - seq.asked + row0 / p.per, pos1 = seq.len - seq.asked + (row0 + rows - 1) / p.per;
+        const int all_hi = p.causal ? min(seq.len, pos0 + 1) : seq.len, all_lo = p.window > 0 ? pos1 + 1 - p.window : 0;
+
+        struct Keys { uint32_t k[2][NB], v[4][NS], kp[2][NG], vp[2][NG]; } cur, nxt;
+        const int32_t* table = p.s.table + (int64_t)w.b * p.s.width;
+        const auto slice = [&](int i) { return (it.span.first + i) * TILE + warp * 16; };
+        const auto wanted = [&](int i) { return i < tb && slice(i) < it.span.hi && slice(i) + 16 > it.span.lo; };
+        const auto page_of = [&](int i) -> int { return wanted(i) ? __ldg(table + (slice(i) >> p.c.page_shift)) : 0; };
+        const auto load = [&](Keys& k, int i, int page) -> bool {
+            if (!wanted(i)) return false;
+            if (page < 0 || page >= p.c.pages) { if (lane == 0) *p.status = OXQ_ERR_INVALID_ARGUMENT; return false; }
+            const int64_t row = (((int64_t)page * p.c.heads + it.head) << p.c.page_shift) + (slice(i) & ((1 << p.c.page_shift) - 1));
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                load_words(k.k[h], p.c.kc + (row + r + 8 * h) * (D / 2) + c * (D / 8));
+                load_words(k.kp[h], p.c.kp + (row + r + 8 * h) * NG);
+                load_words(k.vp[h], p.c.vp + (row + r + 8 * h) * NG);
+            }
+#pragma unroll
+            for (int h = 0; h < 4; h++) load_words(k.v[h], p.c.vc + (row + 2 * c + (h & 1) + (h >> 1) * 8) * (D / 2) + r * (D / 16));
+            return true;
+        };
+
+        bool have = load(cur, ta, page_of(ta));
+        int next_page = page_of(ta + 1);
+        for (int i = ta; i < tb; i++) {
+            const bool next_have = load(nxt, i + 1, next_page);
+            next_page = page_of(i + 2);
+            if (have) {
+                const int t0 = slice(i);
+                // ---- x = scores of keys t0 + r (elements 0, 1) and t0 + r + 8 (elements 2, 3)
+                float x[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[nt][e] = 0.0f;
+                const bool masked = t0 < all_lo || t0 + 16 > all_hi;
+                if (t0 + 16 > seq.len) {                              // rows behind the last key hold anything
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        if (t0 + r + 8 * h >= seq.len) {
+#pragma unroll
+                            for (int g = 0; g < NG; g++) { cur.kp[h][g] = 0; cur.vp[h][g] = 0; }
+                        }
+                }
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    float s4[NT][4];
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s4[nt][e] = 0.0f;
+#pragma unroll
+                    for (int i2 = 0; i2 < NB / NG; i2++) {
+                        const int blk = g * (NB / NG) + i2;
+                        const uint32_t w0 = cur.k[0][blk], w1 = cur.k[1][blk], u0 = w0 >> 8, u1 = w1 >> 8;
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            const uint4 qf = *reinterpret_cast<const uint4*>(&sm.q[(nt * 8 + r) * QPAD + blk * 32 + c * 8]);
+                            mma_16816(s4[nt], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf.x, qf.y);
+                            mma_16816(s4[nt], u0 & 0x000F000Fu, u1 & 0x000F000Fu, u0 & 0x00F000F0u, u1 & 0x00F000F0u, qf.z, qf.w);
+                        }
+                    }
+                    const float ks0 = lo_f32(cur.kp[0][g]), km0 = hi_f32(cur.kp[0][g]), ks1 = lo_f32(cur.kp[1][g]), km1 = hi_f32(cur.kp[1][g]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        x[nt][0] = fmaf(s4[nt][0] * ks0, qa[nt][0], fmaf(km0, qb[nt][0][g], x[nt][0]));
+                        x[nt][1] = fmaf(s4[nt][1] * ks0, qa[nt][1], fmaf(km0, qb[nt][1][g], x[nt][1]));
+                        x[nt][2] = fmaf(s4[nt][2] * ks1, qa[nt][0], fmaf(km1, qb[nt][0][g], x[nt][2]));
+                        x[nt][3] = fmaf(s4[nt][3] * ks1, qa[nt][1], fmaf(km1, qb[nt][1][g], x[nt][3]));
+                    }
+                }
+                if (masked) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int t = t0 + r + (e >> 1) * 8;
+                            if (t < vlo[nt][e & 1] || t >= vhi[nt][e & 1]) x[nt][e] = -INFINITY;
+                        }
+                }
+                // ---- the rows' reference
+                float vs[2][NG], vm[2][NG], big[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int g = 0; g < NG; g++) {
+                        vs[h][g] = lo_f32(cur.vp[h][g]); vm[h][g] = hi_f32(cur.vp[h][g]);
+                        top = fmaxf(top, vs[h][g]);
+                    }
+                    big[h] = log2_floor(top);
+                }
+                bool over = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) over |= x[nt][e] + big[e >> 1] > M[nt][e & 1] + 8.0f;
+                if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float top = fmaxf(x[nt][e] + big[0], x[nt][e + 2] + big[1]);
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            top = fmaxf(top, M[nt][e]);
+                            const float f = exp2f(M[nt][e] - top);
+                            M[nt][e] = top;
+                            l[nt][e] *= f;
+#pragma unroll
+                            for (int g = 0; g < NG; g++) po[nt][e][g] *= f;
+#pragma unroll
+                            for (int q = 0; q < NS * 4; q++) { acc[q][nt][e] *= f; acc[q][nt][e + 2] *= f; }
+                        }
+                }
+                // ---- p, its sums, and w = p s as the second product's operand
+                uint32_t wb[NT][NG][2], wc[NT][NG][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float e4[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) e4[e] = exp2f(x[nt][e] - M[nt][e & 1]);
+                    l[nt][0] += e4[0] + e4[2];
+                    l[nt][1] += e4[1] + e4[3];
+#pragma unroll
+                    for (int g = 0; g < NG; g++) {
+                        po[nt][0][g] = fmaf(e4[0], vm[0][g], fmaf(e4[2], vm[1][g], po[nt][0][g]));
+                        po[nt][1][g] = fmaf(e4[1], vm[0][g], fmaf(e4[3], vm[1][g], po[nt][1][g]));
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const float w0 = e4[2 * h] * vs[h][g], w1 = e4[2 * h + 1] * vs[h][g];
+                            const uint32_t hi = pack_f16(w0, w1);
+                            wb[nt][g][h] = transpose_8x8(hi);
+                            if constexpr (SPLIT) wc[nt][g][h] = transpose_8x8(pack_f16(w0 - lo_f32(hi), w1 - hi_f32(hi)));
+                        }
+                    }
+                }
+                // ---- O^T: rows r and r + 8 of block (s, j) are elements 64 s + 8 r + 2 j and + 1, the second one times 16
+#pragma unroll
+                for (int s = 0; s < NS; s++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        constexpr uint32_t kSel[4] = {0x4400u, 0x5511u, 0x6622u, 0x7733u};
+                        const int g = NG == 1 ? 0 : s;
+                        const uint32_t u = __byte_perm(cur.v[0][s], cur.v[1][s], kSel[j]), v = __byte_perm(cur.v[2][s], cur.v[3][s], kSel[j]);
+                        const uint32_t a0 = u & 0x000F000Fu, a1 = u & 0x00F000F0u, a2 = v & 0x000F000Fu, a3 = v & 0x00F000F0u;
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            mma_16816(acc[s * 4 + j][nt], a0, a1, a2, a3, wb[nt][g][0], wb[nt][g][1]);
+                            if constexpr (SPLIT) mma_16816(acc[s * 4 + j][nt], a0, a1, a2, a3, wc[nt][g][0], wc[nt][g][1]);
+                        }
+                    }
+            }
+            cur = nxt;
+            have = next_have;
+        }
+
+        // ---- join the warps: common reference, then one slab a warp
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], o);
+#pragma unroll
+                    for (int g = 0; g < NG; g++) po[nt][e][g] += __shfl_xor_sync(0xffffffffu, po[nt][e][g], o);
+                }
+                if (r == 0) { sm.m[warp][nt * 8 + 2 * c + e] = M[nt][e]; sm.l[warp][nt * 8 + 2 * c + e] = l[nt][e]; }
+            }
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int row = nt * 8 + 2 * c + e;
+                float top = sm.m[0][row];
+#pragma unroll
+                for (int q = 1; q < 8; q++) top = fmaxf(top, sm.m[q][row]);
+                const float f = exp2f(M[nt][e] - top);
+#pragma unroll
+                for (int s = 0; s < NS; s++) {
+                    const float off = po[nt][e][NG == 1 ? 0 : s] * f;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        float2 o;
+                        o.x = fmaf(acc[s * 4 + j][nt][e] * 0x1p24f, f, off);
+                        o.y = fmaf(acc[s * 4 + j][nt][e + 2] * 0x1p20f, f, off);
+                        *reinterpret_cast<float2*>(&sm.slab[warp][row * OPAD + 64 * s + 8 * r + 2 * j]) = o;
+                    }
+                }
+            }
+        __syncthreads();
+        float* slot = whole ? nullptr : p.ws + (int64_t)(blockIdx.x * 2 + (at == begin && ta > 0 ? 0 : 1)) * Slot<NT>::floats(D);
+        for (int i = tid; i < ROWS * (D / 2); i += 256) {
+            const int row = i / (D / 2), d = (i % (D / 2)) * 2;
+            float top = sm.m[0][row];
+#pragma unroll
+            for (int q = 1; q < 8; q++) top = fmaxf(top, sm.m[q][row]);
+            float sum = 0.0f;
+            float2 o = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                sum = fmaf(sm.l[q][row], exp2f(sm.m[q][row] - top), sum);
+                const float2 v = *reinterpret_cast<const float2*>(&sm.slab[q][row * OPAD + d]);
+                o.x += v.x; o.y += v.y;
+            }
+            if (slot) {
+                *reinterpret_cast<float2*>(slot + row * D + d) = o;
+                if (d == 0) { slot[ROWS * D + row] = top; slot[ROWS * D + ROWS + row] = sum; }
+            } else if (row < rows) {
+                store_row<T>(p, seq, it.head, row0 + row, d, o, top, sum);
+            }
+        }
+        at += tb - ta;
+    }
+}
+
+// Joins the parts of the items that the CTAs' boundaries cut.  Block x is for boundary x + 1: it acts if that is the first
+// boundary inside its item.  D / 4 threads a row.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnParams p, int ctas) {
+    constexpr int ROWS = NT * 8;
+    __shared__ int64_t red[8];
+    __shared__ Where found;
+    pdl_trigger();
+    pdl_wait();
+    const int64_t total = total_tiles(p, ROWS, red);
+    const int64_t parts = min((int64_t)ctas, total);
+    const int64_t i = blockIdx.x + 1;
+    if (i >= parts) return;
+    const auto bound = [&](int64_t k) { return total * k / parts; };
+    const Where w = find_tile(p, ROWS, bound(i), red, &found);
+    const SeqInfo seq = small_seq(p, w.b);
+    const Item it = find_item(p, seq, ROWS, bound(i) - w.at);
+    const int64_t start = w.at + it.start, stop = start + it.span.tiles;
+    if (start >= bound(i) || bound(i - 1) > start) return;            // not cut here, or not for the first time
+    int64_t last = i;                                                 // the CTA that holds the item's last tile
+    while (bound(last + 1) < stop) last++;
+    const int row0 = it.rt * ROWS, rows = min(ROWS, seq.n * p.per - row0);
+    const auto slot = [&](int64_t k) { return p.ws + (k * 2 + (k == i - 1 ? 1 : 0)) * Slot<NT>::floats(D); };
+    for (int q = threadIdx.x; q < rows * (D / 4); q += 256) {
+        const int row = q / (D / 4), d = (q % (D / 4)) * 4;
+        float top = -1e30f;
+        for (int64_t k = i - 1; k <= last; k++) top = fmaxf(top, slot(k)[ROWS * D + row]);
+        float sum = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int64_t k = i - 1; k <= last; k++) {
+            const float* s = slot(k);
+            const float f = exp2f(s[ROWS * D + row] - top);
+            const float4 v = *reinterpret_cast<const float4*>(s + row * D + d);
+            sum = fmaf(s[ROWS * D + ROWS + row], f, sum);
+            o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+        }
+        store_row<T>(p, seq, it.head, row0 + row, d, make_float2(o.x, o.y), top, sum);
+        store_row<T>(p, seq, it.head, row0 + row, d + 2, make_float2(o.z, o.w), top, sum);
+    }
+}
+
+}  // namespace kv4
+}  // namespace oxq
+
+using namespace oxq;
+using namespace oxq::kv4;
+
+static int attn_ctas(const oxq_handle* h, int nt) { return h->sm_count * (nt == 1 ? 2 : 1); }
+
+template <typename T, int D, int NG, int NT>
+static int32_t launch_rows(oxq_handle* h, const AttnParams& p, int64_t most_tiles, int64_t item_tiles) {
+    const int ctas = (int)(most_tiles < attn_ctas(h, NT) ? most_tiles : attn_ctas(h, NT));
+    auto kernel = kv4_attn_rows_kernel<T, D, NG, NT>;
+    constexpr int bytes = (int)sizeof(Smem<T, D, NG, NT>);
+    static OxqPerDevice ready;
+    if (!ready.get(h->device)) {
+        OXQ_CUDA(h, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        ready.set(h->device, 1);
+    }
+    OXQ_CUDA(h, oxq_launch(kernel, ctas, 256, bytes, h->stream, p));
+    if (ctas > 1 && item_tiles > 1) OXQ_CUDA(h, oxq_launch(kv4_attn_join_kernel<T, D, NT>, ctas - 1, 256, 0, h->stream, p, ctas));
+    return OXQ_OK;
+}
+
+template <typename T, int NT>
+static int32_t launch_dims(oxq_handle* h, const oxq_kv4_cache* cc, const AttnParams& p, int64_t most_tiles, int64_t item_tiles) {
+    if (cc->dim == 64) return launch_rows<T, 64, 1, NT>(h, p, most_tiles, item_tiles);
+    if (cc->group == 64) return launch_rows<T, 128, 2, NT>(h, p, most_tiles, item_tiles);
+    return launch_rows<T, 128, 1, NT>(h, p, most_tiles, item_tiles);
+}
+
+// Blocks of 8 or 16 query rows: 16 where a sequence has more than 8, because the codes are unpacked once for all of them.
+static int row_tiles(int64_t max_rows) { return max_rows <= 8 ? 1 : 2; }
+
+extern "C" {
+
+int32_t oxq_kv4_attention_workspace_bytes(oxq_handle* h, int64_t dim, int64_t max_rows, size_t* bytes_out) {
+    OXQ_CHECK_HANDLE(h);
+    if (!bytes_out) OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "null size");
+    if (dim != 64 && dim != 128) OXQ_FAIL(h, OXQ_ERR_UNSUPPORTED_OPERATION, "kv4: head dimension must be 64 or 128, got %lld", (long long)dim);
+    if (max_rows < 0) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 attention: negative row count");
+    const int nt = row_tiles(max_rows);
+    *bytes_out = (size_t)attn_ctas(h, nt) * 2 * (nt == 1 ? Slot<1>::floats((int)dim) : Slot<2>::floats((int)dim)) * sizeof(float);
+    return OXQ_OK;
+}
+
+int32_t oxq_kv4_attention(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_kv4_batch* batch, const oxq_kv4_attention_args* a, void* workspace,
+                          size_t workspace_bytes) {
+    OXQ_CHECK_HANDLE(h);
+    AttnParams p;
+    memset(&p, 0, sizeof(p));
+    if (int32_t rc = oxq_kv4_check(h, cache, batch, &p.c, &p.s)) return rc;
+    if (!a) OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: null arguments");
+    if (a->dtype != OXQ_BF16 && a->dtype != OXQ_F16) OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: queries are bf16 or f16, got dtype %d", a->dtype);
+    if (a->q_heads <= 0 || a->q_heads % p.c.heads != 0)
+        OXQ_FAIL(h, OXQ_ERR_DIMENSION_MISMATCH, "kv4 attention: %lld query heads over %d kv heads", (long long)a->q_heads, p.c.heads);
+    if (a->window < 0 || (a->window > 0 && !a->causal)) OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: a window must be positive, and needs the causal mask");
+    if (!(a->scale > -3.0e38f && a->scale < 3.0e38f)) OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: the scale is not finite");
+    if (a->max_tokens < 0) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 attention: negative max_tokens");
+    if (p.s.tokens == 0 || p.s.seqs == 0) return OXQ_OK;
+    if (!a->q || !a->out) OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: null queries or output");
+    if (a->q_token_stride < 0 || a->q_head_stride < 0 || a->out_token_stride < 0 || a->out_head_stride < 0)
+        OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: negative stride");
+    if (((uintptr_t)a->out | (uintptr_t)(a->out_token_stride * 2) | (uintptr_t)(a->out_head_stride * 2)) & 3u)
+        OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: output rows must be 4-byte aligned");
+    const int64_t per = a->q_heads / p.c.heads;
+    if (p.s.tokens * per > INT32_MAX / 2) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 attention: too many query rows");
+    const int64_t max_rows = (a->max_tokens > 0 && a->max_tokens < p.s.tokens ? a->max_tokens : p.s.tokens) * per;
+    size_t need = 0;
+    if (int32_t rc = oxq_kv4_attention_workspace_bytes(h, cache->dim, max_rows, &need)) return rc;
+    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15u))
+        OXQ_FAIL(h, OXQ_ERR_BUFFER_TOO_SMALL, "kv4 attention: workspace of %zu bytes (16-byte aligned), got %zu", need, workspace ? workspace_bytes : (size_t)0);
+    if (int32_t rc = oxq_require_sm100(h)) return rc;
+    OxqDeviceGuard guard(h->device);
+    p.q = a->q; p.q_ts = a->q_token_stride; p.q_hs = a->q_head_stride;
+    p.q_vec = (((uintptr_t)a->q | (uintptr_t)(a->q_token_stride * 2) | (uintptr_t)(a->q_head_stride * 2)) & 15u) == 0;
+    p.out = a->out; p.o_ts = a->out_token_stride; p.o_hs = a->out_head_stride; p.lse = a->lse;
+    p.per = (int)per; p.q_heads = (int)a->q_heads;
+    p.scale_log2 = a->scale * 1.44269504088896340736f;
+    p.causal = a->causal ? 1 : 0;
+    p.window = a->window > INT32_MAX ? INT32_MAX : (int)a->window;
+    p.ws = (float*)workspace; p.status = h->dev_status;
+    const int nt = row_tiles(max_rows);
+    // the most tiles that there can be: every row block of every sequence over a whole table row
+    const int64_t item_tiles = (p.s.width * cache->page_size + TILE - 1) / TILE + 1;
+    const int64_t items = (p.s.tokens * per + nt * 8 - 1) / (nt * 8) + p.s.seqs;
+    const int64_t most = items > (1ll << 40) / item_tiles / p.c.heads ? (1ll << 40) : items * item_tiles * p.c.heads;
+    if (a->dtype == OXQ_BF16)
+        return nt == 1 ? launch_dims<__nv_bfloat16, 1>(h, cache, p, most, item_tiles) : launch_dims<__nv_bfloat16, 2>(h, cache, p, most, item_tiles);
+    return nt == 1 ? launch_dims<__half, 1>(h, cache, p, most, item_tiles) : launch_dims<__half, 2>(h, cache, p, most, item_tiles);
+}
+
+}  // extern "C"

@@ -1,0 +1,53 @@
+// What the kernels of attention over the 4-bit cache share: the call's parameters, a sequence's extent, the output row.
+#pragma once
+#include "oxq_kv4.cuh"
+
+namespace oxq {
+namespace kv4 {
+
+struct AttnParams {
+    Pool c;
+    Batch s;
+    const void* q; int64_t q_ts, q_hs; int q_vec;       // strides in elements; 16-byte loads allowed
+    void* out; int64_t o_ts, o_hs;
+    float* lse;                                         // [tokens][q_heads], or null
+    int per, q_heads;                                   // query heads per kv head, all query heads
+    float scale_log2;                                   // scale * log2(e)
+    int causal, window;                                 // window 0: none
+    int row_limit;                                      // see small_seq()
+    float* ws;
+    int32_t* status;
+};
+
+// Sequence b: its first query token, how many of its tokens are in the call's rows, how many it asks for (the positions
+// count from that), how many keys it has.  Offsets and lengths come from the device and are held to their arrays here.
+struct SeqInfo { int start, n, asked, len; };
+__device__ __forceinline__ SeqInfo seq_info(const AttnParams& p, int b) {
+    SeqInfo q;
+    const int a = __ldg(p.s.cu + b), e = __ldg(p.s.cu + b + 1);
+    q.start = a;
+    q.asked = max(e - a, 0);
+    q.n = a < 0 || a >= p.s.tokens ? 0 : min((int64_t)q.asked, p.s.tokens - a);
+    if (a < 0 || e < a) q.asked = 0, q.n = 0;
+    const int len = max(__ldg(p.s.lens + b), 0);
+    const int64_t most = p.s.width << p.c.page_shift;
+    q.len = len > most ? (int)most : len;
+    return q;
+}
+
+// Two elements of an output row: row `row` of kv head `head` is query token row / per, query head head * per + row % per.
+// o / sum, or zeros where nothing was seen; with the first two goes lse = ln(sum over keys of exp(score)).
+template <typename T>
+__device__ __forceinline__ void store_row(const AttnParams& p, const SeqInfo& q, int head, int row, int d, float2 o, float ref, float sum) {
+    const int64_t t = q.start + row / p.per;
+    const int qh = head * p.per + row % p.per;
+    const float inv = sum > 0.0f ? __fdividef(1.0f, sum) : sum != sum ? sum : 0.0f;
+    struct alignas(4) Pair { T x, y; } v;
+    v.x = Elem<T>::from_f32(o.x * inv);
+    v.y = Elem<T>::from_f32(o.y * inv);
+    *reinterpret_cast<Pair*>((T*)p.out + t * p.o_ts + (int64_t)qh * p.o_hs + d) = v;
+    if (d == 0 && p.lse) p.lse[t * p.q_heads + qh] = sum > 0.0f || sum != sum ? (ref + log2f(sum)) * 0.693147180559945309417f : -INFINITY;
+}
+
+}  // namespace kv4
+}  // namespace oxq

@@ -610,6 +610,230 @@ def bias_add_(y: torch.Tensor, bias: torch.Tensor):
     return y
 
 
+# ------------------------------------------------------------------------------------------- between two blocks
+
+def _residual_norm_args(y, residual, weight, post_weight, gate, alpha, eps, residual_out):
+    from .errors import QuantError
+    if y.dim() != 2 or residual.shape != y.shape:
+        raise QuantError("DimensionMismatch", f"y {tuple(y.shape)} vs residual {tuple(residual.shape)}", 4)
+    rows, cols = y.shape
+    _same_device(y, residual, weight, post_weight, gate, residual_out)
+    if y.dtype not in _DT or residual.dtype not in (y.dtype, torch.float32):
+        raise TypeError(f"y is f32, bf16 or f16 and residual the same or f32, got {y.dtype} and {residual.dtype}")
+    for w in (weight, post_weight):
+        if w is not None:
+            _chk(w, torch.float32)
+            if w.numel() != cols:
+                raise QuantError("DimensionMismatch", f"expected {cols} weights, got {w.numel()}", 4)
+    gate_ld = 0
+    if gate is not None:
+        if gate.dtype != y.dtype or tuple(gate.shape) not in ((cols,), (rows, cols)):
+            raise QuantError("DimensionMismatch", f"gate {tuple(gate.shape)} {gate.dtype} for y {tuple(y.shape)} {y.dtype}", 4)
+        gate_ld = _row_stride(gate) if gate.dim() == 2 else 0
+        if gate.stride(-1) != 1 and cols > 1:
+            raise TypeError("expected gate rows of adjacent elements")
+    r_out = torch.empty((rows, cols), dtype=residual.dtype, device=y.device) if residual_out is None else residual_out
+    if r_out.shape != y.shape or r_out.dtype != residual.dtype:
+        raise QuantError("DimensionMismatch", f"residual_out {tuple(r_out.shape)} {r_out.dtype} for {tuple(residual.shape)} {residual.dtype}", 4)
+    return r_out, _ffi.ResidualNorm(y.data_ptr(), _row_stride(y), _DT[y.dtype], residual.data_ptr(), _row_stride(residual), _DT[residual.dtype],
+                                    None if gate is None else gate.data_ptr(), gate_ld, None if post_weight is None else post_weight.data_ptr(),
+                                    weight.data_ptr(), alpha, eps, r_out.data_ptr(), _row_stride(r_out))
+
+
+def _same_device(first, *rest):
+    if not first.is_cuda:
+        raise TypeError("expected a CUDA tensor")
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise TypeError(f"expected tensors on {first.device}, got one on {t.device}")
+
+
+def _row_stride(t):
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise TypeError("expected rows of adjacent elements")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def residual_rmsnorm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, post_weight: torch.Tensor | None = None,
+                     gate: torch.Tensor | None = None, alpha: float = 1.0, residual_out: torch.Tensor | None = None, out: torch.Tensor | None = None):
+    """The seam between two blocks in one pass: t = y or rms(y; post_weight), t *= gate ([cols] or [rows, cols]), r = residual + alpha * t,
+    h = rms(r; weight), RmsNorm::forward (crates/oxicuda-lm/src/layer/norm.rs:73-95) for rms.  Returns (r in residual's dtype, h in y's dtype);
+    residual_out may be residual itself.  y, residual, residual_out and gate may be row-strided views."""
+    r_out, args = _residual_norm_args(y, residual, weight, post_weight, gate, alpha, eps, residual_out)
+    if out is None:
+        out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    else:
+        _chk(out, y.dtype)
+        if out.shape != y.shape or out.device != y.device:
+            raise TypeError(f"out must be {tuple(y.shape)} on {y.device}")
+    handle(y.device.index).call("oxq_residual_rmsnorm", C.byref(args), y.shape[0], y.shape[1], out.data_ptr())
+    return r_out, out
+
+
+def residual_rmsnorm_fp8(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, eps: float = 1e-5,
+                         post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, alpha: float = 1.0,
+                         residual_out: torch.Tensor | None = None):
+    """residual_rmsnorm with h as E4M3 of h / scale[0] (the input of gemm_fp8): returns (r, codes uint8 [rows x cols])."""
+    r_out, args = _residual_norm_args(y, residual, weight, post_weight, gate, alpha, eps, residual_out)
+    _chk(scale, torch.float32)
+    _same_device(y, scale)
+    q = torch.empty(y.shape, dtype=torch.uint8, device=y.device)
+    handle(y.device.index).call("oxq_residual_rmsnorm_fp8", C.byref(args), y.shape[0], y.shape[1], scale.data_ptr(), q.data_ptr())
+    return r_out, q
+
+
+def residual_rmsnorm_int8_rows(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, post_weight: torch.Tensor | None = None,
+                               gate: torch.Tensor | None = None, alpha: float = 1.0, residual_out: torch.Tensor | None = None):
+    """residual_rmsnorm with h through the per-row INT8 quantizer (the input of gemm_w8a8): returns (r, codes int8 [rows x cols], scales f32 [rows])."""
+    r_out, args = _residual_norm_args(y, residual, weight, post_weight, gate, alpha, eps, residual_out)
+    q = torch.empty(y.shape, dtype=torch.int8, device=y.device)
+    sc = torch.empty(y.shape[0], dtype=torch.float32, device=y.device)
+    handle(y.device.index).call("oxq_residual_rmsnorm_int8_rows", C.byref(args), y.shape[0], y.shape[1], q.data_ptr(), sc.data_ptr())
+    return r_out, q, sc
+
+
+# ------------------------------------------------------------------------------------------- 4-bit key / value cache
+
+class Kv4Cache:
+    """A paged pool of 4-bit keys and values: codes uint8 [pages, heads, page_size, dim / 2] and params f16 [pages, heads, page_size, dim / group, 2]
+    (step and offset of each group of `group` elements), for keys and for values.  The affine per-group form of MinMaxQuantizer
+    (crates/oxicuda-quant/src/scheme/minmax.rs:146-167, :226-232) with a float offset.  dim is 64 or 128, group 64 or 128, page_size a power of two
+    from 16 to 4096."""
+
+    def __init__(self, k_codes: torch.Tensor, k_params: torch.Tensor, v_codes: torch.Tensor, v_params: torch.Tensor):
+        if k_codes.dim() != 4 or k_params.dim() != 5 or k_params.shape[4] != 2 or k_codes.shape[:3] != k_params.shape[:3] or \
+                v_codes.shape != k_codes.shape or v_params.shape != k_params.shape:
+            from .errors import QuantError
+            raise QuantError("DimensionMismatch", f"codes {tuple(k_codes.shape)}, {tuple(v_codes.shape)} with params {tuple(k_params.shape)}, {tuple(v_params.shape)}", 4)
+        for t, dt in ((k_codes, torch.uint8), (v_codes, torch.uint8), (k_params, torch.float16), (v_params, torch.float16)):
+            _chk(t, dt)
+        _same_device(k_codes, k_params, v_codes, v_params)
+        self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
+        self.pages, self.heads, self.page_size, half = k_codes.shape
+        self.dim = 2 * half
+        groups = k_params.shape[3]
+        self.group = self.dim // groups if groups and self.dim % groups == 0 else 0
+        self.device = k_codes.device
+        self._desc = _ffi.Kv4CacheDesc(k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(), self.pages, self.page_size,
+                                       self.heads, self.dim, self.group)
+
+    @classmethod
+    def empty(cls, pages: int, page_size: int, heads: int, dim: int, group: int = 64, device=None):
+        """An uninitialised pool; nothing in it is read before it is written."""
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        codes = [torch.empty((pages, heads, page_size, dim // 2), dtype=torch.uint8, device=device) for _ in range(2)]
+        params = [torch.empty((pages, heads, page_size, dim // max(group, 1), 2), dtype=torch.float16, device=device) for _ in range(2)]
+        return cls(codes[0], params[0], codes[1], params[1])
+
+
+def _kv4_batch(cache: Kv4Cache, block_table, seq_lens, cu_tokens, tokens: int):
+    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 or cu_tokens.dtype != torch.int32:
+        raise TypeError("block_table, seq_lens and cu_tokens are int32")
+    seqs = seq_lens.numel()
+    if block_table.dim() != 2 or block_table.shape[0] != seqs or cu_tokens.numel() != seqs + 1:
+        from .errors import QuantError
+        raise QuantError("DimensionMismatch", f"block_table {tuple(block_table.shape)}, seq_lens {tuple(seq_lens.shape)}, cu_tokens {tuple(cu_tokens.shape)}", 4)
+    dev = cache.device
+    if block_table.device != dev or seq_lens.device != dev or cu_tokens.device != dev:
+        raise TypeError(f"expected block_table, seq_lens and cu_tokens on {dev}")
+    if not (block_table.is_contiguous() and seq_lens.is_contiguous() and cu_tokens.is_contiguous()):
+        raise TypeError("expected contiguous block_table, seq_lens and cu_tokens")
+    return _ffi.Kv4BatchDesc(block_table.data_ptr(), block_table.shape[1], seq_lens.data_ptr(), cu_tokens.data_ptr(), seqs, tokens)
+
+
+def _kv4_rows(t: torch.Tensor, heads: int, cache: Kv4Cache, what: str, dtypes):
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != cache.dim:
+        from .errors import QuantError
+        raise QuantError("DimensionMismatch", f"{what} {tuple(t.shape)}, expected [tokens, {heads}, {cache.dim}]", 4)
+    if t.dtype not in dtypes:
+        raise TypeError(f"{what}: expected dtype in {tuple(dtypes)}, got {t.dtype}")
+    if t.device != cache.device:
+        raise TypeError(f"{what}: expected a tensor on {cache.device}")
+    if t.stride(2) != 1:
+        raise TypeError(f"{what}: expected rows of adjacent elements")
+
+
+def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_tokens: torch.Tensor):
+    """Quantises keys and values [tokens, heads, dim] (f32, bf16 or f16; any token and head strides) into the pool.  Sequence b owns tokens
+    cu_tokens[b]:cu_tokens[b + 1], its last ones of seq_lens[b]; position p lives in page block_table[b, p // page_size].  Rows behind the last
+    sequence are not read."""
+    _kv4_rows(k, cache.heads, cache, "k", _DT)
+    _kv4_rows(v, cache.heads, cache, "v", (k.dtype,))
+    if v.shape != k.shape:
+        from .errors import QuantError
+        raise QuantError("DimensionMismatch", f"k {tuple(k.shape)} vs v {tuple(v.shape)}", 4)
+    batch = _kv4_batch(cache, block_table, seq_lens, cu_tokens, k.shape[0])
+    handle(cache.device.index).call("oxq_kv4_append", C.byref(cache._desc), C.byref(batch), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                                    v.stride(1), _DT[k.dtype])
+    return cache
+
+
+def kv4_read(cache: Kv4Cache, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_tokens: torch.Tensor, tokens: int, dtype=torch.bfloat16,
+             k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None):
+    """The last cu_tokens[b + 1] - cu_tokens[b] tokens of every sequence as (k, v) [tokens, heads, dim]; rows behind the last sequence are left as
+    they were (uninitialised where the call allocates)."""
+    shape = (int(tokens), cache.heads, cache.dim)
+    outs = []
+    for t, what in ((k_out, "k_out"), (v_out, "v_out")):
+        if t is None:
+            t = torch.empty(shape, dtype=dtype, device=cache.device)
+        else:
+            _kv4_rows(t, cache.heads, cache, what, (dtype,))
+            if t.shape[0] != shape[0] or not t.is_contiguous():
+                raise TypeError(f"{what}: expected a contiguous tensor of {shape}")
+        outs.append(t)
+    batch = _kv4_batch(cache, block_table, seq_lens, cu_tokens, shape[0])
+    handle(cache.device.index).call("oxq_kv4_read", C.byref(cache._desc), C.byref(batch), outs[0].data_ptr(), outs[1].data_ptr(), _DT[dtype])
+    return outs[0], outs[1]
+
+
+def kv4_attention_workspace_bytes(cache: Kv4Cache, max_rows: int) -> int:
+    """Bytes of workspace for kv4_attention; max_rows = max_tokens * q_heads / heads."""
+    n = C.c_size_t(0)
+    handle(cache.device.index).call("oxq_kv4_attention_workspace_bytes", cache.dim, max_rows, C.byref(n))
+    return n.value
+
+
+def kv4_attention(q: torch.Tensor, cache: Kv4Cache, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_tokens: torch.Tensor, max_tokens: int = 0,
+                  scale: float | None = None, causal: bool = True, window: int = 0, out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                  want_lse: bool = False, workspace: torch.Tensor | None = None):
+    """Attention of queries [tokens, q_heads, dim] (bf16 or f16; any token and head strides) over what the pool holds: softmax(scale * q . k) v, scale
+    dim ** -0.5 unless given, over the keys up to each query's own position (causal; the last `window` of them if window > 0) or all of its sequence.
+    A query that sees no key gives zeros (and -inf in lse).  max_tokens: the most tokens a sequence has in this call, 0 if it is not known; it
+    only chooses kernels.  Returns out, or (out, lse f32 [tokens, q_heads]) if want_lse or lse is given.  Rows behind the last sequence
+    are left as they were.  `workspace` (uint8, kv4_attention_workspace_bytes) may be given to allocate nothing; overlapping calls need one each."""
+    if q.dim() != 3 or q.shape[1] == 0 or cache.heads == 0 or q.shape[1] % cache.heads != 0:
+        from .errors import QuantError
+        raise QuantError("DimensionMismatch", f"q {tuple(q.shape)} over {cache.heads} kv heads", 4)
+    tokens, heads = q.shape[0], q.shape[1]
+    _kv4_rows(q, heads, cache, "q", (torch.bfloat16, torch.float16))
+    if out is None:
+        out = torch.empty((tokens, heads, cache.dim), dtype=q.dtype, device=q.device)
+    else:
+        _kv4_rows(out, heads, cache, "out", (q.dtype,))
+        if out.shape[0] != tokens:
+            raise TypeError(f"out: expected {tokens} tokens, got {out.shape[0]}")
+    if lse is not None:
+        _chk(lse, torch.float32)
+        if tuple(lse.shape) != (tokens, heads) or lse.device != q.device:
+            raise TypeError(f"lse: expected {(tokens, heads)} on {q.device}")
+    elif want_lse:
+        lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
+    batch = _kv4_batch(cache, block_table, seq_lens, cu_tokens, tokens)
+    h = handle(cache.device.index)
+    if workspace is None:
+        most = tokens if max_tokens <= 0 else min(tokens, max_tokens)
+        workspace = torch.empty(max(kv4_attention_workspace_bytes(cache, most * (heads // cache.heads)), 16), dtype=torch.uint8, device=q.device)
+    else:
+        _chk(workspace, torch.uint8)
+        if workspace.device != q.device:
+            raise TypeError(f"workspace: expected a tensor on {q.device}")
+    args = _ffi.Kv4AttentionArgs(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(),
+                                 heads, max_tokens, window, cache.dim ** -0.5 if scale is None else scale, 1 if causal else 0, _DT[q.dtype])
+    h.call("oxq_kv4_attention", C.byref(cache._desc), C.byref(batch), C.byref(args), workspace.data_ptr(), workspace.numel())
+    return out if lse is None else (out, lse)
+
+
 # ------------------------------------------------------------------------------------------- GEMMs
 
 def gemm_fp8(x_q, w_q, sx, sw, out: torch.Tensor | None = None):
