@@ -495,8 +495,9 @@ OXQ_API int32_t oxq_residual_rmsnorm_int8_rows(oxq_handle* h, const oxq_residual
  *                 ln(sum(exp(scale * q . k))), -inf where nothing is seen.  max_tokens: the most tokens that a sequence has in
  *                 this call (0: not known); it chooses kernels and sizes the workspace, results are right whatever it says.
  *                 Out rows have strides like q's and are 4-byte aligned.  Scores, the softmax's statistics and the sums
- *                 are f32.  The workspace (oxq_kv4_attention_workspace_bytes for dim and max_tokens * q_heads / heads; 16-byte
- *                 aligned) needs no initial value and holds nothing between calls; calls that may overlap need one each. */
+ *                 are f32.  The workspace (oxq_kv4_attention_workspace_bytes of the same call; the batch's arrays are not looked
+ *                 at; 16-byte aligned) needs no initial value and holds nothing between calls; calls that may overlap need one
+ *                 each. */
 typedef struct oxq_kv4_cache {
     void* k_codes; void* k_params; void* v_codes; void* v_params;
     int64_t pages;
@@ -518,7 +519,8 @@ typedef struct oxq_kv4_attention_args {
 OXQ_API int32_t oxq_kv4_append(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_kv4_batch* batch, const void* k_dev, int64_t k_token_stride,
                        int64_t k_head_stride, const void* v_dev, int64_t v_token_stride, int64_t v_head_stride, int dtype);
 OXQ_API int32_t oxq_kv4_read(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_kv4_batch* batch, void* k_dev, void* v_dev, int dtype);
-OXQ_API int32_t oxq_kv4_attention_workspace_bytes(oxq_handle* h, int64_t dim, int64_t max_rows, size_t* bytes_out);
+OXQ_API int32_t oxq_kv4_attention_workspace_bytes(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_kv4_batch* batch, int64_t q_heads,
+                                          int64_t max_tokens, size_t* bytes_out);
 OXQ_API int32_t oxq_kv4_attention(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_kv4_batch* batch, const oxq_kv4_attention_args* args,
                           void* workspace_dev, size_t workspace_bytes);
 

@@ -111,7 +111,7 @@ SIGNATURES = {
     "oxq_residual_rmsnorm_int8_rows": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp]),
     "oxq_kv4_append": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _int]),
     "oxq_kv4_read": (_i32, [_vp, _vp, _vp, _vp, _vp, _int]),
-    "oxq_kv4_attention_workspace_bytes": (_i32, [_vp, _i64, _i64, _vp]),
+    "oxq_kv4_attention_workspace_bytes": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),
     "oxq_kv4_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _sz]),
     "oxq_gemm_mxfp8": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64]),
     "oxq_gemm_nvfp4": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64]),

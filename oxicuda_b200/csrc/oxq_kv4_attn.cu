@@ -533,18 +533,49 @@ static int32_t launch_dims(oxq_handle* h, const oxq_kv4_cache* cc, const AttnPar
     return launch_rows<T, 128, 1, NT>(h, p, most_tiles, item_tiles);
 }
 
-// Blocks of 8 or 16 query rows: 16 where a sequence has more than 8, because the codes are unpacked once for all of them.
-static int row_tiles(int64_t max_rows) { return max_rows <= 8 ? 1 : 2; }
+// Which kernels a call needs.  Up to ROWS_MOST query rows per sequence and kv head go to the kernel above, more to the tiles of
+// oxq_kv4_tiles.cu.  A batch may hold both kinds, and only the device knows its sequences, so with more than one both kernels
+// are launched and each takes its own; a single sequence goes whole to the one that its bound asks for.
+constexpr int64_t ROWS_MOST = 64;
+struct Plan {
+    int nt;                             // blocks of 8 or 16 query rows: 16 where a sequence has more than 8, because the codes are unpacked once for all of them
+    bool rows, tiles;
+    int64_t items; int parts;           // tile kernel: most pairs of blocks; CTAs an item
+    size_t rows_bytes, bytes;
+};
+static Plan make_plan(const oxq_handle* h, const oxq_kv4_cache* cc, const oxq_kv4_batch* s, int64_t per, int64_t max_tokens) {
+    Plan f;
+    const int64_t all_rows = s->tokens * per, max_rows = (max_tokens > 0 && max_tokens < s->tokens ? max_tokens : s->tokens) * per;
+    f.nt = max_rows <= 8 ? 1 : 2;
+    f.tiles = max_rows > ROWS_MOST;
+    f.rows = !f.tiles || s->seqs > 1;
+    f.rows_bytes = f.rows ? (size_t)attn_ctas(h, f.nt) * 2 * (f.nt == 1 ? Slot<1>::floats(cc->dim) : Slot<2>::floats(cc->dim)) * sizeof(float) : 0;
+    f.items = 0; f.parts = 1;
+    if (f.tiles) {
+        const int64_t with = all_rows / (ROWS_MOST + 1) < s->seqs ? all_rows / (ROWS_MOST + 1) : s->seqs;
+        f.items = s->seqs == 1 ? (all_rows + 255) / 256 : all_rows / 256 + with;
+        // too few CTAs for the machine: several share an item's keys (at least four tiles each of the longest the table allows)
+        const int64_t ctas = f.items * cc->heads, most = s->table_width * cc->page_size / (4 * TILE);
+        int64_t parts = ctas * 2 <= h->sm_count ? h->sm_count / ctas : 1;
+        if (parts > most) parts = most;
+        if (parts > 16) parts = 16;
+        f.parts = parts < 1 ? 1 : (int)parts;
+    }
+    f.bytes = f.rows_bytes + (f.parts > 1 ? (size_t)f.items * cc->heads * f.parts * oxq_kv4_tiles_slot_bytes(cc->dim) : 0);
+    return f;
+}
 
 extern "C" {
 
-int32_t oxq_kv4_attention_workspace_bytes(oxq_handle* h, int64_t dim, int64_t max_rows, size_t* bytes_out) {
+int32_t oxq_kv4_attention_workspace_bytes(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_kv4_batch* batch, int64_t q_heads, int64_t max_tokens,
+                                          size_t* bytes_out) {
     OXQ_CHECK_HANDLE(h);
+    Pool c; Batch s;
+    if (int32_t rc = oxq_kv4_check(h, cache, batch, &c, &s)) return rc;
     if (!bytes_out) OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "null size");
-    if (dim != 64 && dim != 128) OXQ_FAIL(h, OXQ_ERR_UNSUPPORTED_OPERATION, "kv4: head dimension must be 64 or 128, got %lld", (long long)dim);
-    if (max_rows < 0) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 attention: negative row count");
-    const int nt = row_tiles(max_rows);
-    *bytes_out = (size_t)attn_ctas(h, nt) * 2 * (nt == 1 ? Slot<1>::floats((int)dim) : Slot<2>::floats((int)dim)) * sizeof(float);
+    if (q_heads <= 0 || q_heads % c.heads != 0) OXQ_FAIL(h, OXQ_ERR_DIMENSION_MISMATCH, "kv4 attention: %lld query heads over %d kv heads", (long long)q_heads, c.heads);
+    if (max_tokens < 0) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 attention: negative max_tokens");
+    *bytes_out = make_plan(h, cache, batch, q_heads / c.heads, max_tokens).bytes;
     return OXQ_OK;
 }
 
@@ -569,11 +600,9 @@ int32_t oxq_kv4_attention(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_k
         OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: output rows must be 4-byte aligned");
     const int64_t per = a->q_heads / p.c.heads;
     if (p.s.tokens * per > INT32_MAX / 2) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 attention: too many query rows");
-    const int64_t max_rows = (a->max_tokens > 0 && a->max_tokens < p.s.tokens ? a->max_tokens : p.s.tokens) * per;
-    size_t need = 0;
-    if (int32_t rc = oxq_kv4_attention_workspace_bytes(h, cache->dim, max_rows, &need)) return rc;
-    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15u))
-        OXQ_FAIL(h, OXQ_ERR_BUFFER_TOO_SMALL, "kv4 attention: workspace of %zu bytes (16-byte aligned), got %zu", need, workspace ? workspace_bytes : (size_t)0);
+    const Plan plan = make_plan(h, cache, batch, per, a->max_tokens);
+    if (!workspace || workspace_bytes < plan.bytes || ((uintptr_t)workspace & 15u))
+        OXQ_FAIL(h, OXQ_ERR_BUFFER_TOO_SMALL, "kv4 attention: workspace of %zu bytes (16-byte aligned), got %zu", plan.bytes, workspace ? workspace_bytes : (size_t)0);
     if (int32_t rc = oxq_require_sm100(h)) return rc;
     OxqDeviceGuard guard(h->device);
     p.q = a->q; p.q_ts = a->q_token_stride; p.q_hs = a->q_head_stride;
@@ -583,8 +612,18 @@ int32_t oxq_kv4_attention(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_k
     p.scale_log2 = a->scale * 1.44269504088896340736f;
     p.causal = a->causal ? 1 : 0;
     p.window = a->window > INT32_MAX ? INT32_MAX : (int)a->window;
-    p.ws = (float*)workspace; p.status = h->dev_status;
-    const int nt = row_tiles(max_rows);
+    p.out_vec = (((uintptr_t)a->out | (uintptr_t)(a->out_token_stride * 2) | (uintptr_t)(a->out_head_stride * 2)) & 15u) == 0;
+    p.status = h->dev_status;
+    if (plan.tiles) {
+        p.row_min = plan.rows ? (int)ROWS_MOST : 0;
+        p.parts = plan.parts;
+        p.ws = (float*)((char*)workspace + plan.rows_bytes);
+        if (int32_t rc = oxq_kv4_tiles_launch(h, cache, p, a->dtype, plan.items)) return rc;
+        if (!plan.rows) return OXQ_OK;
+        p.row_limit = (int)ROWS_MOST;
+    }
+    p.ws = (float*)workspace;
+    const int nt = plan.nt;
     // the most tiles that there can be: every row block of every sequence over a whole table row
     const int64_t item_tiles = (p.s.width * cache->page_size + TILE - 1) / TILE + 1;
     const int64_t items = (p.s.tokens * per + nt * 8 - 1) / (nt * 8) + p.s.seqs;

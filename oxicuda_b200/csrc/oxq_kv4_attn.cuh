@@ -14,7 +14,8 @@ struct AttnParams {
     int per, q_heads;                                   // query heads per kv head, all query heads
     float scale_log2;                                   // scale * log2(e)
     int causal, window;                                 // window 0: none
-    int row_limit;                                      // see small_seq()
+    int row_limit, row_min;                             // sequences of at most row_limit rows (0: all) are the row kernel's, of more than row_min the tile kernel's
+    int parts, out_vec;                                 // tile kernel: CTAs that share an item's keys; 16-byte stores allowed
     float* ws;
     int32_t* status;
 };
@@ -51,3 +52,7 @@ __device__ __forceinline__ void store_row(const AttnParams& p, const SeqInfo& q,
 
 }  // namespace kv4
 }  // namespace oxq
+
+// Many query rows: oxq_kv4_tiles.cu.  `items` bounds the pairs of row blocks of all sequences.
+int64_t oxq_kv4_tiles_slot_bytes(int dim);
+int32_t oxq_kv4_tiles_launch(oxq_handle* h, const oxq_kv4_cache* cache, const oxq::kv4::AttnParams& p, int dtype, int64_t items);

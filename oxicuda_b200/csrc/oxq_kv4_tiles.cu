@@ -1,0 +1,532 @@
+// Attention over the paged 4-bit cache for many query rows per kv head (layout: oxq_kv4.cuh): prompts and chunks of them.
+//
+// The mathematics is the usual one: S = Q K^T, a running reference M per row (moved only when a score exceeds it by 2^8, as
+// all exponents are taken in base 2), P = 2^(S - M), O += P V, l += row sums of P, o = O / l at the end.  Keys and values
+// become f16 numbers rounded once from c s + m (halved, so that none overflows: the factor is taken out again in f32), P is
+// f16, everything else f32.  f16 rather than bf16 operands, for either type of the queries: their rounding is eight times
+// finer.  A query row enters scaled by a power of two so that its largest element lies in [2^11, 2^12), which keeps
+// every f16 and bf16 value exact down to 2^-25 of that; the row's factor goes into the softmax.  l is summed from the unrounded p.
+//
+// The shape: a CTA takes two blocks of 128 query rows (tokens and the query heads of one kv head, packed) and walks the keys
+// in tiles of 128.  tcgen05.mma: S from shared memory (Q and the tile's keys), O from P in tensor memory, written over the
+// scores, and the tile's values.  Roles: two warpgroups of softmax (one row a thread), one that turns codes into f16 tiles
+// (two stages each of keys and values), one warp that issues the products.  While one block's scores are in softmax the
+// tensor core works on the other block's.  Inside every eight elements of a head the order is 0 4 1 5 2 6 3 7, which is
+// the order in which a word's nibbles come out in pairs; it is undone where O is stored.
+#include "oxq_kv4_attn.cuh"
+#include "oxq_tc.cuh"
+
+namespace oxq {
+namespace kv4 {
+
+using namespace tc;
+
+constexpr int BLOCK = 128;                      // rows of a block, and keys of a tile
+constexpr int ATOM = BLOCK * 128;               // bytes of 128 rows of 128 bytes (64 f16), the swizzle's unit
+
+template <int D> struct TileSmem {
+    static constexpr int OPERAND = ATOM * (D / 64);
+    static constexpr int Q = 0, K = Q + 2 * OPERAND, V = K + 2 * OPERAND, BARS = V + 2 * OPERAND, VALID = BARS + 128, SLOT = VALID + 32, BYTES = SLOT + 16 + 1024;
+};
+enum { BAR_Q = 0, BAR_KFULL = 1, BAR_KEMPTY = 3, BAR_VFULL = 5, BAR_VEMPTY = 7, BAR_S = 9, BAR_P = 11, BAR_END = 13 };
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
+__device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
+__device__ __forceinline__ float lower(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v & 0xFFFFu))); }
+__device__ __forceinline__ float upper(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
+
+// Eight codes of a word to f16 c s + m, one rounding each, in the order 0 4 1 5 2 6 3 7.  A nibble under the exponent of 1024
+// is the number 1024 + c (or 1024 + 16 c where it is left four bits up), from which c is exact in one operation.
+__device__ __forceinline__ uint4 expand(uint32_t w, __half2 s, __half2 m) {
+    const __half2 k1024 = as_half2(0x64006400u), k16 = as_half2(0x2C002C00u), k64 = as_half2(0xD400D400u);    // 1024, 1 / 16, -64
+    uint4 o;
+    o.x = as_u32(__hfma2(__hsub2(as_half2((w & 0x000F000Fu) | 0x64006400u), k1024), s, m));
+    o.y = as_u32(__hfma2(__hfma2(as_half2((w & 0x00F000F0u) | 0x64006400u), k16, k64), s, m));
+    w >>= 8;
+    o.z = as_u32(__hfma2(__hsub2(as_half2((w & 0x000F000Fu) | 0x64006400u), k1024), s, m));
+    o.w = as_u32(__hfma2(__hfma2(as_half2((w & 0x00F000F0u) | 0x64006400u), k16, k64), s, m));
+    return o;
+}
+
+// The CTA's item: sequence and pair of row blocks.  Items of a sequence come last rows first: they see the most keys.
+struct TileItem { int b, pair; SeqInfo q; };
+__device__ __forceinline__ int pairs_of(const AttnParams& p, int b) {
+    const SeqInfo q = seq_info(p, b);
+    const int64_t rows = (int64_t)q.n * p.per;
+    return rows <= p.row_min ? 0 : (int)((rows + 2 * BLOCK - 1) / (2 * BLOCK));
+}
+// Whole warp; false: there is no such item.
+__device__ __forceinline__ bool find_pair(const AttnParams& p, int want, TileItem& it) {
+    const int lane = threadIdx.x & 31;
+    int base = 0;
+    for (int b0 = 0; b0 < p.s.seqs; b0 += 32) {
+        const int n = b0 + lane < p.s.seqs ? pairs_of(p, b0 + lane) : 0;
+        int x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, want >= base + x - n && want < base + x);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            it.b = b0 + src;
+            it.pair = __shfl_sync(0xffffffffu, x, src) + base - 1 - want;
+            it.q = seq_info(p, it.b);
+            return true;
+        }
+        base += __shfl_sync(0xffffffffu, x, 31);
+    }
+    return false;
+}
+
+// What the rows row0 .. of an item see together: tiles [first, first + n), this CTA's part of them.
+struct Walk { int first, n; };
+__device__ __forceinline__ Walk walk_of(const AttnParams& p, const SeqInfo& q, int pair, int part) {
+    const int row0 = pair * 2 * BLOCK;
+    const int j0 = row0 / p.per, j1 = (min(row0 + 2 * BLOCK, q.n * p.per) - 1) / p.per;
+    const int hi = max(0, p.causal ? min(q.len, q.len - q.asked + j1 + 1) : q.len);
+    const int lo = min(hi, p.window > 0 ? max(0, q.len - q.asked + j0 + 1 - p.window) : 0);
+    const int first = lo / BLOCK, all = (hi + BLOCK - 1) / BLOCK - first;
+    const int a = (int)((int64_t)all * part / p.parts), e = (int)((int64_t)all * (part + 1) / p.parts);
+    return {first + a, e - a};
+}
+
+template <typename T, int D, int NG>
+__global__ void __launch_bounds__(416, 1) kv4_attn_tiles_kernel(AttnParams p) {
+    using L = TileSmem<D>;
+    constexpr int NA = D / 64;
+    extern __shared__ unsigned char smem_dyn[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_wait();
+
+    TileItem it;
+    const int head = blockIdx.x % p.c.heads, part = blockIdx.y;
+    if (!find_pair(p, blockIdx.x / p.c.heads, it)) { pdl_trigger(); return; }      // the grid is an upper bound
+    const SeqInfo q = it.q;
+    const Walk walk = walk_of(p, q, it.pair, part);
+    const int n = walk.n;
+
+    const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
+    unsigned char* smem = smem_dyn + (base - smem_u32(smem_dyn));
+    const auto bar = [&](int i) { return base + L::BARS + 8 * i; };
+    if (warp == 12) {
+        if (lane == 0) {
+            mbar_init(bar(BAR_Q), 256);
+            mbar_init(bar(BAR_END), 1);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                mbar_init(bar(BAR_KFULL + i), 128); mbar_init(bar(BAR_KEMPTY + i), 1);
+                mbar_init(bar(BAR_VFULL + i), 128); mbar_init(bar(BAR_VEMPTY + i), 1);
+                mbar_init(bar(BAR_S + i), 1); mbar_init(bar(BAR_P + i), 128);
+            }
+            fence_barrier_init();
+        }
+        __syncwarp();
+        tmem_alloc(base + L::SLOT, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_trigger();                              // only now: a kernel that starts early must not find tensor memory before this one
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::SLOT);
+    const auto fail = [&]() { *p.status = OXQ_ERR_DEVICE_TIMEOUT; };
+
+    if (warp < 8) {
+        // ------------------------------------------------------------------------------------ softmax: one row a thread
+        const int t = warp >> 2, r = (warp & 3) * 32 + lane;
+        const int row = it.pair * 2 * BLOCK + t * BLOCK + r;
+        const bool real = row < q.n * p.per;
+        const int tok = row / p.per, qh = head * p.per + row % p.per;
+        const int pos = q.len - q.asked + tok;
+        const int vhi = !real ? 0 : p.causal ? min(q.len, pos + 1) : q.len, vlo = p.window > 0 ? pos + 1 - p.window : 0;
+        float a;                                // scores to units of log2
+        {
+            const T* src = (const T*)p.q + (int64_t)(q.start + tok) * p.q_ts + (int64_t)qh * p.q_hs;
+            uint32_t raw[D / 2];
+            if (real && p.q_vec) {
+#pragma unroll
+                for (int i = 0; i < D / 8; i++) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+                    raw[4 * i] = v.x; raw[4 * i + 1] = v.y; raw[4 * i + 2] = v.z; raw[4 * i + 3] = v.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < D / 2; i++)
+                    raw[i] = real ? (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(src) + 2 * i) |
+                                        ((uint32_t)__ldg(reinterpret_cast<const unsigned short*>(src) + 2 * i + 1) << 16) : 0u;
+            }
+            const auto value = [&](int e) {
+                const unsigned short h = (unsigned short)(raw[e >> 1] >> (16 * (e & 1)));
+                if constexpr (Elem<T>::kDtype == OXQ_BF16) return __uint_as_float((uint32_t)h << 16);
+                else return __half2float(__ushort_as_half(h));
+            };
+            float top = 0.0f;
+#pragma unroll
+            for (int e = 0; e < D; e++) top = fmaxf(top, fabsf(value(e)));
+            const int ex = max((int)(__float_as_uint(top) >> 23) - 127, -100);
+            // a negative scale goes into the sign of the queries, a zero one into their magnitude, so that a > 0 below
+            const float up = p.scale_log2 == 0.0f ? 0.0f : copysignf(pow2_of(max(11 - ex, -126)), p.scale_log2);
+            a = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2) * pow2_of(min(ex - 11 + 1, 127));       // + 1: the keys are halved
+            unsigned char* dst = smem + L::Q + t * L::OPERAND + r * 128;
+#pragma unroll
+            for (int i = 0; i < D / 8; i++) {
+                uint4 o;
+                o.x = pack2(value(8 * i) * up, value(8 * i + 4) * up); o.y = pack2(value(8 * i + 1) * up, value(8 * i + 5) * up);
+                o.z = pack2(value(8 * i + 2) * up, value(8 * i + 6) * up); o.w = pack2(value(8 * i + 3) * up, value(8 * i + 7) * up);
+                *reinterpret_cast<uint4*>(dst + (i >> 3) * ATOM + (((i & 7) ^ (r & 7)) << 4)) = o;
+            }
+            fence_proxy_async();
+            mbar_arrive(bar(BAR_Q));
+        }
+        // keys that every row of this warp sees need no mask
+        const int all_hi = __reduce_min_sync(0xffffffffu, real ? vhi : INT32_MAX), all_lo = __reduce_max_sync(0xffffffffu, real ? vlo : 0);
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s_col = tmem + t * BLOCK + lanes, o_col = tmem + 256 + t * BLOCK + lanes;
+        float M = -1e30f, l = 0.0f;
+        bool ok = true;
+        for (int i = 0; i < n; i++) {
+            ok = mbar_wait_warp(bar(BAR_S + t), i & 1);
+            if (!ok) { if (lane == 0) fail(); break; }
+            tc_fence_after();
+            const int t0 = (walk.first + i) * BLOCK;
+            const uint32_t* valid = reinterpret_cast<const uint32_t*>(smem + L::VALID + (i & 3) * 8);
+            const uint32_t v0 = valid[0], v1 = valid[1];
+            const bool masked = t0 < all_lo || t0 + BLOCK > all_hi || (v0 & v1) != 0x01010101u;
+#pragma unroll
+            for (int ch = 0; ch < 4; ch++) {
+                uint32_t s[32];
+                tmem_ld_32x32b_x32(s_col + 32 * ch, s);
+                tmem_ld_wait();
+                if (masked) {
+                    const uint32_t vw = ch < 2 ? v0 : v1;
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        const int key = t0 + 32 * ch + e;
+                        const bool have = (vw >> (8 * ((ch & 1) * 2 + (e >> 4)))) & 1u;
+                        if (key < vlo || key >= vhi || !have) s[e] = 0xFF800000u;
+                    }
+                }
+                float top = __uint_as_float(s[0]);
+#pragma unroll
+                for (int e = 1; e < 32; e++) top = fmaxf(top, __uint_as_float(s[e]));
+                top *= a;
+                const bool over = top > M + 8.0f;
+                if (__any_sync(0xffffffffu, over)) {
+                    // the reference moves: what was summed so far shrinks with it -- l, O (the last product into it is complete:
+                    // it was issued before these scores), and the part of this tile's P that is already written
+                    const float to = over ? top : M, f = exp2_approx(M - to);
+                    M = to;
+                    l *= f;
+                    if (i > 0) {
+#pragma unroll 1
+                        for (int c0 = 0; c0 < D; c0 += 16) {
+                            uint32_t o[16];
+                            tmem_ld_32x32b_x16(o_col + c0, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st_32x32b_x16(o_col + c0, o);
+                        }
+                    }
+#pragma unroll 1
+                    for (int c0 = 0; c0 < ch; c0++) {
+                        uint32_t o[16];
+                        tmem_st_wait();
+                        tmem_ld_32x32b_x16(s_col + 16 * c0, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[e] = pack2(lower(o[e]) * f, upper(o[e]) * f);
+                        tmem_st_32x32b_x16(s_col + 16 * c0, o);
+                    }
+                }
+                uint32_t o[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const float x = exp2_approx(fmaf(__uint_as_float(s[2 * e]), a, -M)), y = exp2_approx(fmaf(__uint_as_float(s[2 * e + 1]), a, -M));
+                    l += x + y;
+                    o[e] = pack2(x, y);
+                }
+                tmem_st_32x32b_x16(s_col + 16 * ch, o);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(bar(BAR_P + t));
+        }
+        if (ok && n > 0) {
+            ok = mbar_wait_warp(bar(BAR_S + t), n & 1);         // the last product into O
+            if (!ok && lane == 0) fail();
+            tc_fence_after();
+        }
+        if (ok) {
+            float* slot = p.parts > 1 ? p.ws + ((int64_t)blockIdx.x * p.parts + part) * (2 * BLOCK * (D + 2)) : nullptr;
+            const float inv = l > 0.0f ? 2.0f / l : l != l ? l : 0.0f;                                    // 2: the values are halved
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 32) {
+                uint32_t o[32];
+                if (n > 0) {
+                    tmem_ld_32x32b_x32(o_col + c0, o);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0;
+                }
+                constexpr int kAt[8] = {0, 2, 4, 6, 1, 3, 5, 7};                                          // column of element e
+                if (real) {
+                    if (slot) {
+                        float* dst = slot + (t * BLOCK + r) * D + c0;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<float4*>(dst + e) = make_float4(
+                                2.0f * __uint_as_float(o[(e & ~7) + kAt[e & 7]]), 2.0f * __uint_as_float(o[(e & ~7) + kAt[(e & 7) + 1]]),
+                                2.0f * __uint_as_float(o[(e & ~7) + kAt[(e & 7) + 2]]), 2.0f * __uint_as_float(o[(e & ~7) + kAt[(e & 7) + 3]]));
+                        if (c0 == 0) { slot[2 * BLOCK * D + t * BLOCK + r] = M; slot[2 * BLOCK * (D + 1) + t * BLOCK + r] = l; }
+                    } else {
+                        T* dst = (T*)p.out + (int64_t)(q.start + tok) * p.o_ts + (int64_t)qh * p.o_hs + c0;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            struct alignas(16) Eight { T v[8]; } w;
+#pragma unroll
+                            for (int k = 0; k < 8; k++) w.v[k] = Elem<T>::from_f32(l > 0.0f || l != l ? __uint_as_float(o[e + kAt[k]]) * inv : 0.0f);
+                            const uint4 u = *reinterpret_cast<const uint4*>(&w);
+                            if (p.out_vec) *reinterpret_cast<uint4*>(dst + e) = u;
+                            else {
+                                uint32_t* d4 = reinterpret_cast<uint32_t*>(dst + e);
+                                d4[0] = u.x; d4[1] = u.y; d4[2] = u.z; d4[3] = u.w;
+                            }
+                        }
+                        if (c0 == 0 && p.lse)
+                            p.lse[(int64_t)(q.start + tok) * p.q_heads + qh] = l > 0.0f || l != l ? (M + log2f(l)) * 0.693147180559945309417f : -INFINITY;
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp < 12) {
+        // ------------------------------------------------------------------------------------ codes to f16 tiles
+        constexpr int Q16 = D / 32;                                 // 16-byte pieces of a row
+        constexpr int ROUNDS = BLOCK * Q16 / 128, PER_ROUND = 128 / Q16;
+        const int pt = tid - 256, piece = pt % Q16, tok0 = pt / Q16;
+        const int32_t* table = p.s.table + (int64_t)it.b * p.s.width;
+        struct Raw { uint4 k[ROUNDS], v[ROUNDS]; uint32_t kp[ROUNDS][NG], vp[ROUNDS][NG]; } raw;
+        int page[ROUNDS];
+        const auto get_pages = [&](int i) {
+#pragma unroll
+            for (int u = 0; u < ROUNDS; u++) {
+                const int key = (walk.first + i) * BLOCK + tok0 + u * PER_ROUND;
+                page[u] = i < n && key < q.len ? __ldg(table + (key >> p.c.page_shift)) : -1;
+            }
+        };
+        // loads tile i; a key without a page of the pool counts as absent, one behind the end is masked by its position
+        const auto load = [&](int i) {
+            if (i >= n) return;
+#pragma unroll
+            for (int u = 0; u < ROUNDS; u++) {
+                const int key = (walk.first + i) * BLOCK + tok0 + u * PER_ROUND;
+                raw.k[u] = make_uint4(0, 0, 0, 0); raw.v[u] = raw.k[u];
+#pragma unroll
+                for (int g = 0; g < NG; g++) { raw.kp[u][g] = 0; raw.vp[u][g] = 0; }
+                bool good = key < q.len;
+                if (good && (page[u] < 0 || page[u] >= p.c.pages)) { good = false; if (piece == 0) *p.status = OXQ_ERR_INVALID_ARGUMENT; }
+                if (good) {
+                    const int64_t row = (((int64_t)page[u] * p.c.heads + head) << p.c.page_shift) + (key & ((1 << p.c.page_shift) - 1));
+                    raw.k[u] = __ldg(reinterpret_cast<const uint4*>(p.c.kc + row * (D / 2)) + piece);
+                    raw.v[u] = __ldg(reinterpret_cast<const uint4*>(p.c.vc + row * (D / 2)) + piece);
+#pragma unroll
+                    for (int g = 0; g < NG; g++) { raw.kp[u][g] = __ldg(p.c.kp + row * NG + g); raw.vp[u][g] = __ldg(p.c.vp + row * NG + g); }
+                }
+            }
+        };
+        const auto put = [&](uint32_t tile, bool keys) {
+#pragma unroll
+            for (int u = 0; u < ROUNDS; u++) {
+                const int tok = tok0 + u * PER_ROUND;
+                const uint4 w4 = keys ? raw.k[u] : raw.v[u];
+                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                __half2 s[NG], m[NG];
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const __half2 sm = __hmul2(as_half2(keys ? raw.kp[u][g] : raw.vp[u][g]), as_half2(0x38003800u));        // halved
+                    s[g] = __low2half2(sm); m[g] = __high2half2(sm);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    constexpr int KI = D / 32, VI = D / 64;
+                    // place 4 * piece + i of the row -> its word; with 16 bytes a piece, i alone decides which group it is in
+                    const int c = keys ? (4 * piece + i) / KI : (4 * piece + i) / VI, b = keys ? (4 * piece + i) % KI : (4 * piece + i) % VI;
+                    const int word = keys ? 4 * b + c : 8 * b + c;
+                    const int g = NG == 1 ? 0 : keys ? (i % KI) / (KI / NG) : i % VI;
+                    const uint32_t at = tile + (word >> 3) * ATOM + tok * 128 + (((word & 7) ^ (tok & 7)) << 4);
+                    const uint4 o = expand(w[i], s[g], m[g]);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(o.x), "r"(o.y), "r"(o.z), "r"(o.w) : "memory");
+                }
+            }
+        };
+        get_pages(0);
+        load(0);
+        for (int i = 0; i < n; i++) {
+            const int st = i & 1;
+            const uint32_t ph = (i >> 1) & 1;
+            bool gone[ROUNDS];
+#pragma unroll
+            for (int u = 0; u < ROUNDS; u++) {
+                const int key = (walk.first + i) * BLOCK + tok0 + u * PER_ROUND;
+                gone[u] = key < q.len && (page[u] < 0 || page[u] >= p.c.pages);
+            }
+            if (!mbar_wait_warp(bar(BAR_KEMPTY + st), ph ^ 1)) { if (lane == 0) fail(); break; }
+            put(base + L::K + st * L::OPERAND, true);
+#pragma unroll
+            for (int u = 0; u < ROUNDS; u++) {
+                const int tok = tok0 + u * PER_ROUND;
+                if (piece == 0 && (tok & 15) == 0) smem[L::VALID + (i & 3) * 8 + (tok >> 4)] = gone[u] ? 0 : 1;
+            }
+            fence_proxy_async();
+            mbar_arrive(bar(BAR_KFULL + st));
+            if (!mbar_wait_warp(bar(BAR_VEMPTY + st), ph ^ 1)) { if (lane == 0) fail(); break; }
+            put(base + L::V + st * L::OPERAND, false);
+            fence_proxy_async();
+            mbar_arrive(bar(BAR_VFULL + st));
+            get_pages(i + 1);
+            load(i + 1);
+        }
+    } else {
+        // ------------------------------------------------------------------------------------ products (whole warp, one lane issues)
+        constexpr uint32_t id_s = idesc_dense(1, 0, 0, BLOCK, BLOCK), id_o = idesc_dense(1, 0, 0, BLOCK, D) | idesc_majors(0, 1);
+        const auto scores = [&](int t, int st) {
+            const uint32_t qa = base + L::Q + t * L::OPERAND, ka = base + L::K + st * L::OPERAND;
+#pragma unroll
+            for (int at = 0; at < NA; at++) {
+                const uint64_t ad = smem_desc_sw128(qa + at * ATOM), bd = smem_desc_sw128(ka + at * ATOM);
+#pragma unroll
+                for (int kk = 0; kk < 4; kk++) mma_f16(tmem + t * BLOCK, ad + kk * 2, bd + kk * 2, id_s, (at | kk) != 0);
+            }
+        };
+        const auto sums = [&](int t, int st, bool more) {
+            const uint64_t bd = smem_desc_mn_sw128(base + L::V + st * L::OPERAND, ATOM);
+#pragma unroll
+            for (int kk = 0; kk < BLOCK / 16; kk++) mma_f16_ts(tmem + 256 + t * BLOCK, tmem + t * BLOCK + kk * 8, bd + kk * 128, id_o, more || kk != 0);
+        };
+        bool ok = true;
+        if (n > 0) {
+            ok = mbar_wait_warp(bar(BAR_Q), 0) && mbar_wait_warp(bar(BAR_KFULL), 0);
+            if (!ok && lane == 0) fail();
+            if (ok) {
+                tc_fence_after();
+                if (elect_one()) {
+                    scores(0, 0); tc_commit(bar(BAR_S));
+                    scores(1, 0); tc_commit(bar(BAR_S + 1));
+                    tc_commit(bar(BAR_KEMPTY));
+                }
+                __syncwarp();
+            }
+        }
+        for (int i = 0; i < n && ok; i++) {
+            const int st = i & 1, nx = (i + 1) & 1;
+            ok = mbar_wait_warp(bar(BAR_VFULL + st), (i >> 1) & 1) && mbar_wait_warp(bar(BAR_P), i & 1);
+            if (ok && i + 1 < n) ok = mbar_wait_warp(bar(BAR_KFULL + nx), ((i + 1) >> 1) & 1);
+            if (!ok) { if (lane == 0) fail(); break; }
+            tc_fence_after();
+            if (elect_one()) {
+                sums(0, st, i > 0);
+                if (i + 1 < n) scores(0, nx);
+                tc_commit(bar(BAR_S));
+            }
+            __syncwarp();
+            ok = mbar_wait_warp(bar(BAR_P + 1), i & 1);
+            if (!ok) { if (lane == 0) fail(); break; }
+            tc_fence_after();
+            if (elect_one()) {
+                sums(1, st, i > 0);
+                if (i + 1 < n) scores(1, nx);
+                tc_commit(bar(BAR_S + 1));
+                tc_commit(bar(BAR_VEMPTY + st));
+                if (i + 1 < n) tc_commit(bar(BAR_KEMPTY + nx));
+            }
+            __syncwarp();
+        }
+        if (!ok) {
+            // Something did not arrive.  What was issued still has to end, with a limit, before tensor memory is given back.
+            if (elect_one()) tc_commit(bar(BAR_END));
+            __syncwarp();
+            mbar_wait_warp(bar(BAR_END), 0);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the parts of an item: block (item and head, eight or sixteen rows), D / 4 threads a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_tiles_join_kernel(AttnParams p) {
+    pdl_trigger();
+    pdl_wait();
+    TileItem it;
+    const int head = blockIdx.x % p.c.heads;
+    if (!find_pair(p, blockIdx.x / p.c.heads, it)) return;
+    const int r = blockIdx.y * (256 / (D / 4)) + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+    const int row = it.pair * 2 * BLOCK + r;
+    if (row >= it.q.n * p.per) return;
+    const float* slot = p.ws + (int64_t)blockIdx.x * p.parts * (2 * BLOCK * (D + 2));
+    float top = -1e30f, sum = 0.0f;
+    for (int k = 0; k < p.parts; k++) top = fmaxf(top, slot[(int64_t)k * (2 * BLOCK * (D + 2)) + 2 * BLOCK * D + r]);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int k = 0; k < p.parts; k++) {
+        const float* s = slot + (int64_t)k * (2 * BLOCK * (D + 2));
+        const float f = exp2_approx(s[2 * BLOCK * D + r] - top);
+        const float4 v = *reinterpret_cast<const float4*>(s + r * D + d);
+        sum = fmaf(s[2 * BLOCK * (D + 1) + r], f, sum);
+        o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+    }
+    store_row<T>(p, it.q, head, row, d, make_float2(o.x, o.y), top, sum);
+    store_row<T>(p, it.q, head, row, d + 2, make_float2(o.z, o.w), top, sum);
+}
+
+}  // namespace kv4
+}  // namespace oxq
+
+using namespace oxq;
+using namespace oxq::kv4;
+
+template <typename T, int D, int NG>
+static int32_t launch_tiles(oxq_handle* h, const AttnParams& p, int64_t items) {
+    auto kernel = kv4_attn_tiles_kernel<T, D, NG>;
+    constexpr int bytes = TileSmem<D>::BYTES < 120 * 1024 ? 120 * 1024 : TileSmem<D>::BYTES;      // one CTA per SM: each takes all of tensor memory
+    static OxqPerDevice ready;
+    if (!ready.get(h->device)) {
+        OXQ_CUDA(h, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        ready.set(h->device, 1);
+    }
+    const dim3 grid((unsigned)(items * p.c.heads), (unsigned)p.parts);
+    OXQ_CUDA(h, oxq_launch(kernel, grid, 416, bytes, h->stream, p));
+    if (p.parts > 1) OXQ_CUDA(h, oxq_launch(kv4_tiles_join_kernel<T, D>, dim3(grid.x, 2 * BLOCK / (256 / (D / 4))), 256, 0, h->stream, p));
+    return OXQ_OK;
+}
+
+int64_t oxq_kv4_tiles_slot_bytes(int dim) { return (int64_t)2 * BLOCK * (dim + 2) * (int64_t)sizeof(float); }
+
+int32_t oxq_kv4_tiles_launch(oxq_handle* h, const oxq_kv4_cache* cc, const AttnParams& p, int dtype, int64_t items) {
+    if (dtype == OXQ_BF16) {
+        if (cc->dim == 64) return launch_tiles<__nv_bfloat16, 64, 1>(h, p, items);
+        if (cc->group == 64) return launch_tiles<__nv_bfloat16, 128, 2>(h, p, items);
+        return launch_tiles<__nv_bfloat16, 128, 1>(h, p, items);
+    }
+    if (cc->dim == 64) return launch_tiles<__half, 64, 1>(h, p, items);
+    if (cc->group == 64) return launch_tiles<__half, 128, 2>(h, p, items);
+    return launch_tiles<__half, 128, 1>(h, p, items);
+}

@@ -787,10 +787,12 @@ def kv4_read(cache: Kv4Cache, block_table: torch.Tensor, seq_lens: torch.Tensor,
     return outs[0], outs[1]
 
 
-def kv4_attention_workspace_bytes(cache: Kv4Cache, max_rows: int) -> int:
-    """Bytes of workspace for kv4_attention; max_rows = max_tokens * q_heads / heads."""
+def kv4_attention_workspace_bytes(cache: Kv4Cache, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_tokens: torch.Tensor, tokens: int, q_heads: int,
+                                  max_tokens: int = 0) -> int:
+    """Bytes of workspace that kv4_attention needs for `tokens` rows of q_heads heads; depends on the arguments' shapes only, not on their contents."""
+    batch = _kv4_batch(cache, block_table, seq_lens, cu_tokens, tokens)
     n = C.c_size_t(0)
-    handle(cache.device.index).call("oxq_kv4_attention_workspace_bytes", cache.dim, max_rows, C.byref(n))
+    handle(cache.device.index).call("oxq_kv4_attention_workspace_bytes", C.byref(cache._desc), C.byref(batch), q_heads, max_tokens, C.byref(n))
     return n.value
 
 
@@ -822,8 +824,9 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, block_table: torch.Tensor, s
     batch = _kv4_batch(cache, block_table, seq_lens, cu_tokens, tokens)
     h = handle(cache.device.index)
     if workspace is None:
-        most = tokens if max_tokens <= 0 else min(tokens, max_tokens)
-        workspace = torch.empty(max(kv4_attention_workspace_bytes(cache, most * (heads // cache.heads)), 16), dtype=torch.uint8, device=q.device)
+        n = C.c_size_t(0)
+        h.call("oxq_kv4_attention_workspace_bytes", C.byref(cache._desc), C.byref(batch), heads, max_tokens, C.byref(n))
+        workspace = torch.empty(max(n.value, 16), dtype=torch.uint8, device=q.device)
     else:
         _chk(workspace, torch.uint8)
         if workspace.device != q.device:

@@ -271,7 +271,8 @@ def check(c, q, out, lse, scale, causal, window, drop=None):
 
 
 def many_rows(c, q):
-    return False
+    """Whether some sequence may have gone to the kernel for many query rows."""
+    return c.tokens * (q.shape[1] // c.heads) > 64
 
 
 def attend(c, q, scale=None, causal=True, window=0, max_tokens=None, **kw):
@@ -321,6 +322,108 @@ def test_groups_of_query_heads(per, new, page):
     q = c.normal(c.tokens, 2 * per, 128, dtype=torch.bfloat16)
     out, lse = attend(c, q, scale=0.2)
     check(c, q, out, lse, 0.2, True, 0)
+
+
+@pytest.mark.parametrize("dim,group", DIMS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("per,page,lens,new,causal,window", [
+    (1, 16, [300], [300], True, 0), (4, 64, [129], [128], True, 0), (4, 32, [1000, 70], [257, 70], True, 0), (3, 16, [500, 64, 333], [87, 64, 130], True, 0),
+    (4, 64, [700], [300], True, 1), (4, 64, [700], [300], True, 130), (8, 128, [400], [33], False, 0), (2, 64, [40], [100], True, 0),
+    (5, 64, [0, 200], [30, 40], True, 0), (16, 64, [260], [260], True, 300)])
+def test_prompts(dim, group, dtype, per, page, lens, new, causal, window):
+    """Many rows a kv head: blocks and tiles that end inside, windows, rows that see nothing, a sequence without keys."""
+    c = Case(lens, new, 2, dim, group, page, seed=per + page, pad_tokens=2)
+    c.fill()
+    q = c.normal(c.tokens, 2 * per, dim, dtype=DT[dtype])
+    out, lse = attend(c, q, causal=causal, window=window, out=torch.full_like(q, 3.0))
+    check(c, q, out, lse, dim ** -0.5, causal, window)
+    assert (out[c.cu_l[-1]:] == 3.0).all()
+    again, _ = attend(c, q, causal=causal, window=window, out=torch.full_like(q, 3.0))
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("scale", [0.3, -0.1, 0.0])
+@pytest.mark.parametrize("rows", [3, 90])
+def test_scales_of_either_sign(scale, rows):
+    c = Case([200], [rows], 1, 128, 64, 16)
+    c.fill()
+    q = c.normal(rows, 1, 128, dtype=torch.bfloat16)
+    out, lse = attend(c, q, scale=scale)
+    check(c, q, out, lse, scale, True, 0)
+
+
+def test_a_mixed_batch():
+    """Single tokens, short runs and prompts together: each sequence goes to the kernel for its number of rows."""
+    new = [1, 200, 0, 3, 16, 17, 1, 90]
+    lens = [900, 200, 50, 3, 1000, 400, 1, 2000]
+    c = Case(lens, new, 2, 128, 64, 32)
+    c.fill()
+    for dt in ("bf16", "f16"):
+        q = c.normal(c.tokens, 8, 128, dtype=DT[dt])
+        out, lse = attend(c, q)
+        check(c, q, out, lse, 128 ** -0.5, True, 0)
+
+
+@pytest.mark.parametrize("heads,per,lens,new", [(1, 4, [9000], [20]), (2, 4, [5000, 3000], [80, 40]), (1, 1, [20000], [100])])
+@pytest.mark.parametrize("dim,group", DIMS)
+def test_few_blocks_share_their_keys(heads, per, lens, new, dim, group):
+    c = Case(lens, new, heads, dim, group, 64)
+    c.fill()
+    q = c.normal(c.tokens, heads * per, dim, dtype=torch.bfloat16)
+    for causal in (True, False):
+        out, lse = attend(c, q, causal=causal)
+        check(c, q, out, lse, dim ** -0.5, causal, 0)
+
+
+def test_large_scores_in_prompts():
+    """The reference moves in the middle of a tile and between tiles, by more than f16 could hold."""
+    c = Case([700], [150], 2, 128, 64, 16, seed=9)
+    c.fill()
+    c.cache.k_params.mul_(6)
+    c.cache.v_params.mul_(torch.exp2(torch.randint(-6, 7, c.cache.v_params.shape[:3], device="cuda", generator=c.g).float()).half()[..., None, None])
+    q = (c.normal(c.tokens, 4, 128) * 4).bfloat16()
+    out, lse = attend(c, q)
+    check(c, q, out, lse, 128 ** -0.5, True, 0)
+
+
+def test_the_largest_values_in_prompts():
+    """Values at the ends of f16's range do not overflow on their way into the products."""
+    from oxicuda_b200 import ops
+    c = Case([200], [200], 1, 128, 64, 16)
+    x = torch.where(c.normal(200, 2, 128) > 0, 65504.0, -65504.0)
+    ops.kv4_append(c.cache, x[:, :1], x[:, 1:], c.table, c.lens, c.cu)
+    q = c.normal(200, 1, 128, dtype=torch.bfloat16) * 1e-4
+    out, lse = attend(c, q)
+    check(c, q, out, lse, 128 ** -0.5, True, 0)
+
+
+def test_rows_with_nan_or_infinite_queries_spoil_themselves_only():
+    for new in (3, 100):
+        c = Case([300], [new], 1, 128, 64, 16)
+        c.fill()
+        q = c.normal(new, 4, 128, dtype=torch.bfloat16)
+        good, _ = attend(c, q)
+        good = good.clone()
+        q[1, 2, 7], q[2, 0, 100] = float("nan"), float("inf")
+        out, _ = attend(c, q)
+        keep = torch.ones(new, 4, dtype=torch.bool, device="cuda")
+        keep[1, 2], keep[2, 0] = False, False
+        assert torch.equal(out[keep], good[keep]) and out[1, 2].isnan().all() and out[2, 0].isnan().all()
+
+
+def test_pages_that_the_table_does_not_give_in_prompts():
+    from oxicuda_b200 import ops
+    c = Case([400, 100], [150, 100], 2, 128, 64, 16)
+    c.fill()
+    drop = [torch.zeros(500, dtype=torch.bool, device="cuda") for _ in range(2)]
+    good = c.table.clone()
+    c.table[0, 2], c.table[0, 20], c.table[1, 0] = c.pages, -1, 1 << 30
+    drop[0][32:48], drop[0][320:336], drop[1][0:16] = True, True, True
+    q = c.normal(c.tokens, 4, 128, dtype=torch.bfloat16)
+    out, lse = attend(c, q)
+    assert ops.handle().device_status() == 15
+    c.table = good
+    check(c, q, out, lse, 128 ** -0.5, True, 0, drop)
 
 
 @pytest.mark.parametrize("heads,lens", [(1, [70001]), (2, [30000, 1, 9, 20011]), (8, [4097] * 3)])

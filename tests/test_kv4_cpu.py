@@ -93,10 +93,10 @@ def test_attention_window_and_workspace(lib, fake):
     assert lib.oxq_kv4_attention(fake, C.byref(c), C.byref(b), C.byref(a), 0x10008, 1 << 30) == 11
     assert lib.oxq_kv4_attention(fake, C.byref(c), C.byref(b), None, 0x10000, 1 << 30) == 15
     n = C.c_size_t(0)
-    assert lib.oxq_kv4_attention_workspace_bytes(fake, 96, 8, C.byref(n)) == 13
-    assert lib.oxq_kv4_attention_workspace_bytes(fake, 128, -1, C.byref(n)) == 10
-    assert lib.oxq_kv4_attention_workspace_bytes(fake, 128, 8, None) == 15
-    assert lib.oxq_kv4_attention_workspace_bytes(fake, 128, 8, C.byref(n)) == 0
+    size = lambda c, b, heads, most, out=C.byref(n): lib.oxq_kv4_attention_workspace_bytes(fake, C.byref(c), C.byref(b), heads, most, out)  # noqa: E731
+    assert size(c, b, 7, 0) == 12 and size(c, b, 8, -1) == 10 and size(c, b, 8, 0, None) == 15
+    assert size(_descs(dim=96)[0], b, 8, 0) == 13
+    assert size(c, b, 8, 0) == 0
 
 
 def test_residual_norm(lib, fake):
