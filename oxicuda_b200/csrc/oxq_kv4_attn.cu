@@ -15,16 +15,19 @@
 //
 // The shape.  mma.sync m16n8k16 with the keys as the 16 rows and 8 query rows as the columns (a kv head's query heads, and
 // the tokens of a run): S^T = K Q^T, then O^T = V^T P^T; P^T moves from accumulator to operand layout by movmatrix.
-// Eight warps of a CTA take 16 keys each of a tile of 128; all tiles of all (sequence, kv head, block of query rows) items
-// lie on one line, which the CTAs cut into equal parts (lengths are known on the device only).  An item that lies inside
-// one part is finished there; of a cut one every CTA leaves o, M and l in the workspace and a second kernel joins them, in
-// the order of the keys, so results do not depend on timing.
+// Eight warps of a CTA take 16 keys each of a tile of 128; bulk copies bring the tiles into a ring in shared memory, LEAD of
+// them ahead, issued by the warps in turn (a warp for nothing else would cost the others a quarter of their registers).  All tiles of all (sequence, kv head, block of query rows) items lie on one line, which the
+// CTAs cut into equal parts (lengths are known on the device only).  An item that lies inside one part is finished there; of a
+// cut one every CTA leaves o, M and l in the workspace and a second kernel joins them, in the order of the keys, so
+// results do not depend on timing.
 #include "oxq_kv4_attn.cuh"
+#include "oxq_tc.cuh"
 
 namespace oxq {
 namespace kv4 {
 
 constexpr int TILE = 128;               // keys per tile: 8 warps x 16
+constexpr int MIN_TILES = 2;            // tiles a CTA takes at least: a join of many small parts costs more than it brings
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -43,11 +46,30 @@ __device__ __forceinline__ float lo_f32(uint32_t v) { return __half2float(__usho
 __device__ __forceinline__ float hi_f32(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
 // floor(log2(s)) of a non-negative f16 number as a float, not below -24 (the smallest s there is; also for s = 0)
 __device__ __forceinline__ float log2_floor(float s) { return fmaxf((float)((int)(__float_as_uint(s) >> 23) - 127), -24.0f); }
-template <int N> __device__ __forceinline__ void load_words(uint32_t (&r)[N], const void* p) {
-    if constexpr (N == 4) { const uint4 v = __ldg(reinterpret_cast<const uint4*>(p)); r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
-    else if constexpr (N == 2) { const uint2 v = __ldg(reinterpret_cast<const uint2*>(p)); r[0] = v.x; r[1] = v.y; }
-    else r[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+template <int N> __device__ __forceinline__ void lds_words(uint32_t (&r)[N], const unsigned char* p) {
+    if constexpr (N == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p); r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
+    else if constexpr (N == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p); r[0] = v.x; r[1] = v.y; }
+    else r[0] = *reinterpret_cast<const uint32_t*>(p);
 }
+// two f32 operations in one instruction
+__device__ __forceinline__ uint64_t pair_bits(float2 v) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y)); return r; }
+__device__ __forceinline__ float2 bits_pair(uint64_t b) { float2 v; asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(b)); return v; }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+    return bits_pair(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+    return bits_pair(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+    return bits_pair(r);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // The tiles of all items of one sequence, and of one item (row block rt).
 struct Span { int first, tiles; int lo, hi; };          // first tile, how many (at least one), visible positions [lo, hi)
@@ -74,48 +96,58 @@ __device__ __forceinline__ SeqInfo small_seq(const AttnParams& p, int b) {
     return q;
 }
 
+// The line of tiles, cut into `parts` parts that differ by one tile at most.
+struct Line {
+    int64_t total, each; int parts, more;
+    __device__ __forceinline__ int64_t bound(int64_t k) const { return each * k + (k < more ? k : more); }
+};
 struct Where { int b; int64_t at; };    // sequence, and the line's position of its first tile
-// Sum of all sequences' tiles; every thread of the CTA gets it.  256 threads.
-__device__ __forceinline__ int64_t total_tiles(const AttnParams& p, int nr, int64_t* red) {
-    int64_t t = 0;
-    for (int b = threadIdx.x; b < p.s.seqs; b += 256) t += head_tiles(p, small_seq(p, b), nr) * p.c.heads;
+
+// Scan over 256 sequences from b0 on: tiles of this thread's one, and how many lie before it (from `base`); base moves on.
+// Whole CTA (its first 256 threads hold the sequences).
+__device__ __forceinline__ int64_t scan_tiles(const AttnParams& p, int nr, int b0, int64_t* red, int64_t& base, int64_t& mine) {
+    const int b = b0 + threadIdx.x;
+    mine = (int)threadIdx.x < 256 && b < p.s.seqs ? head_tiles(p, small_seq(p, b), nr) * p.c.heads : 0;
+    int64_t x = mine;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = t;
-    __syncthreads();
-    t = 0;
-#pragma unroll
-    for (int w = 0; w < 8; w++) t += red[w];
-    __syncthreads();
-    return t;
-}
-// The sequence that holds tile `want` of the line (want < total).
-__device__ __forceinline__ Where find_tile(const AttnParams& p, int nr, int64_t want, int64_t* red, Where* found) {
-    int64_t base = 0;
-    for (int b0 = 0; b0 < p.s.seqs; b0 += 256) {
-        const int b = b0 + threadIdx.x;
-        const int64_t mine = b < p.s.seqs ? head_tiles(p, small_seq(p, b), nr) * p.c.heads : 0;
-        int64_t x = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-            if ((threadIdx.x & 31) >= o) x += y;
-        }
-        if ((threadIdx.x & 31) == 31) red[threadIdx.x >> 5] = x;
-        __syncthreads();
-        int64_t before = base, all = base;
-#pragma unroll
-        for (int w = 0; w < 8; w++) {
-            if (w < (int)(threadIdx.x >> 5)) before += red[w];
-            all += red[w];
-        }
-        const int64_t start = before + x - mine;
-        if (mine > 0 && start <= want && want < start + mine) { found->b = b; found->at = start; }
-        __syncthreads();
-        base = all;
-        if (want < base) break;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if ((threadIdx.x & 31) >= o) x += y;
     }
-    return *found;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 31 && threadIdx.x < 256) red[threadIdx.x >> 5] = x;
+    __syncthreads();
+    int64_t before = base;
+#pragma unroll
+    for (int w = 0; w < 8; w++) {
+        if (w < (int)(threadIdx.x >> 5)) before += red[w];
+        base += red[w];
+    }
+    return before + x - mine;
+}
+// The line, and the sequence that holds tile bound(k), if k < parts.
+__device__ __forceinline__ Line find_part(const AttnParams& p, int nr, int ctas, int k, int64_t* red, Where* found) {
+    Line line;
+    line.total = 0;
+    int64_t mine = 0, start = 0;
+    for (int b0 = 0; b0 < p.s.seqs; b0 += 256) start = scan_tiles(p, nr, b0, red, line.total, mine);
+    const int64_t most = (line.total + MIN_TILES - 1) / MIN_TILES;
+    line.parts = (int)(most < ctas ? most : ctas);
+    line.each = line.parts ? line.total / line.parts : 0;
+    line.more = (int)(line.total - line.each * line.parts);
+    if (k >= line.parts) return line;
+    const int64_t want = line.bound(k);
+    if (p.s.seqs <= 256) {
+        if (mine > 0 && start <= want && want < start + mine) { found->b = threadIdx.x; found->at = start; }
+    } else {
+        int64_t base = 0;
+        for (int b0 = 0; b0 < p.s.seqs && base <= want; b0 += 256) {
+            start = scan_tiles(p, nr, b0, red, base, mine);
+            if (mine > 0 && start <= want && want < start + mine) { found->b = b0 + threadIdx.x; found->at = start; }
+        }
+    }
+    __syncthreads();
+    return line;
 }
 
 // An item of a sequence: which one holds tile `in_seq` of the sequence's own line.
@@ -137,48 +169,112 @@ template <int NT> struct Slot {         // what a cut item's CTA leaves: o [rows
     __host__ __device__ static constexpr int floats(int d) { return ROWS * (d + 2); }
 };
 
-template <typename T, int D, int NG, int NT>
+// Part of the tiles of one item that a CTA works on.
+struct Work {
+    Where w; SeqInfo seq; int64_t seq_tiles, at, end;
+    Item it; int ta, tb;
+    __device__ __forceinline__ bool next(const AttnParams& p, int nr) {
+        if (at >= end) return false;
+        while (at >= w.at + seq_tiles) {                              // on to the next sequence that has tiles
+            w.at += seq_tiles;
+            if (++w.b >= p.s.seqs) return false;                      // cannot happen: `end` is within the line
+            seq = small_seq(p, w.b);
+            seq_tiles = head_tiles(p, seq, nr) * p.c.heads;
+        }
+        it = find_item(p, seq, nr, at - w.at);
+        ta = (int)(at - w.at - it.start);
+        tb = (int)min((int64_t)it.span.tiles, (int64_t)ta + (end - at));
+        at += tb - ta;
+        return true;
+    }
+};
+
+// One stage of the ring: a tile's codes and params, key after key, and for each 16 keys whether they are there.
+template <int D, int NG> struct Stage {
+    static constexpr int KC = 0, VC = KC + TILE * (D / 2), KP = VC + TILE * (D / 2), VP = KP + TILE * NG * 4, BYTES = VP + TILE * NG * 4;
+};
+template <int D, int NG, int NT>
 struct Smem {
-    static constexpr int ROWS = NT * 8, QPAD = D + 8;
+    static constexpr int ROWS = NT * 8, QPAD = D + 8, STAGES = 4, LEAD = 2;
+    unsigned char ring[STAGES][Stage<D, NG>::BYTES];
     __half q[ROWS * QPAD];              // per eight elements in the order 0 4 1 5 2 6 3 7, the odd ones / 16
-    float slab[8][ROWS * (D + 8)];
+    float slab[4][ROWS * (D + 8)];
     float a[ROWS], bsum[ROWS][NG];      // scale log2(e) 2^(24 + e - 11), scale log2(e) * sum of q
     float m[8][ROWS], l[8][ROWS];
+    uint64_t bars[2 * STAGES];
+    unsigned char there[STAGES][8];
     int64_t red[8];
     Where found;
 };
 
 template <typename T, int D, int NG, int NT>
 __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(AttnParams p) {
-    constexpr bool SPLIT = sizeof(T) == 2 && Elem<T>::kDtype == OXQ_F16;
-    constexpr int ROWS = NT * 8, NB = D / 32, NS = D / 64, QPAD = D + 8, OPAD = D + 8;
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    Smem<T, D, NG, NT>& sm = *reinterpret_cast<Smem<T, D, NG, NT>*>(smem_raw);
+    using Sm = Smem<D, NG, NT>;
+    using St = Stage<D, NG>;
+    constexpr bool SPLIT = Elem<T>::kDtype == OXQ_F16;
+    constexpr int ROWS = NT * 8, NB = D / 32, NS = D / 64, QPAD = D + 8, OPAD = D + 8, STAGES = Sm::STAGES, LEAD = Sm::LEAD;
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
+    const uint32_t bars = tc::smem_u32(sm.bars);
+    const auto full = [&](int s) { return bars + 8 * s; };
+    const auto empty = [&](int s) { return bars + 8 * (STAGES + s); };
+    if (tid == 0) {
+#pragma unroll
+        for (int s = 0; s < STAGES; s++) { tc::mbar_init(full(s), 1); tc::mbar_init(empty(s), 8); }
+        tc::fence_barrier_init();
+    }
     pdl_trigger();
     pdl_wait();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
 
-    const int64_t total = total_tiles(p, ROWS, sm.red);
-    const int64_t parts = min((int64_t)gridDim.x, total);
-    if (blockIdx.x >= parts) return;
-    int64_t at = total * blockIdx.x / parts;
-    const int64_t begin = at, end = total * (blockIdx.x + 1) / parts;
-    Where w = find_tile(p, ROWS, at, sm.red, &sm.found);
-    SeqInfo seq = small_seq(p, w.b);
-    int64_t seq_tiles = head_tiles(p, seq, ROWS) * p.c.heads;
+    const Line line = find_part(p, ROWS, gridDim.x, blockIdx.x, sm.red, &sm.found);
+    if (blockIdx.x >= line.parts) return;
+    Work wk;
+    wk.at = line.bound(blockIdx.x);
+    wk.end = line.bound(blockIdx.x + 1);
+    wk.w = sm.found;
+    wk.seq = small_seq(p, wk.w.b);
+    wk.seq_tiles = head_tiles(p, wk.seq, ROWS) * p.c.heads;
+    bool ok = true;
 
-    while (at < end) {
-        while (at >= w.at + seq_tiles) {                              // on to the next sequence that has tiles
-            w.at += seq_tiles;
-            w.b++;
-            if (w.b >= p.s.seqs) return;                              // cannot happen: `end` is within the line
-            seq = small_seq(p, w.b);
-            seq_tiles = head_tiles(p, seq, ROWS) * p.c.heads;
+    // One tile of `wk` into the ring as the CTA's tile number `count`, by this warp: lane = 4 * chunk + array.
+    const auto bring = [&](int i, uint32_t count) {
+        const int chunk = min(1 << p.c.page_shift, TILE), arr = lane & 3, off = (lane >> 2) * chunk;
+        const int key = (wk.it.span.first + i) * TILE + off, slot = count % STAGES;
+        const bool wanted = off < TILE && key < wk.it.span.hi && key + chunk > wk.it.span.lo;
+        const int page = wanted ? __ldg(p.s.table + (int64_t)wk.w.b * p.s.width + (key >> p.c.page_shift)) : 0;
+        const bool good = wanted && page >= 0 && page < p.c.pages;
+        if (wanted && !good && arr == 0) *p.status = OXQ_ERR_INVALID_ARGUMENT;
+        if (ok && !tc::mbar_wait_warp(empty(slot), (count / STAGES & 1) ^ 1)) { ok = false; if (lane == 0) *p.status = OXQ_ERR_DEVICE_TIMEOUT; }
+        if (!ok) return;
+        if (arr == 0 && off < TILE)
+            for (int k = 0; k < chunk; k += 16) sm.there[slot][(off + k) >> 4] = good ? 1 : 0;
+        const int row_bytes = arr < 2 ? D / 2 : NG * 4;
+        const uint32_t bytes = good ? chunk * row_bytes : 0;
+        const uint32_t all = __reduce_add_sync(0xffffffffu, bytes);
+        __syncwarp();                                                 // what the lanes wrote goes before lane 0's arrival
+        if (lane == 0) tc::mbar_arrive_expect_tx(full(slot), all);
+        __syncwarp();
+        if (good) {
+            const unsigned char* src = arr == 0 ? p.c.kc : arr == 1 ? p.c.vc : reinterpret_cast<const unsigned char*>(arr == 2 ? p.c.kp : p.c.vp);
+            const uint32_t to = arr == 0 ? St::KC : arr == 1 ? St::VC : arr == 2 ? St::KP : St::VP;
+            const int64_t row = (((int64_t)page * p.c.heads + wk.it.head) << p.c.page_shift) + (key & ((1 << p.c.page_shift) - 1));
+            tc::bulk_load(tc::smem_u32(&sm.ring[slot][to]) + off * row_bytes, src + row * row_bytes, bytes, full(slot));
         }
-        const Item it = find_item(p, seq, ROWS, at - w.at);
-        const int ta = (int)(at - w.at - it.start);
-        const int tb = (int)min((int64_t)it.span.tiles, (int64_t)ta + (end - at));
-        const bool whole = ta == 0 && tb == it.span.tiles;
+    };
+    uint32_t count = 0;                                               // of the CTA's tiles: the next one to use
+    const auto prime = [&]() {                                        // the first tiles of a new piece of work
+        for (int i = wk.ta; i < wk.tb && i < wk.ta + LEAD; i++)
+            if ((int)((count + i - wk.ta) & 7) == warp) bring(i, count + i - wk.ta);
+    };
+
+    bool more = wk.next(p, ROWS);
+    __syncthreads();                                                  // the barriers are set up
+    if (more) prime();
+    while (more) {
+        const SeqInfo seq = wk.seq;
+        const Item it = wk.it;
+        const int ta = wk.ta, tb = wk.tb;
         const int row0 = it.rt * ROWS, rows = min(ROWS, seq.n * p.per - row0);
 
         // ---- the query rows: D / 8 threads a row
@@ -219,22 +315,15 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
         __syncthreads();
 
         // ---- this warp's constants and accumulators; columns 2 c and 2 c + 1 of each block of eight rows are this lane's
-        float qa[NT][2], qb[NT][2][NG], M[NT][2], l[NT][2], po[NT][2][NG];
-        int vlo[NT][2], vhi[NT][2];
+        float2 qa[NT], qb[NT][NG], M[NT], l[NT], po[NT][NG];
         float acc[NS * 4][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < NT; nt++) {
+            qa[nt] = make_float2(sm.a[nt * 8 + 2 * c], sm.a[nt * 8 + 2 * c + 1]);
+            M[nt] = both(-1e30f); l[nt] = both(0.0f);
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int row = nt * 8 + 2 * c + e;
-                qa[nt][e] = sm.a[row];
-                M[nt][e] = -1e30f; l[nt][e] = 0.0f;
-#pragma unroll
-                for (int g = 0; g < NG; g++) { qb[nt][e][g] = sm.bsum[row][g]; po[nt][e][g] = 0.0f; }
-                const int pos = seq.len - seq.asked + (row0 + row) / p.per;        // the row's own position
-                vhi[nt][e] = p.causal ? min(seq.len, pos + 1) : seq.len;
-                vlo[nt][e] = p.window > 0 ? pos + 1 - p.window : 0;
-            }
+            for (int g = 0; g < NG; g++) { qb[nt][g] = make_float2(sm.bsum[nt * 8 + 2 * c][g], sm.bsum[nt * 8 + 2 * c + 1][g]); po[nt][g] = both(0.0f); }
+        }
 #pragma unroll
         for (int i = 0; i < NS * 4; i++)
 #pragma unroll
@@ -245,48 +334,26 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
         const int pos0 = seq.len - seq.asked + row0 / p.per, pos1 = seq.len - seq.asked + (row0 + rows - 1) / p.per;
         const int all_hi = p.causal ? min(seq.len, pos0 + 1) : seq.len, all_lo = p.window > 0 ? pos1 + 1 - p.window : 0;
 
-        struct Keys { uint32_t k[2][NB], v[4][NS], kp[2][NG], vp[2][NG]; } cur, nxt;
-        const int32_t* table = p.s.table + (int64_t)w.b * p.s.width;
-        const auto slice = [&](int i) { return (it.span.first + i) * TILE + warp * 16; };
-        const auto wanted = [&](int i) { return i < tb && slice(i) < it.span.hi && slice(i) + 16 > it.span.lo; };
-        const auto page_of = [&](int i) -> int { return wanted(i) ? __ldg(table + (slice(i) >> p.c.page_shift)) : 0; };
-        const auto load = [&](Keys& k, int i, int page) -> bool {
-            if (!wanted(i)) return false;
-            if (page < 0 || page >= p.c.pages) { if (lane == 0) *p.status = OXQ_ERR_INVALID_ARGUMENT; return false; }
-            const int64_t row = (((int64_t)page * p.c.heads + it.head) << p.c.page_shift) + (slice(i) & ((1 << p.c.page_shift) - 1));
+        for (int i = ta; i < tb; i++, count++) {
+            if (i + LEAD < tb && (int)((count + LEAD) & 7) == warp) bring(i + LEAD, count + LEAD);
+            const int stage = count % STAGES;
+            if (ok && !tc::mbar_wait(full(stage), count / STAGES & 1)) { ok = false; *p.status = OXQ_ERR_DEVICE_TIMEOUT; }
+            __syncwarp();
+            const int t0 = (it.span.first + i) * TILE + warp * 16;
+            const unsigned char* ring = sm.ring[stage] + warp * (16 * (D / 2));
+            if (__all_sync(0xffffffffu, ok) && t0 < it.span.hi && t0 + 16 > it.span.lo && sm.there[stage][warp]) {
+                const unsigned char* kc = ring + St::KC + r * (D / 2) + c * (D / 8);
+                const unsigned char* vc = ring + St::VC + 2 * c * (D / 2) + r * (D / 16);
+                const unsigned char* pp = sm.ring[stage] + St::KP + (warp * 16 + r) * (NG * 4);
+                uint32_t k[2][NB], kp[2][NG], vp[2][NG];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                load_words(k.k[h], p.c.kc + (row + r + 8 * h) * (D / 2) + c * (D / 8));
-                load_words(k.kp[h], p.c.kp + (row + r + 8 * h) * NG);
-                load_words(k.vp[h], p.c.vp + (row + r + 8 * h) * NG);
-            }
-#pragma unroll
-            for (int h = 0; h < 4; h++) load_words(k.v[h], p.c.vc + (row + 2 * c + (h & 1) + (h >> 1) * 8) * (D / 2) + r * (D / 16));
-            return true;
-        };
-
-        bool have = load(cur, ta, page_of(ta));
-        int next_page = page_of(ta + 1);
-        for (int i = ta; i < tb; i++) {
-            const bool next_have = load(nxt, i + 1, next_page);
-            next_page = page_of(i + 2);
-            if (have) {
-                const int t0 = slice(i);
-                // ---- x = scores of keys t0 + r (elements 0, 1) and t0 + r + 8 (elements 2, 3)
-                float x[NT][4];
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[nt][e] = 0.0f;
-                const bool masked = t0 < all_lo || t0 + 16 > all_hi;
-                if (t0 + 16 > seq.len) {                              // rows behind the last key hold anything
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        if (t0 + r + 8 * h >= seq.len) {
-#pragma unroll
-                            for (int g = 0; g < NG; g++) { cur.kp[h][g] = 0; cur.vp[h][g] = 0; }
-                        }
+                for (int h = 0; h < 2; h++) {
+                    lds_words(k[h], kc + 8 * h * (D / 2));
+                    lds_words(kp[h], pp + 8 * h * (NG * 4));
+                    lds_words(vp[h], pp + (St::VP - St::KP) + 8 * h * (NG * 4));
                 }
+                // ---- x = scores of keys t0 + r (first pair) and t0 + r + 8 (second)
+                float2 x[NT][2];
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
                     float s4[NT][4];
@@ -297,7 +364,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
 #pragma unroll
                     for (int i2 = 0; i2 < NB / NG; i2++) {
                         const int blk = g * (NB / NG) + i2;
-                        const uint32_t w0 = cur.k[0][blk], w1 = cur.k[1][blk], u0 = w0 >> 8, u1 = w1 >> 8;
+                        const uint32_t w0 = k[0][blk], w1 = k[1][blk], u0 = w0 >> 8, u1 = w1 >> 8;
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             const uint4 qf = *reinterpret_cast<const uint4*>(&sm.q[(nt * 8 + r) * QPAD + blk * 32 + c * 8]);
@@ -305,90 +372,103 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                             mma_16816(s4[nt], u0 & 0x000F000Fu, u1 & 0x000F000Fu, u0 & 0x00F000F0u, u1 & 0x00F000F0u, qf.z, qf.w);
                         }
                     }
-                    const float ks0 = lo_f32(cur.kp[0][g]), km0 = hi_f32(cur.kp[0][g]), ks1 = lo_f32(cur.kp[1][g]), km1 = hi_f32(cur.kp[1][g]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        x[nt][0] = fmaf(s4[nt][0] * ks0, qa[nt][0], fmaf(km0, qb[nt][0][g], x[nt][0]));
-                        x[nt][1] = fmaf(s4[nt][1] * ks0, qa[nt][1], fmaf(km0, qb[nt][1][g], x[nt][1]));
-                        x[nt][2] = fmaf(s4[nt][2] * ks1, qa[nt][0], fmaf(km1, qb[nt][0][g], x[nt][2]));
-                        x[nt][3] = fmaf(s4[nt][3] * ks1, qa[nt][1], fmaf(km1, qb[nt][1][g], x[nt][3]));
+                    for (int h = 0; h < 2; h++) {
+                        const float ks = lo_f32(kp[h][g]), km = hi_f32(kp[h][g]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+                            x[nt][h] = fma2(mul2(make_float2(s4[nt][2 * h], s4[nt][2 * h + 1]), both(ks)), qa[nt],
+                                            g == 0 ? mul2(both(km), qb[nt][0]) : fma2(both(km), qb[nt][g], x[nt][h]));
                     }
                 }
-                if (masked) {
+                if (t0 < all_lo || t0 + 16 > all_hi) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
+                    for (int h = 0; h < 2; h++) {
+                        const int t = t0 + r + 8 * h;
+                        if (t >= seq.len)                             // rows behind the last key hold anything
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int t = t0 + r + (e >> 1) * 8;
-                            if (t < vlo[nt][e & 1] || t >= vhi[nt][e & 1]) x[nt][e] = -INFINITY;
-                        }
+                            for (int g = 0; g < NG; g++) vp[h][g] = 0;
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                const int pos = seq.len - seq.asked + (row0 + nt * 8 + 2 * c + e) / p.per;      // the row's own position
+                                const int vhi = p.causal ? min(seq.len, pos + 1) : seq.len, vlo = p.window > 0 ? pos + 1 - p.window : 0;
+                                if (t < vlo || t >= vhi) (e ? x[nt][h].y : x[nt][h].x) = -INFINITY;
+                            }
+                    }
                 }
                 // ---- the rows' reference
-                float vs[2][NG], vm[2][NG], big[2];
+                float vs[2][NG], vm[2][NG], most[2];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    float top = 0.0f;
 #pragma unroll
-                    for (int g = 0; g < NG; g++) {
-                        vs[h][g] = lo_f32(cur.vp[h][g]); vm[h][g] = hi_f32(cur.vp[h][g]);
-                        top = fmaxf(top, vs[h][g]);
-                    }
-                    big[h] = log2_floor(top);
+                    for (int g = 0; g < NG; g++) { vs[h][g] = lo_f32(vp[h][g]); vm[h][g] = hi_f32(vp[h][g]); }
+                    most[h] = 8.0f - log2_floor(NG == 1 ? vs[h][0] : fmaxf(vs[h][0], vs[h][NG - 1]));
                 }
                 bool over = false;
+                float2 y[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) over |= x[nt][e] + big[e >> 1] > M[nt][e & 1] + 8.0f;
+                    for (int h = 0; h < 2; h++) {
+                        y[nt][h] = make_float2(x[nt][h].x - M[nt].x, x[nt][h].y - M[nt].y);
+                        over |= fmaxf(y[nt][h].x, y[nt][h].y) > most[h];
+                    }
                 if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
+                    for (int nt = 0; nt < NT; nt++) {
+                        float2 top = make_float2(fmaxf(x[nt][0].x - most[0], x[nt][1].x - most[1]) + 8.0f, fmaxf(x[nt][0].y - most[0], x[nt][1].y - most[1]) + 8.0f);
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            float top = fmaxf(x[nt][e] + big[0], x[nt][e + 2] + big[1]);
-#pragma unroll
-                            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                            top = fmaxf(top, M[nt][e]);
-                            const float f = exp2f(M[nt][e] - top);
-                            M[nt][e] = top;
-                            l[nt][e] *= f;
-#pragma unroll
-                            for (int g = 0; g < NG; g++) po[nt][e][g] *= f;
-#pragma unroll
-                            for (int q = 0; q < NS * 4; q++) { acc[q][nt][e] *= f; acc[q][nt][e + 2] *= f; }
+                        for (int o = 4; o < 32; o <<= 1) {
+                            top.x = fmaxf(top.x, __shfl_xor_sync(0xffffffffu, top.x, o));
+                            top.y = fmaxf(top.y, __shfl_xor_sync(0xffffffffu, top.y, o));
                         }
+                        top = make_float2(fmaxf(top.x, M[nt].x), fmaxf(top.y, M[nt].y));
+                        const float2 f = make_float2(exp2_approx(M[nt].x - top.x), exp2_approx(M[nt].y - top.y));
+                        M[nt] = top;
+                        l[nt] = mul2(l[nt], f);
+#pragma unroll
+                        for (int g = 0; g < NG; g++) po[nt][g] = mul2(po[nt][g], f);
+#pragma unroll
+                        for (int q = 0; q < NS * 4; q++) { acc[q][nt][0] *= f.x; acc[q][nt][1] *= f.y; acc[q][nt][2] *= f.x; acc[q][nt][3] *= f.y; }
+#pragma unroll
+                        for (int h = 0; h < 2; h++) y[nt][h] = make_float2(x[nt][h].x - top.x, x[nt][h].y - top.y);
+                    }
                 }
                 // ---- p, its sums, and w = p s as the second product's operand
                 uint32_t wb[NT][NG][2], wc[NT][NG][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    float e4[4];
+                    float2 e2[2];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) e4[e] = exp2f(x[nt][e] - M[nt][e & 1]);
-                    l[nt][0] += e4[0] + e4[2];
-                    l[nt][1] += e4[1] + e4[3];
+                    for (int h = 0; h < 2; h++) {
+                        e2[h] = make_float2(exp2_approx(y[nt][h].x), exp2_approx(y[nt][h].y));
+                        l[nt] = add2(l[nt], e2[h]);
+                    }
 #pragma unroll
-                    for (int g = 0; g < NG; g++) {
-                        po[nt][0][g] = fmaf(e4[0], vm[0][g], fmaf(e4[2], vm[1][g], po[nt][0][g]));
-                        po[nt][1][g] = fmaf(e4[1], vm[0][g], fmaf(e4[3], vm[1][g], po[nt][1][g]));
+                    for (int g = 0; g < NG; g++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const float w0 = e4[2 * h] * vs[h][g], w1 = e4[2 * h + 1] * vs[h][g];
-                            const uint32_t hi = pack_f16(w0, w1);
+                            po[nt][g] = fma2(e2[h], both(vm[h][g]), po[nt][g]);
+                            const float2 w = mul2(e2[h], both(vs[h][g]));
+                            const uint32_t hi = pack_f16(w.x, w.y);
                             wb[nt][g][h] = transpose_8x8(hi);
-                            if constexpr (SPLIT) wc[nt][g][h] = transpose_8x8(pack_f16(w0 - lo_f32(hi), w1 - hi_f32(hi)));
+                            if constexpr (SPLIT) wc[nt][g][h] = transpose_8x8(pack_f16(w.x - lo_f32(hi), w.y - hi_f32(hi)));
                         }
-                    }
                 }
                 // ---- O^T: rows r and r + 8 of block (s, j) are elements 64 s + 8 r + 2 j and + 1, the second one times 16
+                uint32_t v[4][NS];
+#pragma unroll
+                for (int h = 0; h < 4; h++) lds_words(v[h], vc + ((h & 1) + (h >> 1) * 8) * (D / 2));
 #pragma unroll
                 for (int s = 0; s < NS; s++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         constexpr uint32_t kSel[4] = {0x4400u, 0x5511u, 0x6622u, 0x7733u};
                         const int g = NG == 1 ? 0 : s;
-                        const uint32_t u = __byte_perm(cur.v[0][s], cur.v[1][s], kSel[j]), v = __byte_perm(cur.v[2][s], cur.v[3][s], kSel[j]);
-                        const uint32_t a0 = u & 0x000F000Fu, a1 = u & 0x00F000F0u, a2 = v & 0x000F000Fu, a3 = v & 0x00F000F0u;
+                        const uint32_t u = __byte_perm(v[0][s], v[1][s], kSel[j]), w = __byte_perm(v[2][s], v[3][s], kSel[j]);
+                        const uint32_t a0 = u & 0x000F000Fu, a1 = u & 0x00F000F0u, a2 = w & 0x000F000Fu, a3 = w & 0x00F000F0u;
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             mma_16816(acc[s * 4 + j][nt], a0, a1, a2, a3, wb[nt][g][0], wb[nt][g][1]);
@@ -396,110 +476,141 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                         }
                     }
             }
-            cur = nxt;
-            have = next_have;
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(empty(stage));
         }
+        const bool whole = ta == 0 && tb == it.span.tiles;
+        more = wk.next(p, ROWS);
+        if (more) prime();                                            // under the end of this piece
 
-        // ---- join the warps: common reference, then one slab a warp
+        // ---- join the warps: common reference, then four slabs, two warps each one after the other
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
+            for (int o = 4; o < 32; o <<= 1) {
+                l[nt].x += __shfl_xor_sync(0xffffffffu, l[nt].x, o);
+                l[nt].y += __shfl_xor_sync(0xffffffffu, l[nt].y, o);
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) {
-                    l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], o);
-#pragma unroll
-                    for (int g = 0; g < NG; g++) po[nt][e][g] += __shfl_xor_sync(0xffffffffu, po[nt][e][g], o);
+                for (int g = 0; g < NG; g++) {
+                    po[nt][g].x += __shfl_xor_sync(0xffffffffu, po[nt][g].x, o);
+                    po[nt][g].y += __shfl_xor_sync(0xffffffffu, po[nt][g].y, o);
                 }
-                if (r == 0) { sm.m[warp][nt * 8 + 2 * c + e] = M[nt][e]; sm.l[warp][nt * 8 + 2 * c + e] = l[nt][e]; }
             }
+            if (r == 0) {
+                *reinterpret_cast<float2*>(&sm.m[warp][nt * 8 + 2 * c]) = M[nt];
+                *reinterpret_cast<float2*>(&sm.l[warp][nt * 8 + 2 * c]) = l[nt];
+            }
+        }
         __syncthreads();
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int half = 0; half < 2; half++) {
+            if ((warp >> 2) == half) {
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int row = nt * 8 + 2 * c + e;
-                float top = sm.m[0][row];
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int q = 1; q < 8; q++) top = fmaxf(top, sm.m[q][row]);
-                const float f = exp2f(M[nt][e] - top);
+                    for (int e = 0; e < 2; e++) {
+                        const int row = nt * 8 + 2 * c + e;
+                        float top = sm.m[0][row];
 #pragma unroll
-                for (int s = 0; s < NS; s++) {
-                    const float off = po[nt][e][NG == 1 ? 0 : s] * f;
+                        for (int q = 1; q < 8; q++) top = fmaxf(top, sm.m[q][row]);
+                        const float f = exp2_approx((e ? M[nt].y : M[nt].x) - top);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        float2 o;
-                        o.x = fmaf(acc[s * 4 + j][nt][e] * 0x1p24f, f, off);
-                        o.y = fmaf(acc[s * 4 + j][nt][e + 2] * 0x1p20f, f, off);
-                        *reinterpret_cast<float2*>(&sm.slab[warp][row * OPAD + 64 * s + 8 * r + 2 * j]) = o;
+                        for (int s = 0; s < NS; s++) {
+                            const float2 pg = po[nt][NG == 1 ? 0 : s];
+                            const float off = (e ? pg.y : pg.x) * f;
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                float2& at = *reinterpret_cast<float2*>(&sm.slab[warp & 3][row * OPAD + 64 * s + 8 * r + 2 * j]);
+                                float2 o;
+                                o.x = fmaf(acc[s * 4 + j][nt][e] * 0x1p24f, f, off);
+                                o.y = fmaf(acc[s * 4 + j][nt][e + 2] * 0x1p20f, f, off);
+                                if (half) { o.x += at.x; o.y += at.y; }
+                                at = o;
+                            }
+                        }
                     }
-                }
             }
-        __syncthreads();
-        float* slot = whole ? nullptr : p.ws + (int64_t)(blockIdx.x * 2 + (at == begin && ta > 0 ? 0 : 1)) * Slot<NT>::floats(D);
-        for (int i = tid; i < ROWS * (D / 2); i += 256) {
-            const int row = i / (D / 2), d = (i % (D / 2)) * 2;
+            __syncthreads();
+        }
+        float* slot = whole ? nullptr : p.ws + (int64_t)(blockIdx.x * 2 + (ta > 0 ? 0 : 1)) * Slot<NT>::floats(D);
+        for (int i = tid; i < ROWS * (D / 4); i += 256) {
+            const int row = i / (D / 4), d = (i % (D / 4)) * 4;
             float top = sm.m[0][row];
 #pragma unroll
             for (int q = 1; q < 8; q++) top = fmaxf(top, sm.m[q][row]);
             float sum = 0.0f;
-            float2 o = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int q = 0; q < 8; q++) {
-                sum = fmaf(sm.l[q][row], exp2f(sm.m[q][row] - top), sum);
-                const float2 v = *reinterpret_cast<const float2*>(&sm.slab[q][row * OPAD + d]);
-                o.x += v.x; o.y += v.y;
+            for (int q = 0; q < 8; q++) sum = fmaf(sm.l[q][row], exp2_approx(sm.m[q][row] - top), sum);
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const float4 v = *reinterpret_cast<const float4*>(&sm.slab[q][row * OPAD + d]);
+                o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
             }
             if (slot) {
-                *reinterpret_cast<float2*>(slot + row * D + d) = o;
+                *reinterpret_cast<float4*>(slot + row * D + d) = o;
                 if (d == 0) { slot[ROWS * D + row] = top; slot[ROWS * D + ROWS + row] = sum; }
             } else if (row < rows) {
-                store_row<T>(p, seq, it.head, row0 + row, d, o, top, sum);
+                store_row<T>(p, seq, it.head, row0 + row, d, make_float2(o.x, o.y), top, sum);
+                store_row<T>(p, seq, it.head, row0 + row, d + 2, make_float2(o.z, o.w), top, sum);
             }
         }
-        at += tb - ta;
     }
 }
 
 // Joins the parts of the items that the CTAs' boundaries cut.  Block x is for boundary x + 1: it acts if that is the first
-// boundary inside its item.  D / 4 threads a row.
+// boundary inside its item.  256 / ROWS threads a row, which share the parts and the elements.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnParams p, int ctas) {
-    constexpr int ROWS = NT * 8;
+__global__ void __launch_bounds__(512) kv4_attn_join_kernel(AttnParams p, int ctas) {
+    constexpr int ROWS = NT * 8, D4 = D / 4, GROUPS = 512 / (8 * D4);                  // eight rows at a time, GROUPS sets of threads share their parts
     __shared__ int64_t red[8];
     __shared__ Where found;
+    __shared__ float4 part_o[GROUPS][8][D4];
+    __shared__ float part_l[GROUPS][8];
     pdl_trigger();
     pdl_wait();
-    const int64_t total = total_tiles(p, ROWS, red);
-    const int64_t parts = min((int64_t)ctas, total);
-    const int64_t i = blockIdx.x + 1;
-    if (i >= parts) return;
-    const auto bound = [&](int64_t k) { return total * k / parts; };
-    const Where w = find_tile(p, ROWS, bound(i), red, &found);
+    const int i = blockIdx.x + 1;
+    const Line line = find_part(p, ROWS, ctas, i, red, &found);
+    if (i >= line.parts) return;
+    const Where w = found;
     const SeqInfo seq = small_seq(p, w.b);
-    const Item it = find_item(p, seq, ROWS, bound(i) - w.at);
+    const Item it = find_item(p, seq, ROWS, line.bound(i) - w.at);
     const int64_t start = w.at + it.start, stop = start + it.span.tiles;
-    if (start >= bound(i) || bound(i - 1) > start) return;            // not cut here, or not for the first time
-    int64_t last = i;                                                 // the CTA that holds the item's last tile
-    while (bound(last + 1) < stop) last++;
+    if (start >= line.bound(i) || line.bound(i - 1) > start) return;  // not cut here, or not for the first time
+    int last = i;                                                     // the CTA that holds the item's last tile
+    while (line.bound(last + 1) < stop) last++;
     const int row0 = it.rt * ROWS, rows = min(ROWS, seq.n * p.per - row0);
-    const auto slot = [&](int64_t k) { return p.ws + (k * 2 + (k == i - 1 ? 1 : 0)) * Slot<NT>::floats(D); };
-    for (int q = threadIdx.x; q < rows * (D / 4); q += 256) {
-        const int row = q / (D / 4), d = (q % (D / 4)) * 4;
+    const auto slot = [&](int k) { return p.ws + (int64_t)(k * 2 + (k == i - 1 ? 1 : 0)) * Slot<NT>::floats(D); };
+    const int group = threadIdx.x / (8 * D4), rr = threadIdx.x / D4 % 8, d = threadIdx.x % D4 * 4;
+    for (int r0 = 0; r0 < rows; r0 += 8) {
+        const int row = r0 + rr;
         float top = -1e30f;
-        for (int64_t k = i - 1; k <= last; k++) top = fmaxf(top, slot(k)[ROWS * D + row]);
+#pragma unroll 4
+        for (int k = i - 1; k <= last; k++) top = fmaxf(top, slot(k)[ROWS * D + row]);
         float sum = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-        for (int64_t k = i - 1; k <= last; k++) {
+        for (int k = i - 1 + group; k <= last; k += GROUPS) {
             const float* s = slot(k);
-            const float f = exp2f(s[ROWS * D + row] - top);
+            const float f = exp2_approx(s[ROWS * D + row] - top);
             const float4 v = *reinterpret_cast<const float4*>(s + row * D + d);
             sum = fmaf(s[ROWS * D + ROWS + row], f, sum);
             o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
         }
-        store_row<T>(p, seq, it.head, row0 + row, d, make_float2(o.x, o.y), top, sum);
-        store_row<T>(p, seq, it.head, row0 + row, d + 2, make_float2(o.z, o.w), top, sum);
+        __syncthreads();
+        part_o[group][rr][d / 4] = o;
+        if (d == 0) part_l[group][rr] = sum;
+        __syncthreads();
+        if (group == 0 && row < rows) {
+#pragma unroll
+            for (int g = 1; g < GROUPS; g++) {
+                const float4 v = part_o[g][rr][d / 4];
+                o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+                sum += part_l[g][rr];
+            }
+            store_row<T>(p, seq, it.head, row0 + row, d, make_float2(o.x, o.y), top, sum);
+            store_row<T>(p, seq, it.head, row0 + row, d + 2, make_float2(o.z, o.w), top, sum);
+        }
     }
 }
 
@@ -515,14 +626,14 @@ template <typename T, int D, int NG, int NT>
 static int32_t launch_rows(oxq_handle* h, const AttnParams& p, int64_t most_tiles, int64_t item_tiles) {
     const int ctas = (int)(most_tiles < attn_ctas(h, NT) ? most_tiles : attn_ctas(h, NT));
     auto kernel = kv4_attn_rows_kernel<T, D, NG, NT>;
-    constexpr int bytes = (int)sizeof(Smem<T, D, NG, NT>);
+    constexpr int bytes = (int)sizeof(Smem<D, NG, NT>);
     static OxqPerDevice ready;
     if (!ready.get(h->device)) {
         OXQ_CUDA(h, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
         ready.set(h->device, 1);
     }
     OXQ_CUDA(h, oxq_launch(kernel, ctas, 256, bytes, h->stream, p));
-    if (ctas > 1 && item_tiles > 1) OXQ_CUDA(h, oxq_launch(kv4_attn_join_kernel<T, D, NT>, ctas - 1, 256, 0, h->stream, p, ctas));
+    if (ctas > 1 && item_tiles > MIN_TILES) OXQ_CUDA(h, oxq_launch(kv4_attn_join_kernel<T, D, NT>, ctas - 1, 512, 0, h->stream, p, ctas));
     return OXQ_OK;
 }
 

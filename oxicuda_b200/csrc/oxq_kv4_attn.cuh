@@ -36,13 +36,19 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnParams& p, int b) {
     return q;
 }
 
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 // Two elements of an output row: row `row` of kv head `head` is query token row / per, query head head * per + row % per.
 // o / sum, or zeros where nothing was seen; with the first two goes lse = ln(sum over keys of exp(score)).
 template <typename T>
 __device__ __forceinline__ void store_row(const AttnParams& p, const SeqInfo& q, int head, int row, int d, float2 o, float ref, float sum) {
     const int64_t t = q.start + row / p.per;
     const int qh = head * p.per + row % p.per;
-    const float inv = sum > 0.0f ? __fdividef(1.0f, sum) : sum != sum ? sum : 0.0f;
+    const float inv = sum > 0.0f ? 1.0f / sum : sum != sum ? sum : 0.0f;
     struct alignas(4) Pair { T x, y; } v;
     v.x = Elem<T>::from_f32(o.x * inv);
     v.y = Elem<T>::from_f32(o.y * inv);
