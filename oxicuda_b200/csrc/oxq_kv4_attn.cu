@@ -75,7 +75,7 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 struct Span { int first, tiles; int lo, hi; };          // first tile, how many (at least one), visible positions [lo, hi)
 __device__ __forceinline__ Span item_span(const AttnParams& p, const SeqInfo& q, int rt, int nr) {
     Span s;
-    const int j0 = (rt * nr) / p.per, j1 = min(q.n, (min((rt + 1) * nr, q.n * p.per) - 1) / p.per + 1) - 1;
+    const int j0 = p.by_per.div(rt * nr), j1 = p.by_per.div(min((rt + 1) * nr, q.n * p.per) - 1);
     s.hi = p.causal ? min(q.len, q.len - q.asked + j1 + 1) : q.len;
     s.lo = p.window > 0 ? max(0, q.len - q.asked + j0 + 1 - p.window) : 0;
     s.hi = max(s.hi, 0);
@@ -84,8 +84,8 @@ __device__ __forceinline__ Span item_span(const AttnParams& p, const SeqInfo& q,
     return s;
 }
 __device__ __forceinline__ int row_blocks(const AttnParams& p, const SeqInfo& q, int nr) { return (q.n * p.per + nr - 1) / nr; }
-__device__ __forceinline__ int64_t head_tiles(const AttnParams& p, const SeqInfo& q, int nr) {
-    int64_t t = 0;
+__device__ __forceinline__ int head_tiles(const AttnParams& p, const SeqInfo& q, int nr) {
+    int t = 0;
     for (int rt = 0, e = row_blocks(p, q, nr); rt < e; rt++) t += item_span(p, q, rt, nr).tiles;
     return t;
 }
@@ -98,52 +98,53 @@ __device__ __forceinline__ SeqInfo small_seq(const AttnParams& p, int b) {
 
 // The line of tiles, cut into `parts` parts that differ by one tile at most.
 struct Line {
-    int64_t total, each; int parts, more;
-    __device__ __forceinline__ int64_t bound(int64_t k) const { return each * k + (k < more ? k : more); }
+    int total, parts, each, more;
+    __device__ __forceinline__ int bound(int k) const { return each * k + min(k, more); }
+    __device__ __forceinline__ int part_of(int tile) const {
+        const int wide = more * (each + 1);
+        return tile < wide ? tile / (each + 1) : more + (tile - wide) / each;
+    }
 };
-struct Where { int b; int64_t at; };    // sequence, and the line's position of its first tile
+struct Where { int b, at; };            // sequence, and the line's position of its first tile
 
-// Scan over 256 sequences from b0 on: tiles of this thread's one, and how many lie before it (from `base`); base moves on.
-// Whole CTA (its first 256 threads hold the sequences).
-__device__ __forceinline__ int64_t scan_tiles(const AttnParams& p, int nr, int b0, int64_t* red, int64_t& base, int64_t& mine) {
-    const int b = b0 + threadIdx.x;
-    mine = (int)threadIdx.x < 256 && b < p.s.seqs ? head_tiles(p, small_seq(p, b), nr) * p.c.heads : 0;
-    int64_t x = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if ((threadIdx.x & 31) >= o) x += y;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 31 && threadIdx.x < 256) red[threadIdx.x >> 5] = x;
-    __syncthreads();
-    int64_t before = base;
-#pragma unroll
-    for (int w = 0; w < 8; w++) {
-        if (w < (int)(threadIdx.x >> 5)) before += red[w];
-        base += red[w];
-    }
-    return before + x - mine;
-}
-// The line, and the sequence that holds tile bound(k), if k < parts.
-__device__ __forceinline__ Line find_part(const AttnParams& p, int nr, int ctas, int k, int64_t* red, Where* found) {
+// The line, and the sequence that holds tile bound(k), if k < parts.  Whole CTA of 256 threads: a scan over 256 sequences at a
+// time, once for the total and, where there are more of them, once again for the place.
+__device__ __forceinline__ Line find_part(const AttnParams& p, int nr, int ctas, int k, int* red, Where* found) {
     Line line;
-    line.total = 0;
-    int64_t mine = 0, start = 0;
-    for (int b0 = 0; b0 < p.s.seqs; b0 += 256) start = scan_tiles(p, nr, b0, red, line.total, mine);
-    const int64_t most = (line.total + MIN_TILES - 1) / MIN_TILES;
-    line.parts = (int)(most < ctas ? most : ctas);
-    line.each = line.parts ? line.total / line.parts : 0;
-    line.more = (int)(line.total - line.each * line.parts);
-    if (k >= line.parts) return line;
-    const int64_t want = line.bound(k);
-    if (p.s.seqs <= 256) {
-        if (mine > 0 && start <= want && want < start + mine) { found->b = threadIdx.x; found->at = start; }
-    } else {
-        int64_t base = 0;
-        for (int b0 = 0; b0 < p.s.seqs && base <= want; b0 += 256) {
-            start = scan_tiles(p, nr, b0, red, base, mine);
-            if (mine > 0 && start <= want && want < start + mine) { found->b = b0 + threadIdx.x; found->at = start; }
+    int want = -1;
+    for (int pass = 0; pass < 2; pass++) {
+        int base = 0, mine = 0, start = 0;
+        for (int b0 = 0; b0 < p.s.seqs; b0 += 256) {
+            const int b = b0 + (int)threadIdx.x;
+            mine = b < p.s.seqs ? head_tiles(p, small_seq(p, b), nr) * p.c.heads : 0;
+            int x = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if ((threadIdx.x & 31) >= o) x += y;
+            }
+            __syncthreads();
+            if ((threadIdx.x & 31) == 31) red[threadIdx.x >> 5] = x;
+            __syncthreads();
+            start = base + x - mine;
+#pragma unroll
+            for (int w = 0; w < 8; w++) {
+                const int v = red[w];
+                if (w < (int)(threadIdx.x >> 5)) start += v;
+                base += v;
+            }
+            if (pass == 1 && mine > 0 && start <= want && want < start + mine) { found->b = b; found->at = start; }
+        }
+        if (pass == 1) break;
+        line.total = base;
+        line.parts = min(ctas, (base + MIN_TILES - 1) / MIN_TILES);
+        line.each = line.parts ? (int)((unsigned)base / (unsigned)line.parts) : 0;
+        line.more = base - line.each * line.parts;
+        if (k >= line.parts) return line;
+        want = line.bound(k);
+        if (p.s.seqs <= 256) {
+            if (mine > 0 && start <= want && want < start + mine) { found->b = threadIdx.x; found->at = start; }
+            break;
         }
     }
     __syncthreads();
@@ -151,11 +152,11 @@ __device__ __forceinline__ Line find_part(const AttnParams& p, int nr, int ctas,
 }
 
 // An item of a sequence: which one holds tile `in_seq` of the sequence's own line.
-struct Item { int head, rt; int64_t start; Span span; };
-__device__ __forceinline__ Item find_item(const AttnParams& p, const SeqInfo& q, int nr, int64_t in_seq) {
+struct Item { int head, rt, start; Span span; };
+__device__ __forceinline__ Item find_item(const AttnParams& p, const SeqInfo& q, int nr, int in_seq) {
     Item it;
-    const int64_t per_head = head_tiles(p, q, nr);
-    it.head = (int)(in_seq / per_head);
+    const int per_head = head_tiles(p, q, nr);
+    it.head = (int)((unsigned)in_seq / (unsigned)per_head);
     it.start = it.head * per_head;
     for (it.rt = 0;; it.rt++) {
         it.span = item_span(p, q, it.rt, nr);
@@ -168,10 +169,12 @@ template <int NT> struct Slot {         // what a cut item's CTA leaves: o [rows
     static constexpr int ROWS = NT * 8;
     __host__ __device__ static constexpr int floats(int d) { return ROWS * (d + 2); }
 };
+// Each CTA's note for the join: the item that begins in its part and goes on in the next ones; last < 0: there is none.
+struct alignas(16) Cut { int b, head, rt, last; };
 
 // Part of the tiles of one item that a CTA works on.
 struct Work {
-    Where w; SeqInfo seq; int64_t seq_tiles, at, end;
+    Where w; SeqInfo seq; int seq_tiles, at, end;
     Item it; int ta, tb;
     __device__ __forceinline__ bool next(const AttnParams& p, int nr) {
         if (at >= end) return false;
@@ -182,8 +185,8 @@ struct Work {
             seq_tiles = head_tiles(p, seq, nr) * p.c.heads;
         }
         it = find_item(p, seq, nr, at - w.at);
-        ta = (int)(at - w.at - it.start);
-        tb = (int)min((int64_t)it.span.tiles, (int64_t)ta + (end - at));
+        ta = at - w.at - it.start;
+        tb = min(it.span.tiles, ta + (end - at));
         at += tb - ta;
         return true;
     }
@@ -203,7 +206,7 @@ struct Smem {
     float m[8][ROWS], l[8][ROWS];
     uint64_t bars[2 * STAGES];
     unsigned char there[STAGES][8];
-    int64_t red[8];
+    int red[8];
     Where found;
 };
 
@@ -228,7 +231,11 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
     pdl_wait();
 
     const Line line = find_part(p, ROWS, gridDim.x, blockIdx.x, sm.red, &sm.found);
-    if (blockIdx.x >= line.parts) return;
+    if ((int)blockIdx.x >= line.parts) {
+        if (tid == 0) reinterpret_cast<Cut*>(p.ws)[blockIdx.x] = Cut{0, 0, 0, -1};
+        return;
+    }
+    float* slots = p.ws + gridDim.x * (sizeof(Cut) / sizeof(float));
     Work wk;
     wk.at = line.bound(blockIdx.x);
     wk.end = line.bound(blockIdx.x + 1);
@@ -285,7 +292,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
 #pragma unroll
             for (int e = 0; e < 8; e++) f[e] = 0.0f;
             if (row < rows) {
-                const int j = (row0 + row) / p.per, qh = it.head * p.per + (row0 + row) % p.per;
+                const int j = p.by_per.div(row0 + row), qh = it.head * p.per + p.by_per.mod(row0 + row);
                 const T* src = (const T*)p.q + (int64_t)(seq.start + j) * p.q_ts + (int64_t)qh * p.q_hs + g * 8;
                 if (p.q_vec) {
                     const Vec16<T> v = ld16(src);
@@ -331,7 +338,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[i][nt][e] = 0.0f;
         // keys that every row of the block sees need no mask
-        const int pos0 = seq.len - seq.asked + row0 / p.per, pos1 = seq.len - seq.asked + (row0 + rows - 1) / p.per;
+        const int pos0 = seq.len - seq.asked + p.by_per.div(row0), pos1 = seq.len - seq.asked + p.by_per.div(row0 + rows - 1);
         const int all_hi = p.causal ? min(seq.len, pos0 + 1) : seq.len, all_lo = p.window > 0 ? pos1 + 1 - p.window : 0;
 
         for (int i = ta; i < tb; i++, count++) {
@@ -392,7 +399,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                             for (int e = 0; e < 2; e++) {
-                                const int pos = seq.len - seq.asked + (row0 + nt * 8 + 2 * c + e) / p.per;      // the row's own position
+                                const int pos = seq.len - seq.asked + p.by_per.div(row0 + nt * 8 + 2 * c + e);      // the row's own position
                                 const int vhi = p.causal ? min(seq.len, pos + 1) : seq.len, vlo = p.window > 0 ? pos + 1 - p.window : 0;
                                 if (t < vlo || t >= vhi) (e ? x[nt][h].y : x[nt][h].x) = -INFINITY;
                             }
@@ -480,6 +487,10 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
             if (lane == 0) tc::mbar_arrive(empty(stage));
         }
         const bool whole = ta == 0 && tb == it.span.tiles;
+        if (tid == 0 && wk.at == wk.end) {                            // the CTA's last piece: does its item begin here and go on?
+            const int first = wk.w.at + it.start;
+            reinterpret_cast<Cut*>(p.ws)[blockIdx.x] = Cut{wk.w.b, it.head, it.rt, ta == 0 && tb < it.span.tiles ? line.part_of(first + it.span.tiles - 1) : -1};
+        }
         more = wk.next(p, ROWS);
         if (more) prime();                                            // under the end of this piece
 
@@ -532,7 +543,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
             }
             __syncthreads();
         }
-        float* slot = whole ? nullptr : p.ws + (int64_t)(blockIdx.x * 2 + (ta > 0 ? 0 : 1)) * Slot<NT>::floats(D);
+        float* slot = whole ? nullptr : slots + (int64_t)(blockIdx.x * 2 + (ta > 0 ? 0 : 1)) * Slot<NT>::floats(D);
         for (int i = tid; i < ROWS * (D / 4); i += 256) {
             const int row = i / (D / 4), d = (i % (D / 4)) * 4;
             float top = sm.m[0][row];
@@ -558,39 +569,32 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
     }
 }
 
-// Joins the parts of the items that the CTAs' boundaries cut.  Block x is for boundary x + 1: it acts if that is the first
-// boundary inside its item.  256 / ROWS threads a row, which share the parts and the elements.
+// Joins the parts of the items that the CTAs' boundaries cut: block x takes the one that begins in CTA x.  512 threads: eight
+// rows at a time, and GROUPS sets of threads that share their parts.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(512) kv4_attn_join_kernel(AttnParams p, int ctas) {
-    constexpr int ROWS = NT * 8, D4 = D / 4, GROUPS = 512 / (8 * D4);                  // eight rows at a time, GROUPS sets of threads share their parts
-    __shared__ int64_t red[8];
-    __shared__ Where found;
+__global__ void __launch_bounds__(512) kv4_attn_join_kernel(AttnParams p) {
+    constexpr int ROWS = NT * 8, D4 = D / 4, GROUPS = 512 / (8 * D4);
     __shared__ float4 part_o[GROUPS][8][D4];
     __shared__ float part_l[GROUPS][8];
     pdl_trigger();
     pdl_wait();
-    const int i = blockIdx.x + 1;
-    const Line line = find_part(p, ROWS, ctas, i, red, &found);
-    if (i >= line.parts) return;
-    const Where w = found;
-    const SeqInfo seq = small_seq(p, w.b);
-    const Item it = find_item(p, seq, ROWS, line.bound(i) - w.at);
-    const int64_t start = w.at + it.start, stop = start + it.span.tiles;
-    if (start >= line.bound(i) || line.bound(i - 1) > start) return;  // not cut here, or not for the first time
-    int last = i;                                                     // the CTA that holds the item's last tile
-    while (line.bound(last + 1) < stop) last++;
-    const int row0 = it.rt * ROWS, rows = min(ROWS, seq.n * p.per - row0);
-    const auto slot = [&](int k) { return p.ws + (int64_t)(k * 2 + (k == i - 1 ? 1 : 0)) * Slot<NT>::floats(D); };
+    const int4 note = *reinterpret_cast<const int4*>(reinterpret_cast<const Cut*>(p.ws) + blockIdx.x);
+    const int first = blockIdx.x, last = note.w;
+    if (last < 0) return;
+    const SeqInfo seq = seq_info(p, note.x);
+    const int head = note.y, row0 = note.z * ROWS, rows = min(ROWS, seq.n * p.per - row0);
+    const float* slots = p.ws + (gridDim.x) * (sizeof(Cut) / sizeof(float));
+    const auto slot = [&](int k) { return slots + (int64_t)(k * 2 + (k == first ? 1 : 0)) * Slot<NT>::floats(D); };
     const int group = threadIdx.x / (8 * D4), rr = threadIdx.x / D4 % 8, d = threadIdx.x % D4 * 4;
     for (int r0 = 0; r0 < rows; r0 += 8) {
         const int row = r0 + rr;
         float top = -1e30f;
 #pragma unroll 4
-        for (int k = i - 1; k <= last; k++) top = fmaxf(top, slot(k)[ROWS * D + row]);
+        for (int k = first; k <= last; k++) top = fmaxf(top, slot(k)[ROWS * D + row]);
         float sum = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-        for (int k = i - 1 + group; k <= last; k += GROUPS) {
+        for (int k = first + group; k <= last; k += GROUPS) {
             const float* s = slot(k);
             const float f = exp2_approx(s[ROWS * D + row] - top);
             const float4 v = *reinterpret_cast<const float4*>(s + row * D + d);
@@ -608,8 +612,8 @@ __global__ void __launch_bounds__(512) kv4_attn_join_kernel(AttnParams p, int ct
                 o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
                 sum += part_l[g][rr];
             }
-            store_row<T>(p, seq, it.head, row0 + row, d, make_float2(o.x, o.y), top, sum);
-            store_row<T>(p, seq, it.head, row0 + row, d + 2, make_float2(o.z, o.w), top, sum);
+            store_row<T>(p, seq, head, row0 + row, d, make_float2(o.x, o.y), top, sum);
+            store_row<T>(p, seq, head, row0 + row, d + 2, make_float2(o.z, o.w), top, sum);
         }
     }
 }
@@ -633,7 +637,7 @@ static int32_t launch_rows(oxq_handle* h, const AttnParams& p, int64_t most_tile
         ready.set(h->device, 1);
     }
     OXQ_CUDA(h, oxq_launch(kernel, ctas, 256, bytes, h->stream, p));
-    if (ctas > 1 && item_tiles > MIN_TILES) OXQ_CUDA(h, oxq_launch(kv4_attn_join_kernel<T, D, NT>, ctas - 1, 512, 0, h->stream, p, ctas));
+    if (ctas > 1 && item_tiles > MIN_TILES) OXQ_CUDA(h, oxq_launch(kv4_attn_join_kernel<T, D, NT>, ctas, 512, 0, h->stream, p));
     return OXQ_OK;
 }
 
@@ -660,7 +664,7 @@ static Plan make_plan(const oxq_handle* h, const oxq_kv4_cache* cc, const oxq_kv
     f.nt = max_rows <= 8 ? 1 : 2;
     f.tiles = max_rows > ROWS_MOST;
     f.rows = !f.tiles || s->seqs > 1;
-    f.rows_bytes = f.rows ? (size_t)attn_ctas(h, f.nt) * 2 * (f.nt == 1 ? Slot<1>::floats(cc->dim) : Slot<2>::floats(cc->dim)) * sizeof(float) : 0;
+    f.rows_bytes = f.rows ? (size_t)attn_ctas(h, f.nt) * 2 * (f.nt == 1 ? Slot<1>::floats(cc->dim) : Slot<2>::floats(cc->dim)) * sizeof(float) + attn_ctas(h, f.nt) * sizeof(Cut) : 0;
     f.items = 0; f.parts = 1;
     if (f.tiles) {
         const int64_t with = all_rows / (ROWS_MOST + 1) < s->seqs ? all_rows / (ROWS_MOST + 1) : s->seqs;
@@ -719,12 +723,20 @@ int32_t oxq_kv4_attention(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_k
     p.q = a->q; p.q_ts = a->q_token_stride; p.q_hs = a->q_head_stride;
     p.q_vec = (((uintptr_t)a->q | (uintptr_t)(a->q_token_stride * 2) | (uintptr_t)(a->q_head_stride * 2)) & 15u) == 0;
     p.out = a->out; p.o_ts = a->out_token_stride; p.o_hs = a->out_head_stride; p.lse = a->lse;
+    p.by_per.set((int)per);
     p.per = (int)per; p.q_heads = (int)a->q_heads;
     p.scale_log2 = a->scale * 1.44269504088896340736f;
     p.causal = a->causal ? 1 : 0;
     p.window = a->window > INT32_MAX ? INT32_MAX : (int)a->window;
     p.out_vec = (((uintptr_t)a->out | (uintptr_t)(a->out_token_stride * 2) | (uintptr_t)(a->out_head_stride * 2)) & 15u) == 0;
     p.status = h->dev_status;
+    // the most tiles that there can be for the row kernel: every row block of every sequence over a whole table row
+    const int nt = plan.nt;
+    const int64_t item_tiles = (p.s.width * cache->page_size + TILE - 1) / TILE + 1;
+    const int64_t blocks = plan.tiles ? p.s.seqs * (ROWS_MOST / (nt * 8)) : (p.s.tokens * per + nt * 8 - 1) / (nt * 8) + p.s.seqs;
+    const int64_t items = plan.rows ? blocks * p.c.heads : 0;
+    if (items > INT32_MAX / item_tiles) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 attention: more work than one call counts (2^31 tiles of %d keys)", TILE);
+    const int64_t most = items * item_tiles;
     if (plan.tiles) {
         p.row_min = plan.rows ? (int)ROWS_MOST : 0;
         p.parts = plan.parts;
@@ -734,11 +746,6 @@ int32_t oxq_kv4_attention(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_k
         p.row_limit = (int)ROWS_MOST;
     }
     p.ws = (float*)workspace;
-    const int nt = plan.nt;
-    // the most tiles that there can be: every row block of every sequence over a whole table row
-    const int64_t item_tiles = (p.s.width * cache->page_size + TILE - 1) / TILE + 1;
-    const int64_t items = (p.s.tokens * per + nt * 8 - 1) / (nt * 8) + p.s.seqs;
-    const int64_t most = items > (1ll << 40) / item_tiles / p.c.heads ? (1ll << 40) : items * item_tiles * p.c.heads;
     if (a->dtype == OXQ_BF16)
         return nt == 1 ? launch_dims<__nv_bfloat16, 1>(h, cache, p, most, item_tiles) : launch_dims<__nv_bfloat16, 2>(h, cache, p, most, item_tiles);
     return nt == 1 ? launch_dims<__half, 1>(h, cache, p, most, item_tiles) : launch_dims<__half, 2>(h, cache, p, most, item_tiles);

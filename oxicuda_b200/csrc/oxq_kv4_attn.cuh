@@ -5,6 +5,19 @@
 namespace oxq {
 namespace kv4 {
 
+// n / d for 0 <= n < 2^31 by a product: mul = ceil(2^(32 + shift) / d) with 2^(shift + 1) >= d is exact in that range; d = 1 apart.
+struct FastDiv {
+    uint32_t mul; int shift, d;
+    void set(int div) {
+        d = div;
+        shift = 0;
+        while ((2ll << shift) < div) shift++;
+        mul = div == 1 ? 0u : (uint32_t)((((unsigned long long)1 << (32 + shift)) + (unsigned)div - 1) / (unsigned)div);
+    }
+    __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift); }
+    __device__ __forceinline__ int mod(int n) const { return n - div(n) * d; }
+};
+
 struct AttnParams {
     Pool c;
     Batch s;
@@ -12,6 +25,7 @@ struct AttnParams {
     void* out; int64_t o_ts, o_hs;
     float* lse;                                         // [tokens][q_heads], or null
     int per, q_heads;                                   // query heads per kv head, all query heads
+    FastDiv by_per;
     float scale_log2;                                   // scale * log2(e)
     int causal, window;                                 // window 0: none
     int row_limit, row_min;                             // sequences of at most row_limit rows (0: all) are the row kernel's, of more than row_min the tile kernel's
@@ -46,8 +60,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // o / sum, or zeros where nothing was seen; with the first two goes lse = ln(sum over keys of exp(score)).
 template <typename T>
 __device__ __forceinline__ void store_row(const AttnParams& p, const SeqInfo& q, int head, int row, int d, float2 o, float ref, float sum) {
-    const int64_t t = q.start + row / p.per;
-    const int qh = head * p.per + row % p.per;
+    const int64_t t = q.start + p.by_per.div(row);
+    const int qh = head * p.per + p.by_per.mod(row);
     const float inv = sum > 0.0f ? 1.0f / sum : sum != sum ? sum : 0.0f;
     struct alignas(4) Pair { T x, y; } v;
     v.x = Elem<T>::from_f32(o.x * inv);
