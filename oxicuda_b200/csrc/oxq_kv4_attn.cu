@@ -8,8 +8,8 @@
 // c * 2^-24 (16 c * 2^-24 for a nibble that is left where it lies): one AND per two codes, exact, and the power of two is
 // taken out again in f32.  q enters as f16 scaled per row by a power of two, so that the row's largest element lies in
 // [2^11, 2^12): exact for f16 and bf16 values down to 2^-25 of the row's largest.
-// The running reference M of a row is the maximum over its keys of x + log2(largest s of the key's value row, rounded
-// down), so that w stays in f16's range whatever the scales are; it moves only when a key exceeds it by 2^8 (w <= 2^9),
+// The running reference M of a row is the maximum over its keys of x + log2(largest s of the value rows of the key and of
+// the one eight behind it, rounded down, at least -15), so that w stays in f16's range whatever the scales are; it moves only when a key exceeds it by 2^8 (w <= 2^9),
 // which one vote per 16 keys finds out.  l = sum p, the offsets' sum and all accumulators are f32.
 // f16 outputs are finer than one f16 rounding of w; for them w is split into two f16 terms (two products).
 //
@@ -30,12 +30,12 @@ constexpr int TILE = 128;               // keys per tile: 8 warps x 16
 constexpr int MIN_TILES = 2;            // tiles a CTA takes at least: a join of many small parts costs more than it brings
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -44,8 +44,11 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 __device__ __forceinline__ float lo_f32(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v & 0xFFFFu))); }
 __device__ __forceinline__ float hi_f32(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
-// floor(log2(s)) of a non-negative f16 number as a float, not below -24 (the smallest s there is; also for s = 0)
-__device__ __forceinline__ float log2_floor(float s) { return fmaxf((float)((int)(__float_as_uint(s) >> 23) - 127), -24.0f); }
+// floor(log2(s)) of the larger of two words' low halves, non-negative f16 numbers; -15 for those below 2^-14
+__device__ __forceinline__ float log2_floor(uint32_t a, uint32_t b) {
+    const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return (float)((int)((*reinterpret_cast<const uint32_t*>(&m) >> 10) & 31u) - 15);
+}
 template <int N> __device__ __forceinline__ void lds_words(uint32_t (&r)[N], const unsigned char* p) {
     if constexpr (N == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p); r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
     else if constexpr (N == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p); r[0] = v.x; r[1] = v.y; }
@@ -170,7 +173,7 @@ template <int NT> struct Slot {         // what a cut item's CTA leaves: o [rows
     __host__ __device__ static constexpr int floats(int d) { return ROWS * (d + 2); }
 };
 // Each CTA's note for the join: the item that begins in its part and goes on in the next ones; last < 0: there is none.
-struct alignas(16) Cut { int b, head, rt, last; };
+struct alignas(16) Cut { int start, n, block, last; };     // the sequence's first row and how many, head * row blocks + row block
 
 // Part of the tiles of one item that a CTA works on.
 struct Work {
@@ -198,7 +201,7 @@ template <int D, int NG> struct Stage {
 };
 template <int D, int NG, int NT>
 struct Smem {
-    static constexpr int ROWS = NT * 8, QPAD = D + 8, STAGES = 4, LEAD = 2;
+    static constexpr int ROWS = NT * 8, QPAD = D + 8, STAGES = 5, LEAD = 3;
     unsigned char ring[STAGES][Stage<D, NG>::BYTES];
     __half q[ROWS * QPAD];              // per eight elements in the order 0 4 1 5 2 6 3 7, the odd ones / 16
     float slab[4][ROWS * (D + 8)];
@@ -244,18 +247,24 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
     wk.seq_tiles = head_tiles(p, wk.seq, ROWS) * p.c.heads;
     bool ok = true;
 
-    // One tile of `wk` into the ring as the CTA's tile number `count`, by this warp: lane = 4 * chunk + array.
-    const auto bring = [&](int i, uint32_t count) {
-        const int chunk = min(1 << p.c.page_shift, TILE), arr = lane & 3, off = (lane >> 2) * chunk;
-        const int key = (wk.it.span.first + i) * TILE + off, slot = count % STAGES;
+    // One tile of `wk` into the ring as the CTA's tile number `number`, by this warp: lane = 4 * chunk + array.  The warps
+    // take turns; the table's entry for a warp's next turn is fetched a turn ahead.
+    const int chunk = min(1 << p.c.page_shift, TILE), arr = lane & 3, off = (lane >> 2) * chunk;
+    int page = 0;
+    const auto fetch_page = [&](int i) {
+        const int key = (wk.it.span.first + i) * TILE + off;
+        if (i < wk.tb && off < TILE && key < wk.it.span.hi && key + chunk > wk.it.span.lo)
+            page = __ldg(p.s.table + (int64_t)wk.w.b * p.s.width + (key >> p.c.page_shift));
+    };
+    const auto bring = [&](int i, uint32_t number) {
+        const int key = (wk.it.span.first + i) * TILE + off, slot = number % STAGES;
         const bool wanted = off < TILE && key < wk.it.span.hi && key + chunk > wk.it.span.lo;
-        const int page = wanted ? __ldg(p.s.table + (int64_t)wk.w.b * p.s.width + (key >> p.c.page_shift)) : 0;
         const bool good = wanted && page >= 0 && page < p.c.pages;
         if (wanted && !good && arr == 0) *p.status = OXQ_ERR_INVALID_ARGUMENT;
-        if (ok && !tc::mbar_wait_warp(empty(slot), (count / STAGES & 1) ^ 1)) { ok = false; if (lane == 0) *p.status = OXQ_ERR_DEVICE_TIMEOUT; }
+        if (ok && !tc::mbar_wait_warp(empty(slot), (number / STAGES & 1) ^ 1)) { ok = false; if (lane == 0) *p.status = OXQ_ERR_DEVICE_TIMEOUT; }
         if (!ok) return;
         if (arr == 0 && off < TILE)
-            for (int k = 0; k < chunk; k += 16) sm.there[slot][(off + k) >> 4] = good ? 1 : 0;
+            for (int k = 0; k < chunk; k += 16) sm.there[slot][(off + k) >> 4] = good && key + k < wk.it.span.hi && key + k + 16 > wk.it.span.lo ? 1 : 0;
         const int row_bytes = arr < 2 ? D / 2 : NG * 4;
         const uint32_t bytes = good ? chunk * row_bytes : 0;
         const uint32_t all = __reduce_add_sync(0xffffffffu, bytes);
@@ -271,8 +280,12 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
     };
     uint32_t count = 0;                                               // of the CTA's tiles: the next one to use
     const auto prime = [&]() {                                        // the first tiles of a new piece of work
-        for (int i = wk.ta; i < wk.tb && i < wk.ta + LEAD; i++)
-            if ((int)((count + i - wk.ta) & 7) == warp) bring(i, count + i - wk.ta);
+        const int i = wk.ta + (int)((warp - count) & 7);
+        fetch_page(i);
+        if (i < wk.tb && i < wk.ta + LEAD) {
+            bring(i, count + i - wk.ta);
+            fetch_page(i + 8);
+        }
     };
 
     bool more = wk.next(p, ROWS);
@@ -342,13 +355,16 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
         const int all_hi = p.causal ? min(seq.len, pos0 + 1) : seq.len, all_lo = p.window > 0 ? pos1 + 1 - p.window : 0;
 
         for (int i = ta; i < tb; i++, count++) {
-            if (i + LEAD < tb && (int)((count + LEAD) & 7) == warp) bring(i + LEAD, count + LEAD);
+            if (i + LEAD < tb && (int)((count + LEAD) & 7) == warp) {
+                bring(i + LEAD, count + LEAD);
+                fetch_page(i + LEAD + 8);
+            }
             const int stage = count % STAGES;
             if (ok && !tc::mbar_wait(full(stage), count / STAGES & 1)) { ok = false; *p.status = OXQ_ERR_DEVICE_TIMEOUT; }
             __syncwarp();
             const int t0 = (it.span.first + i) * TILE + warp * 16;
             const unsigned char* ring = sm.ring[stage] + warp * (16 * (D / 2));
-            if (__all_sync(0xffffffffu, ok) && t0 < it.span.hi && t0 + 16 > it.span.lo && sm.there[stage][warp]) {
+            if (__all_sync(0xffffffffu, ok) && sm.there[stage][warp]) {
                 const unsigned char* kc = ring + St::KC + r * (D / 2) + c * (D / 8);
                 const unsigned char* vc = ring + St::VC + 2 * c * (D / 2) + r * (D / 16);
                 const unsigned char* pp = sm.ring[stage] + St::KP + (warp * 16 + r) * (NG * 4);
@@ -363,11 +379,11 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                 float2 x[NT][2];
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
-                    float s4[NT][4];
+                    float s4[NT][4], s5[NT][4];                       // two sums, so that a product need not wait for the one before it
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) s4[nt][e] = 0.0f;
+                        for (int e = 0; e < 4; e++) { s4[nt][e] = 0.0f; s5[nt][e] = 0.0f; }
 #pragma unroll
                     for (int i2 = 0; i2 < NB / NG; i2++) {
                         const int blk = g * (NB / NG) + i2;
@@ -376,7 +392,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                         for (int nt = 0; nt < NT; nt++) {
                             const uint4 qf = *reinterpret_cast<const uint4*>(&sm.q[(nt * 8 + r) * QPAD + blk * 32 + c * 8]);
                             mma_16816(s4[nt], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf.x, qf.y);
-                            mma_16816(s4[nt], u0 & 0x000F000Fu, u1 & 0x000F000Fu, u0 & 0x00F000F0u, u1 & 0x00F000F0u, qf.z, qf.w);
+                            mma_16816(s5[nt], u0 & 0x000F000Fu, u1 & 0x000F000Fu, u0 & 0x00F000F0u, u1 & 0x00F000F0u, qf.z, qf.w);
                         }
                     }
 #pragma unroll
@@ -384,7 +400,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                         const float ks = lo_f32(kp[h][g]), km = hi_f32(kp[h][g]);
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
-                            x[nt][h] = fma2(mul2(make_float2(s4[nt][2 * h], s4[nt][2 * h + 1]), both(ks)), qa[nt],
+                            x[nt][h] = fma2(mul2(add2(make_float2(s4[nt][2 * h], s4[nt][2 * h + 1]), make_float2(s5[nt][2 * h], s5[nt][2 * h + 1])), both(ks)), qa[nt],
                                             g == 0 ? mul2(both(km), qb[nt][0]) : fma2(both(km), qb[nt][g], x[nt][h]));
                     }
                 }
@@ -406,13 +422,14 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                     }
                 }
                 // ---- the rows' reference
-                float vs[2][NG], vm[2][NG], most[2];
+                float vs[2][NG], vm[2][NG];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int h = 0; h < 2; h++)
 #pragma unroll
                     for (int g = 0; g < NG; g++) { vs[h][g] = lo_f32(vp[h][g]); vm[h][g] = hi_f32(vp[h][g]); }
-                    most[h] = 8.0f - log2_floor(NG == 1 ? vs[h][0] : fmaxf(vs[h][0], vs[h][NG - 1]));
-                }
+                float large = log2_floor(vp[0][0], vp[1][0]);         // of this lane's two keys
+                if constexpr (NG == 2) large = fmaxf(large, log2_floor(vp[0][NG - 1], vp[1][NG - 1]));
+                const float most = 8.0f - large;
                 bool over = false;
                 float2 y[NT][2];
 #pragma unroll
@@ -420,12 +437,12 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         y[nt][h] = make_float2(x[nt][h].x - M[nt].x, x[nt][h].y - M[nt].y);
-                        over |= fmaxf(y[nt][h].x, y[nt][h].y) > most[h];
+                        over |= fmaxf(y[nt][h].x, y[nt][h].y) > most;
                     }
                 if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        float2 top = make_float2(fmaxf(x[nt][0].x - most[0], x[nt][1].x - most[1]) + 8.0f, fmaxf(x[nt][0].y - most[0], x[nt][1].y - most[1]) + 8.0f);
+                        float2 top = make_float2(fmaxf(x[nt][0].x, x[nt][1].x) + large, fmaxf(x[nt][0].y, x[nt][1].y) + large);
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) {
                             top.x = fmaxf(top.x, __shfl_xor_sync(0xffffffffu, top.x, o));
@@ -489,7 +506,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
         const bool whole = ta == 0 && tb == it.span.tiles;
         if (tid == 0 && wk.at == wk.end) {                            // the CTA's last piece: does its item begin here and go on?
             const int first = wk.w.at + it.start;
-            reinterpret_cast<Cut*>(p.ws)[blockIdx.x] = Cut{wk.w.b, it.head, it.rt, ta == 0 && tb < it.span.tiles ? line.part_of(first + it.span.tiles - 1) : -1};
+            reinterpret_cast<Cut*>(p.ws)[blockIdx.x] = Cut{seq.start, seq.n, it.head * row_blocks(p, seq, ROWS) + it.rt, ta == 0 && tb < it.span.tiles ? line.part_of(first + it.span.tiles - 1) : -1};
         }
         more = wk.next(p, ROWS);
         if (more) prime();                                            // under the end of this piece
@@ -575,43 +592,46 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(512) kv4_attn_join_kernel(AttnParams p) {
     constexpr int ROWS = NT * 8, D4 = D / 4, GROUPS = 512 / (8 * D4);
     __shared__ float4 part_o[GROUPS][8][D4];
-    __shared__ float part_l[GROUPS][8];
+    __shared__ float2 part_ml[GROUPS][8];
     pdl_trigger();
     pdl_wait();
     const int4 note = *reinterpret_cast<const int4*>(reinterpret_cast<const Cut*>(p.ws) + blockIdx.x);
     const int first = blockIdx.x, last = note.w;
     if (last < 0) return;
-    const SeqInfo seq = seq_info(p, note.x);
-    const int head = note.y, row0 = note.z * ROWS, rows = min(ROWS, seq.n * p.per - row0);
+    const SeqInfo seq = {note.x, note.y, 0, 0};
+    const int blocks = row_blocks(p, seq, ROWS), head = note.z / blocks, row0 = (note.z - head * blocks) * ROWS, rows = min(ROWS, seq.n * p.per - row0);
     const float* slots = p.ws + (gridDim.x) * (sizeof(Cut) / sizeof(float));
     const auto slot = [&](int k) { return slots + (int64_t)(k * 2 + (k == first ? 1 : 0)) * Slot<NT>::floats(D); };
     const int group = threadIdx.x / (8 * D4), rr = threadIdx.x / D4 % 8, d = threadIdx.x % D4 * 4;
     for (int r0 = 0; r0 < rows; r0 += 8) {
         const int row = r0 + rr;
-        float top = -1e30f;
-#pragma unroll 4
-        for (int k = first; k <= last; k++) top = fmaxf(top, slot(k)[ROWS * D + row]);
-        float sum = 0.0f;
+        float top = -1e30f, sum = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int k = first + group; k <= last; k += GROUPS) {
-            const float* s = slot(k);
-            const float f = exp2_approx(s[ROWS * D + row] - top);
-            const float4 v = *reinterpret_cast<const float4*>(s + row * D + d);
-            sum = fmaf(s[ROWS * D + ROWS + row], f, sum);
-            o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+        const auto take = [&](float m, float l, const float4& v) {
+            const float now = fmaxf(top, m), f = exp2_approx(top - now), g = exp2_approx(m - now);
+            top = now;
+            sum = fmaf(sum, f, l * g);
+            o.x = fmaf(o.x, f, v.x * g); o.y = fmaf(o.y, f, v.y * g); o.z = fmaf(o.z, f, v.z * g); o.w = fmaf(o.w, f, v.w * g);
+        };
+        for (int k0 = first + group; k0 <= last; k0 += 4 * GROUPS) {  // four parts' loads at a time
+            float m[4], l[4];
+            float4 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float* s = slot(min(k0 + u * GROUPS, last));
+                m[u] = s[ROWS * D + row]; l[u] = s[ROWS * D + ROWS + row]; v[u] = *reinterpret_cast<const float4*>(s + row * D + d);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (k0 + u * GROUPS <= last) take(m[u], l[u], v[u]);
         }
         __syncthreads();
         part_o[group][rr][d / 4] = o;
-        if (d == 0) part_l[group][rr] = sum;
+        if (d == 0) part_ml[group][rr] = make_float2(top, sum);
         __syncthreads();
         if (group == 0 && row < rows) {
 #pragma unroll
-            for (int g = 1; g < GROUPS; g++) {
-                const float4 v = part_o[g][rr][d / 4];
-                o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
-                sum += part_l[g][rr];
-            }
+            for (int g = 1; g < GROUPS; g++) take(part_ml[g][rr].x, part_ml[g][rr].y, part_o[g][rr][d / 4]);
             store_row<T>(p, seq, head, row0 + row, d, make_float2(o.x, o.y), top, sum);
             store_row<T>(p, seq, head, row0 + row, d + 2, make_float2(o.z, o.w), top, sum);
         }
