@@ -9,14 +9,15 @@
 // taken out again in f32.  q enters as f16 scaled per row by a power of two, so that the row's largest element lies in
 // [2^11, 2^12): exact for f16 and bf16 values down to 2^-25 of the row's largest.
 // The running reference M of a row is the maximum over its keys of x + log2(largest s of the value rows of the key and of
-// the one eight behind it, rounded down, at least -15), so that w stays in f16's range whatever the scales are; it moves only when a key exceeds it by 2^8 (w <= 2^9),
-// which one vote per 16 keys finds out.  l = sum p, the offsets' sum and all accumulators are f32.
+// its three companions 8, 16 and 24 places apart, rounded down, at least -15), so that w stays in f16's range whatever the scales are; it moves only when a key exceeds it by 2^8 (w <= 2^9),
+// which one vote per 32 keys finds out.  l = sum p, the offsets' sum and all accumulators are f32.
 // f16 outputs are finer than one f16 rounding of w; for them w is split into two f16 terms (two products).
 //
 // The shape.  mma.sync m16n8k16 with the keys as the 16 rows and 8 query rows as the columns (a kv head's query heads, and
 // the tokens of a run): S^T = K Q^T, then O^T = V^T P^T; P^T moves from accumulator to operand layout by movmatrix.
-// Eight warps of a CTA take 16 keys each of a tile of 128; bulk copies bring the tiles into a ring in shared memory, LEAD of
-// them ahead, issued by the warps in turn (a warp for nothing else would cost the others a quarter of their registers).  All tiles of all (sequence, kv head, block of query rows) items lie on one line, which the
+// Four warps of a CTA take 32 keys each of a tile of 128, the other four of the next tile; bulk copies bring the tiles into a
+// ring in shared memory, LEAD of them ahead, issued by the warps in turn (a warp for nothing else would cost the others a
+// quarter of their registers).  All tiles of all (sequence, kv head, block of query rows) items lie on one line, which the
 // CTAs cut into equal parts (lengths are known on the device only).  An item that lies inside one part is finished there; of a
 // cut one every CTA leaves o, M and l in the workspace and a second kernel joins them, in the order of the keys, so
 // results do not depend on timing.
@@ -26,7 +27,7 @@
 namespace oxq {
 namespace kv4 {
 
-constexpr int TILE = 128;               // keys per tile: 8 warps x 16
+constexpr int TILE = 128;               // keys per tile: 4 warps x 32
 constexpr int MIN_TILES = 2;            // tiles a CTA takes at least: a join of many small parts costs more than it brings
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -44,9 +45,11 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 __device__ __forceinline__ float lo_f32(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v & 0xFFFFu))); }
 __device__ __forceinline__ float hi_f32(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
-// floor(log2(s)) of the larger of two words' low halves, non-negative f16 numbers; -15 for those below 2^-14
-__device__ __forceinline__ float log2_floor(uint32_t a, uint32_t b) {
-    const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+// floor(log2(s)) of the largest of the words' low halves, non-negative f16 numbers; -15 for those below 2^-14
+template <int NG> __device__ __forceinline__ float log2_floor(const uint32_t (&v)[4][NG]) {
+    __half2 m = *reinterpret_cast<const __half2*>(&v[0][0]);
+#pragma unroll
+    for (int i = 1; i < 4 * NG; i++) m = __hmax2(m, *reinterpret_cast<const __half2*>(&v[i / NG][i % NG]));
     return (float)((int)((*reinterpret_cast<const uint32_t*>(&m) >> 10) & 31u) - 15);
 }
 template <int N> __device__ __forceinline__ void lds_words(uint32_t (&r)[N], const unsigned char* p) {
@@ -227,7 +230,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
     const auto empty = [&](int s) { return bars + 8 * (STAGES + s); };
     if (tid == 0) {
 #pragma unroll
-        for (int s = 0; s < STAGES; s++) { tc::mbar_init(full(s), 1); tc::mbar_init(empty(s), 8); }
+        for (int s = 0; s < STAGES; s++) { tc::mbar_init(full(s), 1); tc::mbar_init(empty(s), 4); }
         tc::fence_barrier_init();
     }
     pdl_trigger();
@@ -279,8 +282,11 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
         }
     };
     uint32_t count = 0;                                               // of the CTA's tiles: the next one to use
+    // Tile number t is for the group t & 1 of four warps; it is brought by warp (t >> 1) & 3 of the other group, LEAD = 3 tiles
+    // before, when that group has just left the slot.
+    const int group = warp >> 2;
     const auto prime = [&]() {                                        // the first tiles of a new piece of work
-        const int i = wk.ta + (int)((warp - count) & 7);
+        const int i = wk.ta + (int)((2 * (warp & 3) + 1 - group - count) & 7);
         fetch_page(i);
         if (i < wk.tb && i < wk.ta + LEAD) {
             bring(i, count + i - wk.ta);
@@ -354,61 +360,67 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
         const int pos0 = seq.len - seq.asked + p.by_per.div(row0), pos1 = seq.len - seq.asked + p.by_per.div(row0 + rows - 1);
         const int all_hi = p.causal ? min(seq.len, pos0 + 1) : seq.len, all_lo = p.window > 0 ? pos1 + 1 - p.window : 0;
 
-        for (int i = ta; i < tb; i++, count++) {
-            if (i + LEAD < tb && (int)((count + LEAD) & 7) == warp) {
-                bring(i + LEAD, count + LEAD);
+        for (int i = ta + (int)((group - count) & 1); i < tb; i += 2) {
+            const uint32_t number = count + i - ta;
+            if (i + LEAD < tb && (int)((number + LEAD) >> 1 & 3) == (warp & 3)) {
+                bring(i + LEAD, number + LEAD);
                 fetch_page(i + LEAD + 8);
             }
-            const int stage = count % STAGES;
-            if (ok && !tc::mbar_wait(full(stage), count / STAGES & 1)) { ok = false; *p.status = OXQ_ERR_DEVICE_TIMEOUT; }
-            __syncwarp();
-            const int t0 = (it.span.first + i) * TILE + warp * 16;
-            const unsigned char* ring = sm.ring[stage] + warp * (16 * (D / 2));
-            if (__all_sync(0xffffffffu, ok) && sm.there[stage][warp]) {
+            const int stage = number % STAGES;
+            if (ok && !tc::mbar_wait(full(stage), number / STAGES & 1)) { ok = false; *p.status = OXQ_ERR_DEVICE_TIMEOUT; }
+            const uint32_t there = *reinterpret_cast<const uint16_t*>(&sm.there[stage][2 * (warp & 3)]);
+            if (__all_sync(0xffffffffu, ok) && there) {
+                const int t0 = (it.span.first + i) * TILE + (warp & 3) * 32;
+                const unsigned char* ring = sm.ring[stage] + (warp & 3) * (32 * (D / 2));
                 const unsigned char* kc = ring + St::KC + r * (D / 2) + c * (D / 8);
                 const unsigned char* vc = ring + St::VC + 2 * c * (D / 2) + r * (D / 16);
-                const unsigned char* pp = sm.ring[stage] + St::KP + (warp * 16 + r) * (NG * 4);
-                uint32_t k[2][NB], kp[2][NG], vp[2][NG];
+                const unsigned char* pp = sm.ring[stage] + St::KP + ((warp & 3) * 32 + r) * (NG * 4);
+                // ---- x = scores of keys t0 + r + 8 h; sixteen keys are one matrix instruction's
+                float2 x[NT][4];
+                uint32_t vp[4][NG];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    lds_words(k[h], kc + 8 * h * (D / 2));
-                    lds_words(kp[h], pp + 8 * h * (NG * 4));
-                    lds_words(vp[h], pp + (St::VP - St::KP) + 8 * h * (NG * 4));
-                }
-                // ---- x = scores of keys t0 + r (first pair) and t0 + r + 8 (second)
-                float2 x[NT][2];
-#pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    float s4[NT][4], s5[NT][4];                       // two sums, so that a product need not wait for the one before it
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) { s4[nt][e] = 0.0f; s5[nt][e] = 0.0f; }
-#pragma unroll
-                    for (int i2 = 0; i2 < NB / NG; i2++) {
-                        const int blk = g * (NB / NG) + i2;
-                        const uint32_t w0 = k[0][blk], w1 = k[1][blk], u0 = w0 >> 8, u1 = w1 >> 8;
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            const uint4 qf = *reinterpret_cast<const uint4*>(&sm.q[(nt * 8 + r) * QPAD + blk * 32 + c * 8]);
-                            mma_16816(s4[nt], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf.x, qf.y);
-                            mma_16816(s5[nt], u0 & 0x000F000Fu, u1 & 0x000F000Fu, u0 & 0x00F000F0u, u1 & 0x00F000F0u, qf.z, qf.w);
-                        }
-                    }
+                for (int u = 0; u < 2; u++) {
+                    uint32_t k[2][NB], kp[2][NG];
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        const float ks = lo_f32(kp[h][g]), km = hi_f32(kp[h][g]);
+                        lds_words(k[h], kc + (16 * u + 8 * h) * (D / 2));
+                        lds_words(kp[h], pp + (16 * u + 8 * h) * (NG * 4));
+                        lds_words(vp[2 * u + h], pp + (St::VP - St::KP) + (16 * u + 8 * h) * (NG * 4));
+                    }
+#pragma unroll
+                    for (int g = 0; g < NG; g++) {
+                        float s4[NT][4];
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
-                            x[nt][h] = fma2(mul2(add2(make_float2(s4[nt][2 * h], s4[nt][2 * h + 1]), make_float2(s5[nt][2 * h], s5[nt][2 * h + 1])), both(ks)), qa[nt],
-                                            g == 0 ? mul2(both(km), qb[nt][0]) : fma2(both(km), qb[nt][g], x[nt][h]));
+#pragma unroll
+                            for (int e = 0; e < 4; e++) s4[nt][e] = 0.0f;
+#pragma unroll
+                        for (int i2 = 0; i2 < NB / NG; i2++) {
+                            const int blk = g * (NB / NG) + i2;
+                            const uint32_t w0 = k[0][blk], w1 = k[1][blk], u0 = w0 >> 8, u1 = w1 >> 8;
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                const uint4 qf = *reinterpret_cast<const uint4*>(&sm.q[(nt * 8 + r) * QPAD + blk * 32 + c * 8]);
+                                mma_16816(s4[nt], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf.x, qf.y);
+                                mma_16816(s4[nt], u0 & 0x000F000Fu, u1 & 0x000F000Fu, u0 & 0x00F000F0u, u1 & 0x00F000F0u, qf.z, qf.w);
+                            }
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const float ks = lo_f32(kp[h][g]), km = hi_f32(kp[h][g]);
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++)
+                                x[nt][2 * u + h] = fma2(mul2(make_float2(s4[nt][2 * h], s4[nt][2 * h + 1]), both(ks)), qa[nt],
+                                                        g == 0 ? mul2(both(km), qb[nt][0]) : fma2(both(km), qb[nt][g], x[nt][2 * u + h]));
+                        }
                     }
                 }
-                if (t0 < all_lo || t0 + 16 > all_hi) {
+                if (t0 < all_lo || t0 + 32 > all_hi || there != 0x0101u) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
+                    for (int h = 0; h < 4; h++) {
                         const int t = t0 + r + 8 * h;
-                        if (t >= seq.len)                             // rows behind the last key hold anything
+                        const bool have = t < seq.len && (there >> (8 * (h >> 1)) & 1u);
+                        if (!have)                                    // places behind the last key, and absent ones, hold anything
 #pragma unroll
                             for (int g = 0; g < NG; g++) vp[h][g] = 0;
 #pragma unroll
@@ -417,32 +429,31 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                             for (int e = 0; e < 2; e++) {
                                 const int pos = seq.len - seq.asked + p.by_per.div(row0 + nt * 8 + 2 * c + e);      // the row's own position
                                 const int vhi = p.causal ? min(seq.len, pos + 1) : seq.len, vlo = p.window > 0 ? pos + 1 - p.window : 0;
-                                if (t < vlo || t >= vhi) (e ? x[nt][h].y : x[nt][h].x) = -INFINITY;
+                                if (t < vlo || t >= vhi || !have) (e ? x[nt][h].y : x[nt][h].x) = -INFINITY;
                             }
                     }
                 }
                 // ---- the rows' reference
-                float vs[2][NG], vm[2][NG];
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int g = 0; g < NG; g++) { vs[h][g] = lo_f32(vp[h][g]); vm[h][g] = hi_f32(vp[h][g]); }
-                float large = log2_floor(vp[0][0], vp[1][0]);         // of this lane's two keys
-                if constexpr (NG == 2) large = fmaxf(large, log2_floor(vp[0][NG - 1], vp[1][NG - 1]));
+                float large = log2_floor(vp);                         // of this lane's four keys
                 const float most = 8.0f - large;
                 bool over = false;
-                float2 y[NT][2];
+                float2 y[NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                for (int nt = 0; nt < NT; nt++) {
+                    float top = -INFINITY;
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        y[nt][h] = make_float2(x[nt][h].x - M[nt].x, x[nt][h].y - M[nt].y);
-                        over |= fmaxf(y[nt][h].x, y[nt][h].y) > most;
+                    for (int h = 0; h < 4; h++) {
+                        y[nt][h] = add2(x[nt][h], make_float2(-M[nt].x, -M[nt].y));
+                        top = fmaxf(top, fmaxf(y[nt][h].x, y[nt][h].y));
                     }
+                    over |= top > most;
+                }
                 if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        float2 top = make_float2(fmaxf(x[nt][0].x, x[nt][1].x) + large, fmaxf(x[nt][0].y, x[nt][1].y) + large);
+                        float2 top = make_float2(-INFINITY, -INFINITY);
+#pragma unroll
+                        for (int h = 0; h < 4; h++) top = make_float2(fmaxf(top.x, x[nt][h].x + large), fmaxf(top.y, x[nt][h].y + large));
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) {
                             top.x = fmaxf(top.x, __shfl_xor_sync(0xffffffffu, top.x, o));
@@ -457,52 +468,58 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
 #pragma unroll
                         for (int q = 0; q < NS * 4; q++) { acc[q][nt][0] *= f.x; acc[q][nt][1] *= f.y; acc[q][nt][2] *= f.x; acc[q][nt][3] *= f.y; }
 #pragma unroll
-                        for (int h = 0; h < 2; h++) y[nt][h] = make_float2(x[nt][h].x - top.x, x[nt][h].y - top.y);
+                        for (int h = 0; h < 4; h++) y[nt][h] = make_float2(x[nt][h].x - top.x, x[nt][h].y - top.y);
                     }
                 }
                 // ---- p, its sums, and w = p s as the second product's operand
-                uint32_t wb[NT][NG][2], wc[NT][NG][2];
+                uint32_t wb[NT][NG][4], wc[NT][NG][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    float2 e2[2];
+                for (int h = 0; h < 4; h++) {
+                    float2 e2[NT];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        e2[h] = make_float2(exp2_approx(y[nt][h].x), exp2_approx(y[nt][h].y));
-                        l[nt] = add2(l[nt], e2[h]);
+                    for (int nt = 0; nt < NT; nt++) {
+                        e2[nt] = make_float2(exp2_approx(y[nt][h].x), exp2_approx(y[nt][h].y));
+                        l[nt] = add2(l[nt], e2[nt]);
                     }
 #pragma unroll
-                    for (int g = 0; g < NG; g++)
+                    for (int g = 0; g < NG; g++) {
+                        const float vs = lo_f32(vp[h][g]), vm = hi_f32(vp[h][g]);
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            po[nt][g] = fma2(e2[h], both(vm[h][g]), po[nt][g]);
-                            const float2 w = mul2(e2[h], both(vs[h][g]));
+                        for (int nt = 0; nt < NT; nt++) {
+                            po[nt][g] = fma2(e2[nt], both(vm), po[nt][g]);
+                            const float2 w = mul2(e2[nt], both(vs));
                             const uint32_t hi = pack_f16(w.x, w.y);
                             wb[nt][g][h] = transpose_8x8(hi);
                             if constexpr (SPLIT) wc[nt][g][h] = transpose_8x8(pack_f16(w.x - lo_f32(hi), w.y - hi_f32(hi)));
                         }
+                    }
                 }
                 // ---- O^T: rows r and r + 8 of block (s, j) are elements 64 s + 8 r + 2 j and + 1, the second one times 16
-                uint32_t v[4][NS];
 #pragma unroll
-                for (int h = 0; h < 4; h++) lds_words(v[h], vc + ((h & 1) + (h >> 1) * 8) * (D / 2));
+                for (int u = 0; u < 2; u++) {
+                    uint32_t v[4][NS];
 #pragma unroll
-                for (int s = 0; s < NS; s++)
+                    for (int h = 0; h < 4; h++) lds_words(v[h], vc + (16 * u + (h & 1) + (h >> 1) * 8) * (D / 2));
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        constexpr uint32_t kSel[4] = {0x4400u, 0x5511u, 0x6622u, 0x7733u};
-                        const int g = NG == 1 ? 0 : s;
-                        const uint32_t u = __byte_perm(v[0][s], v[1][s], kSel[j]), w = __byte_perm(v[2][s], v[3][s], kSel[j]);
-                        const uint32_t a0 = u & 0x000F000Fu, a1 = u & 0x00F000F0u, a2 = w & 0x000F000Fu, a3 = w & 0x00F000F0u;
+                    for (int s = 0; s < NS; s++)
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            mma_16816(acc[s * 4 + j][nt], a0, a1, a2, a3, wb[nt][g][0], wb[nt][g][1]);
-                            if constexpr (SPLIT) mma_16816(acc[s * 4 + j][nt], a0, a1, a2, a3, wc[nt][g][0], wc[nt][g][1]);
+                        for (int j = 0; j < 4; j++) {
+                            constexpr uint32_t kSel[4] = {0x4400u, 0x5511u, 0x6622u, 0x7733u};
+                            const int g = NG == 1 ? 0 : s;
+                            const uint32_t b0 = __byte_perm(v[0][s], v[1][s], kSel[j]), b1 = __byte_perm(v[2][s], v[3][s], kSel[j]);
+                            const uint32_t a0 = b0 & 0x000F000Fu, a1 = b0 & 0x00F000F0u, a2 = b1 & 0x000F000Fu, a3 = b1 & 0x00F000F0u;
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                mma_16816(acc[s * 4 + j][nt], a0, a1, a2, a3, wb[nt][g][2 * u], wb[nt][g][2 * u + 1]);
+                                if constexpr (SPLIT) mma_16816(acc[s * 4 + j][nt], a0, a1, a2, a3, wc[nt][g][2 * u], wc[nt][g][2 * u + 1]);
+                            }
                         }
-                    }
+                }
             }
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(empty(stage));
         }
+        count += tb - ta;
         const bool whole = ta == 0 && tb == it.span.tiles;
         if (tid == 0 && wk.at == wk.end) {                            // the CTA's last piece: does its item begin here and go on?
             const int first = wk.w.at + it.start;
