@@ -29,6 +29,7 @@ namespace kv4 {
 
 constexpr int TILE = 128;               // keys per tile: 4 warps x 32
 constexpr int MIN_TILES = 2;            // tiles a CTA takes at least: a join of many small parts costs more than it brings
+constexpr int SETUP = 3;                // what an item costs besides its tiles, in tiles: 3.3 us against 1.2 us a tile, measured
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -77,7 +78,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// The tiles of all items of one sequence, and of one item (row block rt).
+// The tiles of one item (row block rt), and the steps of all items of a kv head: an item is p.setup steps and one for each tile.
 struct Span { int first, tiles; int lo, hi; };          // first tile, how many (at least one), visible positions [lo, hi)
 __device__ __forceinline__ Span item_span(const AttnParams& p, const SeqInfo& q, int rt, int nr) {
     Span s;
@@ -90,9 +91,9 @@ __device__ __forceinline__ Span item_span(const AttnParams& p, const SeqInfo& q,
     return s;
 }
 __device__ __forceinline__ int row_blocks(const AttnParams& p, const SeqInfo& q, int nr) { return (q.n * p.per + nr - 1) / nr; }
-__device__ __forceinline__ int head_tiles(const AttnParams& p, const SeqInfo& q, int nr) {
+__device__ __forceinline__ int head_steps(const AttnParams& p, const SeqInfo& q, int nr) {
     int t = 0;
-    for (int rt = 0, e = row_blocks(p, q, nr); rt < e; rt++) t += item_span(p, q, rt, nr).tiles;
+    for (int rt = 0, e = row_blocks(p, q, nr); rt < e; rt++) t += p.setup + item_span(p, q, rt, nr).tiles;
     return t;
 }
 // Rows of this kernel: those of sequences with at most row_limit of them (0: all); the other kernel takes the rest.
@@ -102,18 +103,18 @@ __device__ __forceinline__ SeqInfo small_seq(const AttnParams& p, int b) {
     return q;
 }
 
-// The line of tiles, cut into `parts` parts that differ by one tile at most.
+// The line of steps, cut into `parts` parts that differ by one step at most.
 struct Line {
     int total, parts, each, more;
     __device__ __forceinline__ int bound(int k) const { return each * k + min(k, more); }
-    __device__ __forceinline__ int part_of(int tile) const {
+    __device__ __forceinline__ int part_of(int step) const {
         const int wide = more * (each + 1);
-        return tile < wide ? tile / (each + 1) : more + (tile - wide) / each;
+        return step < wide ? step / (each + 1) : more + (step - wide) / each;
     }
 };
-struct Where { int b, at; };            // sequence, and the line's position of its first tile
+struct Where { int b, at; };            // sequence, and the line's position of its first step
 
-// The line, and the sequence that holds tile bound(k), if k < parts.  Whole CTA of 256 threads: a scan over 256 sequences at a
+// The line, and the sequence that holds step bound(k), if k < parts.  Whole CTA of 256 threads: a scan over 256 sequences at a
 // time, once for the total and, where there are more of them, once again for the place.
 __device__ __forceinline__ Line find_part(const AttnParams& p, int nr, int ctas, int k, int* red, Where* found) {
     Line line;
@@ -122,7 +123,7 @@ __device__ __forceinline__ Line find_part(const AttnParams& p, int nr, int ctas,
         int base = 0, mine = 0, start = 0;
         for (int b0 = 0; b0 < p.s.seqs; b0 += 256) {
             const int b = b0 + (int)threadIdx.x;
-            mine = b < p.s.seqs ? head_tiles(p, small_seq(p, b), nr) * p.c.heads : 0;
+            mine = b < p.s.seqs ? head_steps(p, small_seq(p, b), nr) * p.c.heads : 0;
             int x = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -143,7 +144,7 @@ __device__ __forceinline__ Line find_part(const AttnParams& p, int nr, int ctas,
         }
         if (pass == 1) break;
         line.total = base;
-        line.parts = min(ctas, (base + MIN_TILES - 1) / MIN_TILES);
+        line.parts = base ? min(ctas, max(1, base / (MIN_TILES + p.setup))) : 0;
         line.each = line.parts ? (int)((unsigned)base / (unsigned)line.parts) : 0;
         line.more = base - line.each * line.parts;
         if (k >= line.parts) return line;
@@ -157,17 +158,17 @@ __device__ __forceinline__ Line find_part(const AttnParams& p, int nr, int ctas,
     return line;
 }
 
-// An item of a sequence: which one holds tile `in_seq` of the sequence's own line.
+// An item of a sequence: which one holds step `in_seq` of the sequence's own line.
 struct Item { int head, rt, start; Span span; };
 __device__ __forceinline__ Item find_item(const AttnParams& p, const SeqInfo& q, int nr, int in_seq) {
     Item it;
-    const int per_head = head_tiles(p, q, nr);
+    const int per_head = head_steps(p, q, nr);
     it.head = (int)((unsigned)in_seq / (unsigned)per_head);
     it.start = it.head * per_head;
     for (it.rt = 0;; it.rt++) {
         it.span = item_span(p, q, it.rt, nr);
-        if (in_seq < it.start + it.span.tiles) return it;
-        it.start += it.span.tiles;
+        if (in_seq < it.start + p.setup + it.span.tiles) return it;
+        it.start += p.setup + it.span.tiles;
     }
 }
 
@@ -180,21 +181,24 @@ struct alignas(16) Cut { int start, n, block, last; };     // the sequence's fir
 
 // Part of the tiles of one item that a CTA works on.
 struct Work {
-    Where w; SeqInfo seq; int seq_tiles, at, end;
+    Where w; SeqInfo seq; int seq_steps, at, end;
     Item it; int ta, tb;
     __device__ __forceinline__ bool next(const AttnParams& p, int nr) {
-        if (at >= end) return false;
-        while (at >= w.at + seq_tiles) {                              // on to the next sequence that has tiles
-            w.at += seq_tiles;
-            if (++w.b >= p.s.seqs) return false;                      // cannot happen: `end` is within the line
-            seq = small_seq(p, w.b);
-            seq_tiles = head_tiles(p, seq, nr) * p.c.heads;
+        while (at < end) {
+            while (at >= w.at + seq_steps) {                          // on to the next sequence that has any
+                w.at += seq_steps;
+                if (++w.b >= p.s.seqs) return false;                  // cannot happen: `end` is within the line
+                seq = small_seq(p, w.b);
+                seq_steps = head_steps(p, seq, nr) * p.c.heads;
+            }
+            it = find_item(p, seq, nr, at - w.at);
+            const int pos = at - w.at - it.start, all = p.setup + it.span.tiles, upto = min(all, pos + (end - at));
+            ta = max(0, pos - p.setup);
+            tb = max(0, upto - p.setup);
+            at += upto - pos;
+            if (tb > ta) return true;                                 // else only steps of its setup are here, and its tiles in the next part
         }
-        it = find_item(p, seq, nr, at - w.at);
-        ta = at - w.at - it.start;
-        tb = min(it.span.tiles, ta + (end - at));
-        at += tb - ta;
-        return true;
+        return false;
     }
 };
 
@@ -237,17 +241,15 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
     pdl_wait();
 
     const Line line = find_part(p, ROWS, gridDim.x, blockIdx.x, sm.red, &sm.found);
-    if ((int)blockIdx.x >= line.parts) {
-        if (tid == 0) reinterpret_cast<Cut*>(p.ws)[blockIdx.x] = Cut{0, 0, 0, -1};
-        return;
-    }
+    if (tid == 0) reinterpret_cast<Cut*>(p.ws)[blockIdx.x] = Cut{0, 0, 0, -1};
+    if ((int)blockIdx.x >= line.parts) return;
     float* slots = p.ws + gridDim.x * (sizeof(Cut) / sizeof(float));
     Work wk;
     wk.at = line.bound(blockIdx.x);
     wk.end = line.bound(blockIdx.x + 1);
     wk.w = sm.found;
     wk.seq = small_seq(p, wk.w.b);
-    wk.seq_tiles = head_tiles(p, wk.seq, ROWS) * p.c.heads;
+    wk.seq_steps = head_steps(p, wk.seq, ROWS) * p.c.heads;
     bool ok = true;
 
     // One tile of `wk` into the ring as the CTA's tile number `number`, by this warp: lane = 4 * chunk + array.  The warps
@@ -294,7 +296,22 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
         }
     };
 
+    // The rows of a piece of work, requested a piece ahead: D / 8 threads a row, eight elements each.
+    Vec16<T> query;
+    const auto fetch_rows = [&]() {
+        const int row = wk.it.rt * ROWS + tid / (D / 8);
+        *reinterpret_cast<uint4*>(&query) = make_uint4(0, 0, 0, 0);
+        if (tid < ROWS * (D / 8) && row < wk.seq.n * p.per) {
+            const T* src = (const T*)p.q + (int64_t)(wk.seq.start + p.by_per.div(row)) * p.q_ts + (int64_t)(wk.it.head * p.per + p.by_per.mod(row)) * p.q_hs + tid % (D / 8) * 8;
+            if (p.q_vec) query = ld16(src);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; e++) query.v[e] = src[e];
+        }
+    };
+
     bool more = wk.next(p, ROWS);
+    if (more) fetch_rows();
     __syncthreads();                                                  // the barriers are set up
     if (more) prime();
     while (more) {
@@ -303,25 +320,13 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
         const int ta = wk.ta, tb = wk.tb;
         const int row0 = it.rt * ROWS, rows = min(ROWS, seq.n * p.per - row0);
 
-        // ---- the query rows: D / 8 threads a row
+        // ---- the query rows
         __syncthreads();
-        for (int i = tid; i < ROWS * (D / 8); i += 256) {
-            const int row = i / (D / 8), g = i % (D / 8);
+        if (tid < ROWS * (D / 8)) {
+            const int row = tid / (D / 8), g = tid % (D / 8);
             float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) f[e] = 0.0f;
-            if (row < rows) {
-                const int j = p.by_per.div(row0 + row), qh = it.head * p.per + p.by_per.mod(row0 + row);
-                const T* src = (const T*)p.q + (int64_t)(seq.start + j) * p.q_ts + (int64_t)qh * p.q_hs + g * 8;
-                if (p.q_vec) {
-                    const Vec16<T> v = ld16(src);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) f[e] = Elem<T>::to_f32(v.v[e]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) f[e] = Elem<T>::to_f32(src[e]);
-                }
-            }
+            for (int e = 0; e < 8; e++) f[e] = Elem<T>::to_f32(query.v[e]);
             float top = 0.0f, sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; e++) { top = fmaxf(top, fabsf(f[e])); sum += f[e]; }
@@ -521,12 +526,13 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
         }
         count += tb - ta;
         const bool whole = ta == 0 && tb == it.span.tiles;
-        if (tid == 0 && wk.at == wk.end) {                            // the CTA's last piece: does its item begin here and go on?
-            const int first = wk.w.at + it.start;
-            reinterpret_cast<Cut*>(p.ws)[blockIdx.x] = Cut{seq.start, seq.n, it.head * row_blocks(p, seq, ROWS) + it.rt, ta == 0 && tb < it.span.tiles ? line.part_of(first + it.span.tiles - 1) : -1};
-        }
+        if (tid == 0 && ta == 0 && tb < it.span.tiles)                // an item that begins here and goes on: the CTA's last piece
+            reinterpret_cast<Cut*>(p.ws)[blockIdx.x] = Cut{seq.start, seq.n, it.head * row_blocks(p, seq, ROWS) + it.rt, line.part_of(wk.w.at + it.start + p.setup + it.span.tiles - 1)};
         more = wk.next(p, ROWS);
-        if (more) prime();                                            // under the end of this piece
+        if (more) {                                                   // under the end of this piece
+            fetch_rows();
+            prime();
+        }
 
         // ---- join the warps: common reference, then four slabs, two warps each one after the other
 #pragma unroll
@@ -674,7 +680,7 @@ static int32_t launch_rows(oxq_handle* h, const AttnParams& p, int64_t most_tile
         ready.set(h->device, 1);
     }
     OXQ_CUDA(h, oxq_launch(kernel, ctas, 256, bytes, h->stream, p));
-    if (ctas > 1 && item_tiles > MIN_TILES) OXQ_CUDA(h, oxq_launch(kv4_attn_join_kernel<T, D, NT>, ctas, 512, 0, h->stream, p));
+    if (ctas > 1 && item_tiles > MIN_TILES + SETUP) OXQ_CUDA(h, oxq_launch(kv4_attn_join_kernel<T, D, NT>, ctas, 512, 0, h->stream, p));
     return OXQ_OK;
 }
 
@@ -769,7 +775,7 @@ int32_t oxq_kv4_attention(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_k
     p.status = h->dev_status;
     // the most tiles that there can be for the row kernel: every row block of every sequence over a whole table row
     const int nt = plan.nt;
-    const int64_t item_tiles = (p.s.width * cache->page_size + TILE - 1) / TILE + 1;
+    const int64_t item_tiles = (p.s.width * cache->page_size + TILE - 1) / TILE + 1 + SETUP;
     const int64_t blocks = plan.tiles ? p.s.seqs * (ROWS_MOST / (nt * 8)) : (p.s.tokens * per + nt * 8 - 1) / (nt * 8) + p.s.seqs;
     const int64_t items = plan.rows ? blocks * p.c.heads : 0;
     if (items > INT32_MAX / item_tiles) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 attention: more work than one call counts (2^31 tiles of %d keys)", TILE);
@@ -783,6 +789,7 @@ int32_t oxq_kv4_attention(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_k
         p.row_limit = (int)ROWS_MOST;
     }
     p.ws = (float*)workspace;
+    p.setup = most >= 8ll * attn_ctas(h, nt) ? SETUP : 0;             // where a CTA has a few tiles only, all count
     if (a->dtype == OXQ_BF16)
         return nt == 1 ? launch_dims<__nv_bfloat16, 1>(h, cache, p, most, item_tiles) : launch_dims<__nv_bfloat16, 2>(h, cache, p, most, item_tiles);
     return nt == 1 ? launch_dims<__half, 1>(h, cache, p, most, item_tiles) : launch_dims<__half, 2>(h, cache, p, most, item_tiles);

@@ -29,6 +29,7 @@ struct AttnParams {
     float scale_log2;                                   // scale * log2(e)
     int causal, window;                                 // window 0: none
     int row_limit, row_min;                             // sequences of at most row_limit rows (0: all) are the row kernel's, of more than row_min the tile kernel's
+    int setup;                                          // row kernel: steps an item costs besides its tiles
     int parts, out_vec;                                 // tile kernel: CTAs that share an item's keys; 16-byte stores allowed
     float* ws;
     int32_t* status;
