@@ -44,8 +44,8 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float lo_f32(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v & 0xFFFFu))); }
-__device__ __forceinline__ float hi_f32(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
+__device__ __forceinline__ float lo_f32(uint32_t v) { return __low2float(*reinterpret_cast<const __half2*>(&v)); }
+__device__ __forceinline__ float hi_f32(uint32_t v) { return __high2float(*reinterpret_cast<const __half2*>(&v)); }
 // floor(log2(s)) of the largest of the words' low halves, non-negative f16 numbers; -15 for those below 2^-14
 template <int NG> __device__ __forceinline__ float log2_floor(const uint32_t (&v)[4][NG]) {
     __half2 m = *reinterpret_cast<const __half2*>(&v[0][0]);
@@ -57,24 +57,6 @@ template <int N> __device__ __forceinline__ void lds_words(uint32_t (&r)[N], con
     if constexpr (N == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p); r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
     else if constexpr (N == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p); r[0] = v.x; r[1] = v.y; }
     else r[0] = *reinterpret_cast<const uint32_t*>(p);
-}
-// two f32 operations in one instruction
-__device__ __forceinline__ uint64_t pair_bits(float2 v) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y)); return r; }
-__device__ __forceinline__ float2 bits_pair(uint64_t b) { float2 v; asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(b)); return v; }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
-    return bits_pair(r);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
-    return bits_pair(r);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
-    return bits_pair(r);
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
@@ -218,6 +200,7 @@ struct Smem {
     unsigned char there[STAGES][8];
     int red[8];
     Where found;
+    Work work[2];                       // this piece and the next: kept here, so that the main loop has the registers
 };
 
 template <typename T, int D, int NG, int NT>
@@ -256,20 +239,20 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
     // take turns; the table's entry for a warp's next turn is fetched a turn ahead.
     const int chunk = min(1 << p.c.page_shift, TILE), arr = lane & 3, off = (lane >> 2) * chunk;
     int page = 0;
+    struct { const int32_t* table; int head, first, lo, hi, tb; } src;                // of the piece whose tiles are being brought
     const auto fetch_page = [&](int i) {
-        const int key = (wk.it.span.first + i) * TILE + off;
-        if (i < wk.tb && off < TILE && key < wk.it.span.hi && key + chunk > wk.it.span.lo)
-            page = __ldg(p.s.table + (int64_t)wk.w.b * p.s.width + (key >> p.c.page_shift));
+        const int key = (src.first + i) * TILE + off;
+        if (i < src.tb && off < TILE && key < src.hi && key + chunk > src.lo) page = __ldg(src.table + (key >> p.c.page_shift));
     };
     const auto bring = [&](int i, uint32_t number) {
-        const int key = (wk.it.span.first + i) * TILE + off, slot = number % STAGES;
-        const bool wanted = off < TILE && key < wk.it.span.hi && key + chunk > wk.it.span.lo;
+        const int key = (src.first + i) * TILE + off, slot = number % STAGES;
+        const bool wanted = off < TILE && key < src.hi && key + chunk > src.lo;
         const bool good = wanted && page >= 0 && page < p.c.pages;
         if (wanted && !good && arr == 0) *p.status = OXQ_ERR_INVALID_ARGUMENT;
         if (ok && !tc::mbar_wait_warp(empty(slot), (number / STAGES & 1) ^ 1)) { ok = false; if (lane == 0) *p.status = OXQ_ERR_DEVICE_TIMEOUT; }
         if (!ok) return;
         if (arr == 0 && off < TILE)
-            for (int k = 0; k < chunk; k += 16) sm.there[slot][(off + k) >> 4] = good && key + k < wk.it.span.hi && key + k + 16 > wk.it.span.lo ? 1 : 0;
+            for (int k = 0; k < chunk; k += 16) sm.there[slot][(off + k) >> 4] = good && key + k < src.hi && key + k + 16 > src.lo ? 1 : 0;
         const int row_bytes = arr < 2 ? D / 2 : NG * 4;
         const uint32_t bytes = good ? chunk * row_bytes : 0;
         const uint32_t all = __reduce_add_sync(0xffffffffu, bytes);
@@ -277,17 +260,18 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
         if (lane == 0) tc::mbar_arrive_expect_tx(full(slot), all);
         __syncwarp();
         if (good) {
-            const unsigned char* src = arr == 0 ? p.c.kc : arr == 1 ? p.c.vc : reinterpret_cast<const unsigned char*>(arr == 2 ? p.c.kp : p.c.vp);
+            const unsigned char* from = arr == 0 ? p.c.kc : arr == 1 ? p.c.vc : reinterpret_cast<const unsigned char*>(arr == 2 ? p.c.kp : p.c.vp);
             const uint32_t to = arr == 0 ? St::KC : arr == 1 ? St::VC : arr == 2 ? St::KP : St::VP;
-            const int64_t row = (((int64_t)page * p.c.heads + wk.it.head) << p.c.page_shift) + (key & ((1 << p.c.page_shift) - 1));
-            tc::bulk_load(tc::smem_u32(&sm.ring[slot][to]) + off * row_bytes, src + row * row_bytes, bytes, full(slot));
+            const int64_t row = (((int64_t)page * p.c.heads + src.head) << p.c.page_shift) + (key & ((1 << p.c.page_shift) - 1));
+            tc::bulk_load(tc::smem_u32(&sm.ring[slot][to]) + off * row_bytes, from + row * row_bytes, bytes, full(slot));
         }
     };
     uint32_t count = 0;                                               // of the CTA's tiles: the next one to use
     // Tile number t is for the group t & 1 of four warps; it is brought by warp (t >> 1) & 3 of the other group, LEAD = 3 tiles
     // before, when that group has just left the slot.
     const int group = warp >> 2;
-    const auto prime = [&]() {                                        // the first tiles of a new piece of work
+    const auto prime = [&](const Work& wk) {                          // the first tiles of a new piece of work
+        src = {p.s.table + (int64_t)wk.w.b * p.s.width, wk.it.head, wk.it.span.first, wk.it.span.lo, wk.it.span.hi, wk.tb};
         const int i = wk.ta + (int)((2 * (warp & 3) + 1 - group - count) & 7);
         fetch_page(i);
         if (i < wk.tb && i < wk.ta + LEAD) {
@@ -298,7 +282,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
 
     // The rows of a piece of work, requested a piece ahead: D / 8 threads a row, eight elements each.
     Vec16<T> query;
-    const auto fetch_rows = [&]() {
+    const auto fetch_rows = [&](const Work& wk) {
         const int row = wk.it.rt * ROWS + tid / (D / 8);
         *reinterpret_cast<uint4*>(&query) = make_uint4(0, 0, 0, 0);
         if (tid < ROWS * (D / 8) && row < wk.seq.n * p.per) {
@@ -311,14 +295,15 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
     };
 
     bool more = wk.next(p, ROWS);
-    if (more) fetch_rows();
+    if (more) fetch_rows(wk);
     __syncthreads();                                                  // the barriers are set up
-    if (more) prime();
-    while (more) {
-        const SeqInfo seq = wk.seq;
-        const Item it = wk.it;
-        const int ta = wk.ta, tb = wk.tb;
-        const int row0 = it.rt * ROWS, rows = min(ROWS, seq.n * p.per - row0);
+    if (more) prime(wk);
+    for (int turn = 0; more; turn ^= 1) {
+        const int ta = wk.ta, tb = wk.tb, len = wk.seq.len, before = wk.seq.len - wk.seq.asked, first = wk.it.span.first;
+        const int row0 = wk.it.rt * ROWS;
+        // keys that every row of the block sees need no mask
+        const int pos0 = before + p.by_per.div(row0), pos1 = before + p.by_per.div(min(row0 + ROWS, wk.seq.n * p.per) - 1);
+        const int all_hi = p.causal ? min(len, pos0 + 1) : len, all_lo = p.window > 0 ? pos1 + 1 - p.window : 0;
 
         // ---- the query rows
         __syncthreads();
@@ -343,6 +328,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
             if (g == 0) sm.a[row] = p.scale_log2 * pow2_of(min(24 - 11 + ex, 127));
             if (g % (D / 8 / NG) == 0) sm.bsum[row][g / (D / 8 / NG)] = p.scale_log2 * sum;
         }
+        if (tid == 0) sm.work[turn] = wk;
         __syncthreads();
 
         // ---- this warp's constants and accumulators; columns 2 c and 2 c + 1 of each block of eight rows are this lane's
@@ -361,21 +347,19 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[i][nt][e] = 0.0f;
-        // keys that every row of the block sees need no mask
-        const int pos0 = seq.len - seq.asked + p.by_per.div(row0), pos1 = seq.len - seq.asked + p.by_per.div(row0 + rows - 1);
-        const int all_hi = p.causal ? min(seq.len, pos0 + 1) : seq.len, all_lo = p.window > 0 ? pos1 + 1 - p.window : 0;
 
         for (int i = ta + (int)((group - count) & 1); i < tb; i += 2) {
             const uint32_t number = count + i - ta;
+            const int stage = number % STAGES;
+            if (ok && !tc::mbar_wait(full(stage), number / STAGES & 1)) { ok = false; *p.status = OXQ_ERR_DEVICE_TIMEOUT; }
+            __syncwarp();
             if (i + LEAD < tb && (int)((number + LEAD) >> 1 & 3) == (warp & 3)) {
                 bring(i + LEAD, number + LEAD);
                 fetch_page(i + LEAD + 8);
             }
-            const int stage = number % STAGES;
-            if (ok && !tc::mbar_wait(full(stage), number / STAGES & 1)) { ok = false; *p.status = OXQ_ERR_DEVICE_TIMEOUT; }
             const uint32_t there = *reinterpret_cast<const uint16_t*>(&sm.there[stage][2 * (warp & 3)]);
             if (__all_sync(0xffffffffu, ok) && there) {
-                const int t0 = (it.span.first + i) * TILE + (warp & 3) * 32;
+                const int t0 = (first + i) * TILE + (warp & 3) * 32;
                 const unsigned char* ring = sm.ring[stage] + (warp & 3) * (32 * (D / 2));
                 const unsigned char* kc = ring + St::KC + r * (D / 2) + c * (D / 8);
                 const unsigned char* vc = ring + St::VC + 2 * c * (D / 2) + r * (D / 16);
@@ -415,8 +399,8 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                             const float ks = lo_f32(kp[h][g]), km = hi_f32(kp[h][g]);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++)
-                                x[nt][2 * u + h] = fma2(mul2(make_float2(s4[nt][2 * h], s4[nt][2 * h + 1]), both(ks)), qa[nt],
-                                                        g == 0 ? mul2(both(km), qb[nt][0]) : fma2(both(km), qb[nt][g], x[nt][2 * u + h]));
+                                x[nt][2 * u + h] = make_float2(fmaf(s4[nt][2 * h] * ks, qa[nt].x, g == 0 ? km * qb[nt][0].x : fmaf(km, qb[nt][g].x, x[nt][2 * u + h].x)),
+                                                               fmaf(s4[nt][2 * h + 1] * ks, qa[nt].y, g == 0 ? km * qb[nt][0].y : fmaf(km, qb[nt][g].y, x[nt][2 * u + h].y)));
                         }
                     }
                 }
@@ -424,7 +408,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
 #pragma unroll
                     for (int h = 0; h < 4; h++) {
                         const int t = t0 + r + 8 * h;
-                        const bool have = t < seq.len && (there >> (8 * (h >> 1)) & 1u);
+                        const bool have = t < len && (there >> (8 * (h >> 1)) & 1u);
                         if (!have)                                    // places behind the last key, and absent ones, hold anything
 #pragma unroll
                             for (int g = 0; g < NG; g++) vp[h][g] = 0;
@@ -432,8 +416,8 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                             for (int e = 0; e < 2; e++) {
-                                const int pos = seq.len - seq.asked + p.by_per.div(row0 + nt * 8 + 2 * c + e);      // the row's own position
-                                const int vhi = p.causal ? min(seq.len, pos + 1) : seq.len, vlo = p.window > 0 ? pos + 1 - p.window : 0;
+                                const int pos = before + p.by_per.div(row0 + nt * 8 + 2 * c + e);      // the row's own position
+                                const int vhi = p.causal ? min(len, pos + 1) : len, vlo = p.window > 0 ? pos + 1 - p.window : 0;
                                 if (t < vlo || t >= vhi || !have) (e ? x[nt][h].y : x[nt][h].x) = -INFINITY;
                             }
                     }
@@ -448,7 +432,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                     float top = -INFINITY;
 #pragma unroll
                     for (int h = 0; h < 4; h++) {
-                        y[nt][h] = add2(x[nt][h], make_float2(-M[nt].x, -M[nt].y));
+                        y[nt][h] = make_float2(x[nt][h].x - M[nt].x, x[nt][h].y - M[nt].y);
                         top = fmaxf(top, fmaxf(y[nt][h].x, y[nt][h].y));
                     }
                     over |= top > most;
@@ -467,9 +451,9 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                         top = make_float2(fmaxf(top.x, M[nt].x), fmaxf(top.y, M[nt].y));
                         const float2 f = make_float2(exp2_approx(M[nt].x - top.x), exp2_approx(M[nt].y - top.y));
                         M[nt] = top;
-                        l[nt] = mul2(l[nt], f);
+                        l[nt].x *= f.x; l[nt].y *= f.y;
 #pragma unroll
-                        for (int g = 0; g < NG; g++) po[nt][g] = mul2(po[nt][g], f);
+                        for (int g = 0; g < NG; g++) { po[nt][g].x *= f.x; po[nt][g].y *= f.y; }
 #pragma unroll
                         for (int q = 0; q < NS * 4; q++) { acc[q][nt][0] *= f.x; acc[q][nt][1] *= f.y; acc[q][nt][2] *= f.x; acc[q][nt][3] *= f.y; }
 #pragma unroll
@@ -484,15 +468,15 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
                         e2[nt] = make_float2(exp2_approx(y[nt][h].x), exp2_approx(y[nt][h].y));
-                        l[nt] = add2(l[nt], e2[nt]);
+                        l[nt].x += e2[nt].x; l[nt].y += e2[nt].y;
                     }
 #pragma unroll
                     for (int g = 0; g < NG; g++) {
                         const float vs = lo_f32(vp[h][g]), vm = hi_f32(vp[h][g]);
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
-                            po[nt][g] = fma2(e2[nt], both(vm), po[nt][g]);
-                            const float2 w = mul2(e2[nt], both(vs));
+                            po[nt][g] = make_float2(fmaf(e2[nt].x, vm, po[nt][g].x), fmaf(e2[nt].y, vm, po[nt][g].y));
+                            const float2 w = make_float2(e2[nt].x * vs, e2[nt].y * vs);
                             const uint32_t hi = pack_f16(w.x, w.y);
                             wb[nt][g][h] = transpose_8x8(hi);
                             if constexpr (SPLIT) wc[nt][g][h] = transpose_8x8(pack_f16(w.x - lo_f32(hi), w.y - hi_f32(hi)));
@@ -525,14 +509,13 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
             if (lane == 0) tc::mbar_arrive(empty(stage));
         }
         count += tb - ta;
-        const bool whole = ta == 0 && tb == it.span.tiles;
-        if (tid == 0 && ta == 0 && tb < it.span.tiles)                // an item that begins here and goes on: the CTA's last piece
-            reinterpret_cast<Cut*>(p.ws)[blockIdx.x] = Cut{seq.start, seq.n, it.head * row_blocks(p, seq, ROWS) + it.rt, line.part_of(wk.w.at + it.start + p.setup + it.span.tiles - 1)};
+        const Work done = sm.work[turn];
+        if (tid == 0 && done.ta == 0 && done.tb < done.it.span.tiles)  // an item that begins here and goes on: the CTA's last piece
+            reinterpret_cast<Cut*>(p.ws)[blockIdx.x] = Cut{done.seq.start, done.seq.n, done.it.head * row_blocks(p, done.seq, ROWS) + done.it.rt,
+                                                           line.part_of(done.w.at + done.it.start + p.setup + done.it.span.tiles - 1)};
+        wk = done;
         more = wk.next(p, ROWS);
-        if (more) {                                                   // under the end of this piece
-            fetch_rows();
-            prime();
-        }
+        if (more) fetch_rows(wk);
 
         // ---- join the warps: common reference, then four slabs, two warps each one after the other
 #pragma unroll
@@ -553,6 +536,11 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
             }
         }
         __syncthreads();
+        // Only now, when every warp has left the ring: a parity wait tells a phase from the one before it, not from the one two
+        // before, and nothing else keeps a warp that is done from running that far ahead of a slow one of its own group.  In the
+        // loop above the order does it: tile t + 3 is brought after t has been seen, into the place of t - 2 that the same warp
+        // has seen before, so whoever has seen t + 3 may wait for t + 5 in the place of t.
+        if (more) prime(wk);
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             if ((warp >> 2) == half) {
@@ -583,7 +571,9 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
             }
             __syncthreads();
         }
-        float* slot = whole ? nullptr : slots + (int64_t)(blockIdx.x * 2 + (ta > 0 ? 0 : 1)) * Slot<NT>::floats(D);
+        const bool whole = done.ta == 0 && done.tb == done.it.span.tiles;
+        const int rows = min(ROWS, done.seq.n * p.per - done.it.rt * ROWS);
+        float* slot = whole ? nullptr : slots + (int64_t)(blockIdx.x * 2 + (done.ta > 0 ? 0 : 1)) * Slot<NT>::floats(D);
         for (int i = tid; i < ROWS * (D / 4); i += 256) {
             const int row = i / (D / 4), d = (i % (D / 4)) * 4;
             float top = sm.m[0][row];
@@ -602,10 +592,14 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                 *reinterpret_cast<float4*>(slot + row * D + d) = o;
                 if (d == 0) { slot[ROWS * D + row] = top; slot[ROWS * D + ROWS + row] = sum; }
             } else if (row < rows) {
-                store_row<T>(p, seq, it.head, row0 + row, d, make_float2(o.x, o.y), top, sum);
-                store_row<T>(p, seq, it.head, row0 + row, d + 2, make_float2(o.z, o.w), top, sum);
+                store_row<T>(p, done.seq, done.it.head, done.it.rt * ROWS + row, d, make_float2(o.x, o.y), top, sum);
+                store_row<T>(p, done.seq, done.it.head, done.it.rt * ROWS + row, d + 2, make_float2(o.z, o.w), top, sum);
             }
         }
+    }
+    if (!ok) {                                                        // a wait ran out: what was asked for still has to land, with a limit
+        const uint64_t t0 = tc::globaltimer_ns();
+        while (tc::globaltimer_ns() - t0 < 1000000ull) { }
     }
 }
 
