@@ -7,31 +7,19 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 from . import _build
 
 _i32, _i64, _sz, _vp, _int, _f32p = C.c_int32, C.c_int64, C.c_size_t, C.c_void_p, C.c_int, C.c_void_p
 
 
-class ResidualNorm(C.Structure):            # oxq_residual_norm
-    _fields_ = [("y", _vp), ("y_ld", _i64), ("dtype", _i32), ("residual", _vp), ("residual_ld", _i64), ("residual_dtype", _i32), ("gate", _vp),
-                ("gate_ld", _i64), ("post_weight", _vp), ("weight", _vp), ("alpha", C.c_float), ("eps", C.c_float), ("residual_out", _vp),
-                ("residual_out_ld", _i64)]
-
-
-class Kv4CacheDesc(C.Structure):            # oxq_kv4_cache
-    _fields_ = [("k_codes", _vp), ("k_params", _vp), ("v_codes", _vp), ("v_params", _vp), ("pages", _i64), ("page_size", _i32), ("heads", _i32),
-                ("dim", _i32), ("group", _i32)]
-
-
-class Kv4BatchDesc(C.Structure):            # oxq_kv4_batch
-    _fields_ = [("block_table", _vp), ("table_width", _i64), ("seq_lens", _vp), ("cu_tokens", _vp), ("seqs", _i64), ("tokens", _i64)]
-
-
-class Kv4AttentionArgs(C.Structure):        # oxq_kv4_attention_args
-    _fields_ = [("q", _vp), ("q_token_stride", _i64), ("q_head_stride", _i64), ("out", _vp), ("out_token_stride", _i64), ("out_head_stride", _i64),
-                ("lse", _vp), ("q_heads", _i64), ("max_tokens", _i64), ("window", _i64), ("scale", C.c_float), ("causal", _i32), ("dtype", _i32)]
-
+# Descriptor structs of the header as packed bytes (native alignment): a bytes object passes as a pointer to its contents.
+# Field by field in the header's order; a fraction of the cost of a ctypes.Structure per call.
+residual_norm = struct.Struct("@PqiPqiPqPPffPq").pack           # oxq_residual_norm
+kv4_cache = struct.Struct("@PPPPqiiii").pack                    # oxq_kv4_cache
+kv4_batch = struct.Struct("@PqPPqq").pack                       # oxq_kv4_batch
+kv4_attention_args = struct.Struct("@PqqPqqPqqqfii").pack       # oxq_kv4_attention_args
 
 # symbol -> (restype, argtypes); mirrors include/oxq.h one to one
 SIGNATURES = {

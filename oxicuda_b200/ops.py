@@ -3,6 +3,7 @@ every computation happens inside liboxq_b200.so.  Function names follow the C en
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -44,7 +45,7 @@ class Handle:
 
     def sync_stream(self):
         """Follow torch's current stream (BlasHandle::set_stream)."""
-        s = torch.cuda.current_stream(self.device).cuda_stream
+        s = torch._C._cuda_getCurrentRawStream(self.device)          # current_stream() without building a Stream object
         if s != self._stream:
             raise_for_status(self.lib.oxq_set_stream(self._h, C.c_void_p(s)))
             self._stream = s
@@ -635,8 +636,8 @@ def _residual_norm_args(y, residual, weight, post_weight, gate, alpha, eps, resi
     r_out = torch.empty((rows, cols), dtype=residual.dtype, device=y.device) if residual_out is None else residual_out
     if r_out.shape != y.shape or r_out.dtype != residual.dtype:
         raise QuantError("DimensionMismatch", f"residual_out {tuple(r_out.shape)} {r_out.dtype} for {tuple(residual.shape)} {residual.dtype}", 4)
-    return r_out, _ffi.ResidualNorm(y.data_ptr(), _row_stride(y), _DT[y.dtype], residual.data_ptr(), _row_stride(residual), _DT[residual.dtype],
-                                    None if gate is None else gate.data_ptr(), gate_ld, None if post_weight is None else post_weight.data_ptr(),
+    return r_out, _ffi.residual_norm(y.data_ptr(), _row_stride(y), _DT[y.dtype], residual.data_ptr(), _row_stride(residual), _DT[residual.dtype],
+                                    0 if gate is None else gate.data_ptr(), gate_ld, 0 if post_weight is None else post_weight.data_ptr(),
                                     weight.data_ptr(), alpha, eps, r_out.data_ptr(), _row_stride(r_out))
 
 
@@ -666,7 +667,7 @@ def residual_rmsnorm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
         _chk(out, y.dtype)
         if out.shape != y.shape or out.device != y.device:
             raise TypeError(f"out must be {tuple(y.shape)} on {y.device}")
-    handle(y.device.index).call("oxq_residual_rmsnorm", C.byref(args), y.shape[0], y.shape[1], out.data_ptr())
+    handle(y.device.index).call("oxq_residual_rmsnorm", args, y.shape[0], y.shape[1], out.data_ptr())
     return r_out, out
 
 
@@ -678,7 +679,7 @@ def residual_rmsnorm_fp8(y: torch.Tensor, residual: torch.Tensor, weight: torch.
     _chk(scale, torch.float32)
     _same_device(y, scale)
     q = torch.empty(y.shape, dtype=torch.uint8, device=y.device)
-    handle(y.device.index).call("oxq_residual_rmsnorm_fp8", C.byref(args), y.shape[0], y.shape[1], scale.data_ptr(), q.data_ptr())
+    handle(y.device.index).call("oxq_residual_rmsnorm_fp8", args, y.shape[0], y.shape[1], scale.data_ptr(), q.data_ptr())
     return r_out, q
 
 
@@ -688,11 +689,14 @@ def residual_rmsnorm_int8_rows(y: torch.Tensor, residual: torch.Tensor, weight: 
     r_out, args = _residual_norm_args(y, residual, weight, post_weight, gate, alpha, eps, residual_out)
     q = torch.empty(y.shape, dtype=torch.int8, device=y.device)
     sc = torch.empty(y.shape[0], dtype=torch.float32, device=y.device)
-    handle(y.device.index).call("oxq_residual_rmsnorm_int8_rows", C.byref(args), y.shape[0], y.shape[1], q.data_ptr(), sc.data_ptr())
+    handle(y.device.index).call("oxq_residual_rmsnorm_int8_rows", args, y.shape[0], y.shape[1], q.data_ptr(), sc.data_ptr())
     return r_out, q, sc
 
 
 # ------------------------------------------------------------------------------------------- 4-bit key / value cache
+
+_HALVES = (torch.bfloat16, torch.float16)
+
 
 class Kv4Cache:
     """A paged pool of 4-bit keys and values: codes uint8 [pages, heads, page_size, dim / 2] and params f16 [pages, heads, page_size, dim / group, 2]
@@ -700,22 +704,27 @@ class Kv4Cache:
     (crates/oxicuda-quant/src/scheme/minmax.rs:146-167, :226-232) with a float offset.  dim is 64 or 128, group 64 or 128, page_size a power of two
     from 16 to 4096."""
 
+    __slots__ = ("k_codes", "k_params", "v_codes", "v_params", "pages", "heads", "page_size", "dim", "group", "device", "_desc", "_shape")
+
     def __init__(self, k_codes: torch.Tensor, k_params: torch.Tensor, v_codes: torch.Tensor, v_params: torch.Tensor):
-        if k_codes.dim() != 4 or k_params.dim() != 5 or k_params.shape[4] != 2 or k_codes.shape[:3] != k_params.shape[:3] or \
-                v_codes.shape != k_codes.shape or v_params.shape != k_params.shape:
+        cs, ps = k_codes.shape, k_params.shape
+        if len(cs) != 4 or len(ps) != 5 or ps[4] != 2 or cs[:3] != ps[:3] or v_codes.shape != cs or v_params.shape != ps:
             from .errors import QuantError
-            raise QuantError("DimensionMismatch", f"codes {tuple(k_codes.shape)}, {tuple(v_codes.shape)} with params {tuple(k_params.shape)}, {tuple(v_params.shape)}", 4)
+            raise QuantError("DimensionMismatch", f"codes {tuple(cs)}, {tuple(v_codes.shape)} with params {tuple(ps)}, {tuple(v_params.shape)}", 4)
+        device = k_codes.device
         for t, dt in ((k_codes, torch.uint8), (v_codes, torch.uint8), (k_params, torch.float16), (v_params, torch.float16)):
-            _chk(t, dt)
-        _same_device(k_codes, k_params, v_codes, v_params)
+            if t.dtype != dt or not t.is_contiguous() or t.device != device:
+                raise TypeError(f"expected contiguous {dt} tensors on one device")
+        if device.type != "cuda":
+            raise TypeError("expected CUDA tensors")
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
-        self.pages, self.heads, self.page_size, half = k_codes.shape
+        self.pages, self.heads, self.page_size, half = cs
         self.dim = 2 * half
-        groups = k_params.shape[3]
-        self.group = self.dim // groups if groups and self.dim % groups == 0 else 0
-        self.device = k_codes.device
-        self._desc = _ffi.Kv4CacheDesc(k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(), self.pages, self.page_size,
-                                       self.heads, self.dim, self.group)
+        self.group = self.dim // ps[3] if ps[3] and self.dim % ps[3] == 0 else 0
+        self.device = device
+        self._shape = (self.page_size, self.heads, self.dim, self.group)
+        self._desc = _ffi.kv4_cache(k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(), self.pages, self.page_size, self.heads,
+                                    self.dim, self.group)
 
     @classmethod
     def empty(cls, pages: int, page_size: int, heads: int, dim: int, group: int = 64, device=None):
@@ -726,45 +735,58 @@ class Kv4Cache:
         return cls(codes[0], params[0], codes[1], params[1])
 
 
-def _kv4_batch(cache: Kv4Cache, block_table, seq_lens, cu_tokens, tokens: int):
-    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 or cu_tokens.dtype != torch.int32:
+def _kv4_batch(cache: Kv4Cache, block_table, seq_lens, cu_tokens, tokens: int) -> bytes:
+    if not (block_table.dtype == seq_lens.dtype == cu_tokens.dtype == torch.int32):
         raise TypeError("block_table, seq_lens and cu_tokens are int32")
-    seqs = seq_lens.numel()
-    if block_table.dim() != 2 or block_table.shape[0] != seqs or cu_tokens.numel() != seqs + 1:
+    shape, seqs = block_table.shape, seq_lens.numel()
+    if len(shape) != 2 or shape[0] != seqs or cu_tokens.numel() != seqs + 1:
         from .errors import QuantError
-        raise QuantError("DimensionMismatch", f"block_table {tuple(block_table.shape)}, seq_lens {tuple(seq_lens.shape)}, cu_tokens {tuple(cu_tokens.shape)}", 4)
+        raise QuantError("DimensionMismatch", f"block_table {tuple(shape)}, seq_lens {tuple(seq_lens.shape)}, cu_tokens {tuple(cu_tokens.shape)}", 4)
     dev = cache.device
     if block_table.device != dev or seq_lens.device != dev or cu_tokens.device != dev:
         raise TypeError(f"expected block_table, seq_lens and cu_tokens on {dev}")
     if not (block_table.is_contiguous() and seq_lens.is_contiguous() and cu_tokens.is_contiguous()):
         raise TypeError("expected contiguous block_table, seq_lens and cu_tokens")
-    return _ffi.Kv4BatchDesc(block_table.data_ptr(), block_table.shape[1], seq_lens.data_ptr(), cu_tokens.data_ptr(), seqs, tokens)
+    return _ffi.kv4_batch(block_table.data_ptr(), shape[1], seq_lens.data_ptr(), cu_tokens.data_ptr(), seqs, tokens)
 
 
 def _kv4_rows(t: torch.Tensor, heads: int, cache: Kv4Cache, what: str, dtypes):
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != cache.dim:
+    """The tensor's token and head strides, if it is rows of the cache's kind."""
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != cache.dim:
         from .errors import QuantError
-        raise QuantError("DimensionMismatch", f"{what} {tuple(t.shape)}, expected [tokens, {heads}, {cache.dim}]", 4)
+        raise QuantError("DimensionMismatch", f"{what} {tuple(shape)}, expected [tokens, {heads}, {cache.dim}]", 4)
     if t.dtype not in dtypes:
         raise TypeError(f"{what}: expected dtype in {tuple(dtypes)}, got {t.dtype}")
     if t.device != cache.device:
         raise TypeError(f"{what}: expected a tensor on {cache.device}")
-    if t.stride(2) != 1:
+    stride = t.stride()
+    if stride[2] != 1:
         raise TypeError(f"{what}: expected rows of adjacent elements")
+    return stride[0], stride[1]
+
+
+@functools.lru_cache(maxsize=4096)
+def _kv4_workspace(device_index: int, cache_shape: tuple, width: int, seqs: int, tokens: int, q_heads: int, max_tokens: int) -> int:
+    """A size: it follows from the shapes alone, so it is asked for once."""
+    cache = _ffi.kv4_cache(256, 256, 256, 256, 1, *cache_shape)
+    batch = _ffi.kv4_batch(256, width, 256, 256, seqs, tokens)
+    n = C.c_size_t(0)
+    handle(device_index).call("oxq_kv4_attention_workspace_bytes", cache, batch, q_heads, max_tokens, C.byref(n))
+    return n.value
 
 
 def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_tokens: torch.Tensor):
     """Quantises keys and values [tokens, heads, dim] (f32, bf16 or f16; any token and head strides) into the pool.  Sequence b owns tokens
     cu_tokens[b]:cu_tokens[b + 1], its last ones of seq_lens[b]; position p lives in page block_table[b, p // page_size].  Rows behind the last
     sequence are not read."""
-    _kv4_rows(k, cache.heads, cache, "k", _DT)
-    _kv4_rows(v, cache.heads, cache, "v", (k.dtype,))
+    kt, kh = _kv4_rows(k, cache.heads, cache, "k", _DT)
+    vt, vh = _kv4_rows(v, cache.heads, cache, "v", (k.dtype,))
     if v.shape != k.shape:
         from .errors import QuantError
         raise QuantError("DimensionMismatch", f"k {tuple(k.shape)} vs v {tuple(v.shape)}", 4)
     batch = _kv4_batch(cache, block_table, seq_lens, cu_tokens, k.shape[0])
-    handle(cache.device.index).call("oxq_kv4_append", C.byref(cache._desc), C.byref(batch), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                    v.stride(1), _DT[k.dtype])
+    handle(cache.device.index).call("oxq_kv4_append", cache._desc, batch, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DT[k.dtype])
     return cache
 
 
@@ -783,17 +805,15 @@ def kv4_read(cache: Kv4Cache, block_table: torch.Tensor, seq_lens: torch.Tensor,
                 raise TypeError(f"{what}: expected a contiguous tensor of {shape}")
         outs.append(t)
     batch = _kv4_batch(cache, block_table, seq_lens, cu_tokens, shape[0])
-    handle(cache.device.index).call("oxq_kv4_read", C.byref(cache._desc), C.byref(batch), outs[0].data_ptr(), outs[1].data_ptr(), _DT[dtype])
+    handle(cache.device.index).call("oxq_kv4_read", cache._desc, batch, outs[0].data_ptr(), outs[1].data_ptr(), _DT[dtype])
     return outs[0], outs[1]
 
 
 def kv4_attention_workspace_bytes(cache: Kv4Cache, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_tokens: torch.Tensor, tokens: int, q_heads: int,
                                   max_tokens: int = 0) -> int:
     """Bytes of workspace that kv4_attention needs for `tokens` rows of q_heads heads; depends on the arguments' shapes only, not on their contents."""
-    batch = _kv4_batch(cache, block_table, seq_lens, cu_tokens, tokens)
-    n = C.c_size_t(0)
-    handle(cache.device.index).call("oxq_kv4_attention_workspace_bytes", C.byref(cache._desc), C.byref(batch), q_heads, max_tokens, C.byref(n))
-    return n.value
+    _kv4_batch(cache, block_table, seq_lens, cu_tokens, tokens)
+    return _kv4_workspace(cache.device.index, cache._shape, block_table.shape[1], seq_lens.numel(), tokens, q_heads, max_tokens)
 
 
 def kv4_attention(q: torch.Tensor, cache: Kv4Cache, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_tokens: torch.Tensor, max_tokens: int = 0,
@@ -804,36 +824,38 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, block_table: torch.Tensor, s
     A query that sees no key gives zeros (and -inf in lse).  max_tokens: the most tokens a sequence has in this call, 0 if it is not known; it
     only chooses kernels.  Returns out, or (out, lse f32 [tokens, q_heads]) if want_lse or lse is given.  Rows behind the last sequence
     are left as they were.  `workspace` (uint8, kv4_attention_workspace_bytes) may be given to allocate nothing; overlapping calls need one each."""
-    if q.dim() != 3 or q.shape[1] == 0 or cache.heads == 0 or q.shape[1] % cache.heads != 0:
+    shape = q.shape
+    if len(shape) != 3 or shape[1] == 0 or cache.heads == 0 or shape[1] % cache.heads != 0:
         from .errors import QuantError
-        raise QuantError("DimensionMismatch", f"q {tuple(q.shape)} over {cache.heads} kv heads", 4)
-    tokens, heads = q.shape[0], q.shape[1]
-    _kv4_rows(q, heads, cache, "q", (torch.bfloat16, torch.float16))
+        raise QuantError("DimensionMismatch", f"q {tuple(shape)} over {cache.heads} kv heads", 4)
+    tokens, heads = shape[0], shape[1]
+    qt, qh = _kv4_rows(q, heads, cache, "q", _HALVES)
+    dev = cache.device
     if out is None:
-        out = torch.empty((tokens, heads, cache.dim), dtype=q.dtype, device=q.device)
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+        ot, oh = heads * cache.dim, cache.dim
     else:
-        _kv4_rows(out, heads, cache, "out", (q.dtype,))
+        ot, oh = _kv4_rows(out, heads, cache, "out", (q.dtype,))
         if out.shape[0] != tokens:
             raise TypeError(f"out: expected {tokens} tokens, got {out.shape[0]}")
     if lse is not None:
         _chk(lse, torch.float32)
-        if tuple(lse.shape) != (tokens, heads) or lse.device != q.device:
-            raise TypeError(f"lse: expected {(tokens, heads)} on {q.device}")
+        if tuple(lse.shape) != (tokens, heads) or lse.device != dev:
+            raise TypeError(f"lse: expected {(tokens, heads)} on {dev}")
     elif want_lse:
-        lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
+        lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev)
     batch = _kv4_batch(cache, block_table, seq_lens, cu_tokens, tokens)
-    h = handle(cache.device.index)
     if workspace is None:
-        n = C.c_size_t(0)
-        h.call("oxq_kv4_attention_workspace_bytes", C.byref(cache._desc), C.byref(batch), heads, max_tokens, C.byref(n))
-        workspace = torch.empty(max(n.value, 16), dtype=torch.uint8, device=q.device)
+        n = _kv4_workspace(dev.index, cache._shape, block_table.shape[1], seq_lens.numel(), tokens, heads, max_tokens)
+        workspace = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
     else:
         _chk(workspace, torch.uint8)
-        if workspace.device != q.device:
-            raise TypeError(f"workspace: expected a tensor on {q.device}")
-    args = _ffi.Kv4AttentionArgs(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(),
-                                 heads, max_tokens, window, cache.dim ** -0.5 if scale is None else scale, 1 if causal else 0, _DT[q.dtype])
-    h.call("oxq_kv4_attention", C.byref(cache._desc), C.byref(batch), C.byref(args), workspace.data_ptr(), workspace.numel())
+        if workspace.device != dev:
+            raise TypeError(f"workspace: expected a tensor on {dev}")
+        n = workspace.numel()
+    args = _ffi.kv4_attention_args(q.data_ptr(), qt, qh, out.data_ptr(), ot, oh, 0 if lse is None else lse.data_ptr(), heads, max_tokens, window,
+                                   cache.dim ** -0.5 if scale is None else scale, 1 if causal else 0, _DT[q.dtype])
+    handle(dev.index).call("oxq_kv4_attention", cache._desc, batch, args, workspace.data_ptr(), n)
     return out if lse is None else (out, lse)
 
 

@@ -30,11 +30,11 @@ def _descs(**kw):
         for d in (c, b, a):
             if k in d:
                 d[k] = v
-    return _ffi.Kv4CacheDesc(**c), _ffi.Kv4BatchDesc(**b), _ffi.Kv4AttentionArgs(**a)
+    return tuple(pack(*[0 if v is None else v for v in d.values()]) for pack, d in ((_ffi.kv4_cache, c), (_ffi.kv4_batch, b), (_ffi.kv4_attention_args, a)))
 
 
 def _append(lib, h, c, b, k=0xA000, v=0xB000, strides=(256, 128, 256, 128), dtype=1):
-    return lib.oxq_kv4_append(h, C.byref(c), C.byref(b), k, strides[0], strides[1], v, strides[2], strides[3], dtype)
+    return lib.oxq_kv4_append(h, c, b, k, strides[0], strides[1], v, strides[2], strides[3], dtype)
 
 
 POOL = [("dim", 96, 13), ("dim", 256, 13), ("group", 32, 2), ("group", 0, 2), ("page_size", 8, 15), ("page_size", 48, 15), ("page_size", 8192, 15), ("pages", 0, 10),
@@ -46,8 +46,8 @@ POOL = [("dim", 96, 13), ("dim", 256, 13), ("group", 32, 2), ("group", 0, 2), ("
 def test_pool_and_batch(lib, fake, key, value, status):
     c, b, a = _descs(**{key: value})
     assert _append(lib, fake, c, b) == status
-    assert lib.oxq_kv4_read(fake, C.byref(c), C.byref(b), 0xA000, 0xB000, 1) == status
-    assert lib.oxq_kv4_attention(fake, C.byref(c), C.byref(b), C.byref(a), 0x10000, 1 << 30) == status
+    assert lib.oxq_kv4_read(fake, c, b, 0xA000, 0xB000, 1) == status
+    assert lib.oxq_kv4_attention(fake, c, b, a, 0x10000, 1 << 30) == status
     assert lib.oxq_last_error_string(fake)
 
 
@@ -65,15 +65,15 @@ def test_append_and_read(lib, fake):
     assert _append(lib, fake, c, b, k=None) == 15 and _append(lib, fake, c, b, v=None) == 15
     assert _append(lib, fake, c, b, strides=(-256, 128, 256, 128)) == 15
     assert _append(lib, None, c, b) == 15
-    assert lib.oxq_kv4_append(fake, None, C.byref(b), 0xA000, 1, 1, 0xB000, 1, 1, 1) == 15
-    read = lambda k, v, dt=1: lib.oxq_kv4_read(fake, C.byref(c), C.byref(b), k, v, dt)  # noqa: E731
+    assert lib.oxq_kv4_append(fake, None, b, 0xA000, 1, 1, 0xB000, 1, 1, 1) == 15
+    read = lambda k, v, dt=1: lib.oxq_kv4_read(fake, c, b, k, v, dt)  # noqa: E731
     assert read(0xA000, 0xB000) == OK_BUT_NO_DEVICE
     assert read(0xA008, 0xB000) == 15 and read(0xA000, None) == 15 and read(0xA000, 0xB000, 9) == 15
     for kw in ({"tokens": 0}, {"seqs": 0}):              # nothing to do is not an error
         c, b, a = _descs(**kw)
         assert _append(lib, fake, c, b, k=None, v=None) == 0
-        assert lib.oxq_kv4_read(fake, C.byref(c), C.byref(b), None, None, 1) == 0
-        assert lib.oxq_kv4_attention(fake, C.byref(c), C.byref(b), C.byref(a), None, 0) == 0
+        assert lib.oxq_kv4_read(fake, c, b, None, None, 1) == 0
+        assert lib.oxq_kv4_attention(fake, c, b, a, None, 0) == 0
 
 
 @pytest.mark.parametrize("key,value,status", [
@@ -82,18 +82,18 @@ def test_append_and_read(lib, fake):
     ("lse", 0xC000, OK_BUT_NO_DEVICE), ("window", 1 << 40, OK_BUT_NO_DEVICE), ("causal", 0, OK_BUT_NO_DEVICE)])
 def test_attention(lib, fake, key, value, status):
     c, b, a = _descs(**{key: value})
-    assert lib.oxq_kv4_attention(fake, C.byref(c), C.byref(b), C.byref(a), 0x10000, 1 << 30) == status
+    assert lib.oxq_kv4_attention(fake, c, b, a, 0x10000, 1 << 30) == status
 
 
 def test_attention_window_and_workspace(lib, fake):
     c, b, a = _descs(window=4, causal=0)
-    assert lib.oxq_kv4_attention(fake, C.byref(c), C.byref(b), C.byref(a), 0x10000, 1 << 30) == 15
+    assert lib.oxq_kv4_attention(fake, c, b, a, 0x10000, 1 << 30) == 15
     c, b, a = _descs()
-    assert lib.oxq_kv4_attention(fake, C.byref(c), C.byref(b), C.byref(a), None, 1 << 30) == 11
-    assert lib.oxq_kv4_attention(fake, C.byref(c), C.byref(b), C.byref(a), 0x10008, 1 << 30) == 11
-    assert lib.oxq_kv4_attention(fake, C.byref(c), C.byref(b), None, 0x10000, 1 << 30) == 15
+    assert lib.oxq_kv4_attention(fake, c, b, a, None, 1 << 30) == 11
+    assert lib.oxq_kv4_attention(fake, c, b, a, 0x10008, 1 << 30) == 11
+    assert lib.oxq_kv4_attention(fake, c, b, None, 0x10000, 1 << 30) == 15
     n = C.c_size_t(0)
-    size = lambda c, b, heads, most, out=C.byref(n): lib.oxq_kv4_attention_workspace_bytes(fake, C.byref(c), C.byref(b), heads, most, out)  # noqa: E731
+    size = lambda c, b, heads, most, out=C.byref(n): lib.oxq_kv4_attention_workspace_bytes(fake, c, b, heads, most, out)  # noqa: E731
     assert size(c, b, 7, 0) == 12 and size(c, b, 8, -1) == 10 and size(c, b, 8, 0, None) == 15
     assert size(_descs(dim=96)[0], b, 8, 0) == 13
     assert size(c, b, 8, 0) == 0
@@ -106,12 +106,12 @@ def test_residual_norm(lib, fake):
         a = dict(y=0x1000, y_ld=64, dtype=1, residual=0x2000, residual_ld=64, residual_dtype=1, gate=0x3000, gate_ld=0, post_weight=0x4000, weight=0x5000, alpha=1.0,
                  eps=1e-5, residual_out=0x6000, residual_out_ld=64)
         a.update(kw)
-        s = _ffi.ResidualNorm(**a)
+        s = _ffi.residual_norm(*[0 if v is None else v for v in a.values()])
         if fn == "oxq_residual_rmsnorm":
-            return lib.oxq_residual_rmsnorm(fake, C.byref(s), rows, cols, out)
+            return lib.oxq_residual_rmsnorm(fake, s, rows, cols, out)
         if fn == "oxq_residual_rmsnorm_int8_rows":
-            return lib.oxq_residual_rmsnorm_int8_rows(fake, C.byref(s), rows, cols, out, scale)
-        return lib.oxq_residual_rmsnorm_fp8(fake, C.byref(s), rows, cols, scale, out)
+            return lib.oxq_residual_rmsnorm_int8_rows(fake, s, rows, cols, out, scale)
+        return lib.oxq_residual_rmsnorm_fp8(fake, s, rows, cols, scale, out)
 
     for fn in ("oxq_residual_rmsnorm", "oxq_residual_rmsnorm_fp8", "oxq_residual_rmsnorm_int8_rows"):
         assert call(fn=fn) == OK_BUT_NO_DEVICE
