@@ -613,46 +613,52 @@ def bias_add_(y: torch.Tensor, bias: torch.Tensor):
 
 # ------------------------------------------------------------------------------------------- between two blocks
 
+def _row_stride(t, shape):
+    """Leading dimension of a matrix whose rows are adjacent elements."""
+    if t.is_contiguous():
+        return shape[1]
+    stride = t.stride()
+    if stride[1] != 1 and shape[1] > 1:
+        raise TypeError("expected rows of adjacent elements")
+    return stride[0] if shape[0] > 1 else max(stride[0], shape[1])
+
+
 def _residual_norm_args(y, residual, weight, post_weight, gate, alpha, eps, residual_out):
     from .errors import QuantError
-    if y.dim() != 2 or residual.shape != y.shape:
-        raise QuantError("DimensionMismatch", f"y {tuple(y.shape)} vs residual {tuple(residual.shape)}", 4)
-    rows, cols = y.shape
-    _same_device(y, residual, weight, post_weight, gate, residual_out)
-    if y.dtype not in _DT or residual.dtype not in (y.dtype, torch.float32):
-        raise TypeError(f"y is f32, bf16 or f16 and residual the same or f32, got {y.dtype} and {residual.dtype}")
+    shape, index = y.shape, y.get_device()
+    if len(shape) != 2 or residual.shape != shape:
+        raise QuantError("DimensionMismatch", f"y {tuple(shape)} vs residual {tuple(residual.shape)}", 4)
+    rows, cols = shape
+    dt = y.dtype
+    if dt not in _DT or residual.dtype not in (dt, torch.float32):
+        raise TypeError(f"y is f32, bf16 or f16 and residual the same or f32, got {dt} and {residual.dtype}")
+    if index < 0 or residual.get_device() != index:
+        raise TypeError("expected CUDA tensors on one device")
     for w in (weight, post_weight):
         if w is not None:
-            _chk(w, torch.float32)
+            if w.dtype is not torch.float32 or not w.is_contiguous() or w.get_device() != index:
+                raise TypeError(f"expected contiguous float32 weights on {y.device}")
             if w.numel() != cols:
                 raise QuantError("DimensionMismatch", f"expected {cols} weights, got {w.numel()}", 4)
-    gate_ld = 0
+    y_ld = _row_stride(y, shape)
+    gate_ptr = gate_ld = 0
     if gate is not None:
-        if gate.dtype != y.dtype or tuple(gate.shape) not in ((cols,), (rows, cols)):
-            raise QuantError("DimensionMismatch", f"gate {tuple(gate.shape)} {gate.dtype} for y {tuple(y.shape)} {y.dtype}", 4)
-        gate_ld = _row_stride(gate) if gate.dim() == 2 else 0
-        if gate.stride(-1) != 1 and cols > 1:
-            raise TypeError("expected gate rows of adjacent elements")
-    r_out = torch.empty((rows, cols), dtype=residual.dtype, device=y.device) if residual_out is None else residual_out
-    if r_out.shape != y.shape or r_out.dtype != residual.dtype:
-        raise QuantError("DimensionMismatch", f"residual_out {tuple(r_out.shape)} {r_out.dtype} for {tuple(residual.shape)} {residual.dtype}", 4)
-    return r_out, _ffi.residual_norm(y.data_ptr(), _row_stride(y), _DT[y.dtype], residual.data_ptr(), _row_stride(residual), _DT[residual.dtype],
-                                    0 if gate is None else gate.data_ptr(), gate_ld, 0 if post_weight is None else post_weight.data_ptr(),
-                                    weight.data_ptr(), alpha, eps, r_out.data_ptr(), _row_stride(r_out))
-
-
-def _same_device(first, *rest):
-    if not first.is_cuda:
-        raise TypeError("expected a CUDA tensor")
-    for t in rest:
-        if t is not None and t.device != first.device:
-            raise TypeError(f"expected tensors on {first.device}, got one on {t.device}")
-
-
-def _row_stride(t):
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise TypeError("expected rows of adjacent elements")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+        if gate.dtype != dt or tuple(gate.shape) not in ((cols,), (rows, cols)) or gate.get_device() != index:
+            raise QuantError("DimensionMismatch", f"gate {tuple(gate.shape)} {gate.dtype} for y {tuple(shape)} {dt} on {y.device}", 4)
+        if gate.dim() == 2:
+            gate_ld = _row_stride(gate, shape)
+        elif not gate.is_contiguous():
+            raise TypeError("expected a gate of adjacent elements")
+        gate_ptr = gate.data_ptr()
+    r_ld = _row_stride(residual, shape)
+    if residual_out is None:
+        residual_out, ro_ld = residual.new_empty(shape), cols
+    else:
+        if residual_out.shape != shape or residual_out.dtype != residual.dtype or residual_out.get_device() != index:
+            raise QuantError("DimensionMismatch", f"residual_out {tuple(residual_out.shape)} {residual_out.dtype} for {tuple(shape)} {residual.dtype} on {y.device}", 4)
+        ro_ld = _row_stride(residual_out, shape)
+    return residual_out, _ffi.residual_norm(y.data_ptr(), y_ld, _DT[dt], residual.data_ptr(), r_ld, _DT[residual.dtype], gate_ptr, gate_ld,
+                                            0 if post_weight is None else post_weight.data_ptr(), weight.data_ptr(), alpha, eps, residual_out.data_ptr(), ro_ld)
 
 
 def residual_rmsnorm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, post_weight: torch.Tensor | None = None,
@@ -662,7 +668,7 @@ def residual_rmsnorm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
     residual_out may be residual itself.  y, residual, residual_out and gate may be row-strided views."""
     r_out, args = _residual_norm_args(y, residual, weight, post_weight, gate, alpha, eps, residual_out)
     if out is None:
-        out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+        out = y.new_empty(y.shape)
     else:
         _chk(out, y.dtype)
         if out.shape != y.shape or out.device != y.device:
@@ -676,10 +682,10 @@ def residual_rmsnorm_fp8(y: torch.Tensor, residual: torch.Tensor, weight: torch.
                          residual_out: torch.Tensor | None = None):
     """residual_rmsnorm with h as E4M3 of h / scale[0] (the input of gemm_fp8): returns (r, codes uint8 [rows x cols])."""
     r_out, args = _residual_norm_args(y, residual, weight, post_weight, gate, alpha, eps, residual_out)
-    _chk(scale, torch.float32)
-    _same_device(y, scale)
-    q = torch.empty(y.shape, dtype=torch.uint8, device=y.device)
-    handle(y.device.index).call("oxq_residual_rmsnorm_fp8", args, y.shape[0], y.shape[1], scale.data_ptr(), q.data_ptr())
+    if scale.dtype is not torch.float32 or scale.numel() < 1 or scale.get_device() != y.get_device():
+        raise TypeError(f"expected a float32 scale on {y.device}")
+    q = y.new_empty(y.shape, dtype=torch.uint8)
+    handle(y.get_device()).call("oxq_residual_rmsnorm_fp8", args, y.shape[0], y.shape[1], scale.data_ptr(), q.data_ptr())
     return r_out, q
 
 
@@ -687,9 +693,9 @@ def residual_rmsnorm_int8_rows(y: torch.Tensor, residual: torch.Tensor, weight: 
                                gate: torch.Tensor | None = None, alpha: float = 1.0, residual_out: torch.Tensor | None = None):
     """residual_rmsnorm with h through the per-row INT8 quantizer (the input of gemm_w8a8): returns (r, codes int8 [rows x cols], scales f32 [rows])."""
     r_out, args = _residual_norm_args(y, residual, weight, post_weight, gate, alpha, eps, residual_out)
-    q = torch.empty(y.shape, dtype=torch.int8, device=y.device)
-    sc = torch.empty(y.shape[0], dtype=torch.float32, device=y.device)
-    handle(y.device.index).call("oxq_residual_rmsnorm_int8_rows", args, y.shape[0], y.shape[1], q.data_ptr(), sc.data_ptr())
+    q = y.new_empty(y.shape, dtype=torch.int8)
+    sc = y.new_empty(y.shape[0], dtype=torch.float32)
+    handle(y.get_device()).call("oxq_residual_rmsnorm_int8_rows", args, y.shape[0], y.shape[1], q.data_ptr(), sc.data_ptr())
     return r_out, q, sc
 
 
@@ -704,24 +710,27 @@ class Kv4Cache:
     (crates/oxicuda-quant/src/scheme/minmax.rs:146-167, :226-232) with a float offset.  dim is 64 or 128, group 64 or 128, page_size a power of two
     from 16 to 4096."""
 
-    __slots__ = ("k_codes", "k_params", "v_codes", "v_params", "pages", "heads", "page_size", "dim", "group", "device", "_desc", "_shape")
+    __slots__ = ("k_codes", "k_params", "v_codes", "v_params", "pages", "heads", "page_size", "dim", "group", "device", "_index", "_desc", "_shape")
 
     def __init__(self, k_codes: torch.Tensor, k_params: torch.Tensor, v_codes: torch.Tensor, v_params: torch.Tensor):
         cs, ps = k_codes.shape, k_params.shape
         if len(cs) != 4 or len(ps) != 5 or ps[4] != 2 or cs[:3] != ps[:3] or v_codes.shape != cs or v_params.shape != ps:
             from .errors import QuantError
             raise QuantError("DimensionMismatch", f"codes {tuple(cs)}, {tuple(v_codes.shape)} with params {tuple(ps)}, {tuple(v_params.shape)}", 4)
-        device = k_codes.device
-        for t, dt in ((k_codes, torch.uint8), (v_codes, torch.uint8), (k_params, torch.float16), (v_params, torch.float16)):
-            if t.dtype != dt or not t.is_contiguous() or t.device != device:
-                raise TypeError(f"expected contiguous {dt} tensors on one device")
-        if device.type != "cuda":
+        index = k_codes.get_device()
+        if index < 0:
             raise TypeError("expected CUDA tensors")
+        if not (k_codes.dtype is v_codes.dtype is torch.uint8 and k_params.dtype is v_params.dtype is torch.float16):
+            raise TypeError("expected uint8 codes and float16 params")
+        if not (k_codes.is_contiguous() and v_codes.is_contiguous() and k_params.is_contiguous() and v_params.is_contiguous()):
+            raise TypeError("expected contiguous tensors")
+        if not (k_params.get_device() == v_codes.get_device() == v_params.get_device() == index):
+            raise TypeError("expected tensors on one device")
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
         self.pages, self.heads, self.page_size, half = cs
         self.dim = 2 * half
         self.group = self.dim // ps[3] if ps[3] and self.dim % ps[3] == 0 else 0
-        self.device = device
+        self.device, self._index = k_codes.device, index
         self._shape = (self.page_size, self.heads, self.dim, self.group)
         self._desc = _ffi.kv4_cache(k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(), self.pages, self.page_size, self.heads,
                                     self.dim, self.group)
@@ -736,15 +745,14 @@ class Kv4Cache:
 
 
 def _kv4_batch(cache: Kv4Cache, block_table, seq_lens, cu_tokens, tokens: int) -> bytes:
-    if not (block_table.dtype == seq_lens.dtype == cu_tokens.dtype == torch.int32):
+    if not (block_table.dtype is seq_lens.dtype is cu_tokens.dtype is torch.int32):
         raise TypeError("block_table, seq_lens and cu_tokens are int32")
     shape, seqs = block_table.shape, seq_lens.numel()
     if len(shape) != 2 or shape[0] != seqs or cu_tokens.numel() != seqs + 1:
         from .errors import QuantError
         raise QuantError("DimensionMismatch", f"block_table {tuple(shape)}, seq_lens {tuple(seq_lens.shape)}, cu_tokens {tuple(cu_tokens.shape)}", 4)
-    dev = cache.device
-    if block_table.device != dev or seq_lens.device != dev or cu_tokens.device != dev:
-        raise TypeError(f"expected block_table, seq_lens and cu_tokens on {dev}")
+    if not (block_table.get_device() == seq_lens.get_device() == cu_tokens.get_device() == cache._index):
+        raise TypeError(f"expected block_table, seq_lens and cu_tokens on {cache.device}")
     if not (block_table.is_contiguous() and seq_lens.is_contiguous() and cu_tokens.is_contiguous()):
         raise TypeError("expected contiguous block_table, seq_lens and cu_tokens")
     return _ffi.kv4_batch(block_table.data_ptr(), shape[1], seq_lens.data_ptr(), cu_tokens.data_ptr(), seqs, tokens)
@@ -758,7 +766,7 @@ def _kv4_rows(t: torch.Tensor, heads: int, cache: Kv4Cache, what: str, dtypes):
         raise QuantError("DimensionMismatch", f"{what} {tuple(shape)}, expected [tokens, {heads}, {cache.dim}]", 4)
     if t.dtype not in dtypes:
         raise TypeError(f"{what}: expected dtype in {tuple(dtypes)}, got {t.dtype}")
-    if t.device != cache.device:
+    if t.get_device() != cache._index:
         raise TypeError(f"{what}: expected a tensor on {cache.device}")
     stride = t.stride()
     if stride[2] != 1:
@@ -786,7 +794,7 @@ def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
         from .errors import QuantError
         raise QuantError("DimensionMismatch", f"k {tuple(k.shape)} vs v {tuple(v.shape)}", 4)
     batch = _kv4_batch(cache, block_table, seq_lens, cu_tokens, k.shape[0])
-    handle(cache.device.index).call("oxq_kv4_append", cache._desc, batch, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DT[k.dtype])
+    handle(cache._index).call("oxq_kv4_append", cache._desc, batch, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DT[k.dtype])
     return cache
 
 
@@ -798,14 +806,14 @@ def kv4_read(cache: Kv4Cache, block_table: torch.Tensor, seq_lens: torch.Tensor,
     outs = []
     for t, what in ((k_out, "k_out"), (v_out, "v_out")):
         if t is None:
-            t = torch.empty(shape, dtype=dtype, device=cache.device)
+            t = cache.k_codes.new_empty(shape, dtype=dtype)
         else:
             _kv4_rows(t, cache.heads, cache, what, (dtype,))
             if t.shape[0] != shape[0] or not t.is_contiguous():
                 raise TypeError(f"{what}: expected a contiguous tensor of {shape}")
         outs.append(t)
     batch = _kv4_batch(cache, block_table, seq_lens, cu_tokens, shape[0])
-    handle(cache.device.index).call("oxq_kv4_read", cache._desc, batch, outs[0].data_ptr(), outs[1].data_ptr(), _DT[dtype])
+    handle(cache._index).call("oxq_kv4_read", cache._desc, batch, outs[0].data_ptr(), outs[1].data_ptr(), _DT[dtype])
     return outs[0], outs[1]
 
 
@@ -813,7 +821,7 @@ def kv4_attention_workspace_bytes(cache: Kv4Cache, block_table: torch.Tensor, se
                                   max_tokens: int = 0) -> int:
     """Bytes of workspace that kv4_attention needs for `tokens` rows of q_heads heads; depends on the arguments' shapes only, not on their contents."""
     _kv4_batch(cache, block_table, seq_lens, cu_tokens, tokens)
-    return _kv4_workspace(cache.device.index, cache._shape, block_table.shape[1], seq_lens.numel(), tokens, q_heads, max_tokens)
+    return _kv4_workspace(cache._index, cache._shape, block_table.shape[1], seq_lens.numel(), tokens, q_heads, max_tokens)
 
 
 def kv4_attention(q: torch.Tensor, cache: Kv4Cache, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_tokens: torch.Tensor, max_tokens: int = 0,
@@ -830,9 +838,8 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, block_table: torch.Tensor, s
         raise QuantError("DimensionMismatch", f"q {tuple(shape)} over {cache.heads} kv heads", 4)
     tokens, heads = shape[0], shape[1]
     qt, qh = _kv4_rows(q, heads, cache, "q", _HALVES)
-    dev = cache.device
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=dev)
+        out = q.new_empty(shape)
         ot, oh = heads * cache.dim, cache.dim
     else:
         ot, oh = _kv4_rows(out, heads, cache, "out", (q.dtype,))
@@ -840,22 +847,22 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, block_table: torch.Tensor, s
             raise TypeError(f"out: expected {tokens} tokens, got {out.shape[0]}")
     if lse is not None:
         _chk(lse, torch.float32)
-        if tuple(lse.shape) != (tokens, heads) or lse.device != dev:
-            raise TypeError(f"lse: expected {(tokens, heads)} on {dev}")
+        if tuple(lse.shape) != (tokens, heads) or lse.get_device() != cache._index:
+            raise TypeError(f"lse: expected {(tokens, heads)} on {cache.device}")
     elif want_lse:
-        lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev)
+        lse = q.new_empty((tokens, heads), dtype=torch.float32)
     batch = _kv4_batch(cache, block_table, seq_lens, cu_tokens, tokens)
     if workspace is None:
-        n = _kv4_workspace(dev.index, cache._shape, block_table.shape[1], seq_lens.numel(), tokens, heads, max_tokens)
-        workspace = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+        n = _kv4_workspace(cache._index, cache._shape, block_table.shape[1], seq_lens.numel(), tokens, heads, max_tokens)
+        workspace = cache.k_codes.new_empty(max(n, 16))
     else:
         _chk(workspace, torch.uint8)
-        if workspace.device != dev:
-            raise TypeError(f"workspace: expected a tensor on {dev}")
+        if workspace.get_device() != cache._index:
+            raise TypeError(f"workspace: expected a tensor on {cache.device}")
         n = workspace.numel()
     args = _ffi.kv4_attention_args(q.data_ptr(), qt, qh, out.data_ptr(), ot, oh, 0 if lse is None else lse.data_ptr(), heads, max_tokens, window,
                                    cache.dim ** -0.5 if scale is None else scale, 1 if causal else 0, _DT[q.dtype])
-    handle(dev.index).call("oxq_kv4_attention", cache._desc, batch, args, workspace.data_ptr(), n)
+    handle(cache._index).call("oxq_kv4_attention", cache._desc, batch, args, workspace.data_ptr(), n)
     return out if lse is None else (out, lse)
 
 
