@@ -10,6 +10,10 @@
 namespace oxq {
 namespace kv4 {
 
+template <typename T> struct Packed;
+template <> struct Packed<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <> struct Packed<__half> { using type = __half2; };
+
 template <typename T>
 struct Rows {
     const T* p[2];                      // keys, values
@@ -17,131 +21,202 @@ struct Rows {
     int vec;                            // 16-byte loads are aligned
 };
 
-// Eight elements as f32, NaN as 0, held to the range of f16 (s and m are f16).
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int vec, float (&f)[8]) {
-    if (vec) {
-        constexpr int N = Vec16<T>::N;
-#pragma unroll
-        for (int i = 0; i < 8 / N; i++) {
-            const Vec16<T> v = ld16_stream(p + i * N);
-#pragma unroll
-            for (int e = 0; e < N; e++) f[i * N + e] = Elem<T>::to_f32(v.v[e]);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) f[e] = Elem<T>::to_f32(p[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; e++) f[e] = f[e] != f[e] ? 0.0f : fminf(fmaxf(f[e], -65504.0f), 65504.0f);
+// A warp takes `each` (at most 32) tokens.  Lane j finds the place of token first + j; the tokens' words are then one run of
+// each * heads * D / 8 words that the lanes walk side by side, each asking the token's lane for its place.
+constexpr int64_t NO_PLACE = -1, NO_SEQUENCE = -2;
+__device__ __forceinline__ int64_t place_of(const Pool& c, const Batch& s, int64_t first, int each, int32_t* status) {
+    int b = sequence_of(s.cu, s.seqs, first);
+    const int64_t t = first + (threadIdx.x & 31);
+    if ((int)(threadIdx.x & 31) >= each || t >= s.tokens) return NO_SEQUENCE;
+    while (b < s.seqs && __ldg(s.cu + b + 1) <= t) b++;
+    if (b >= s.seqs || t < __ldg(s.cu + b)) return NO_SEQUENCE;
+    return pool_row(c, s, b, (int64_t)__ldg(s.lens + b) - __ldg(s.cu + b + 1) + t, 0, status);
 }
 
-// A thread takes one word (eight elements) of U rows; D / 8 neighbouring lanes make a row.
-template <typename T, int D, int G, int U>
-__global__ void __launch_bounds__(256) kv4_append_kernel(Pool c, Batch s, Rows<T> in, int32_t* status) {
-    pdl_trigger();
-    pdl_wait();
-    constexpr int LANES = D / 8, PER_WARP = 32 / LANES;
-    const int lane = threadIdx.x & 31, word = lane % LANES;
-    const int which = blockIdx.y;
-    const int64_t rows = s.tokens * c.heads;
-    const int64_t first = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (PER_WARP * U);
-    if (first >= rows) return;                                      // whole warps
-    int b = sequence_of(s.cu, s.seqs, first / c.heads);
-    float f[U][8];
-    int64_t at[U];                                                  // row in the pool, -1: none
+// Eight elements as they lie.
+template <typename T> struct Eight { uint32_t w[sizeof(T) * 2]; };
+template <typename T> __device__ __forceinline__ void load8(const T* p, int vec, Eight<T>& r) {
+    if (vec) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int64_t row = first + u * PER_WARP + lane / LANES;
-        const int64_t t = row / c.heads;
-        const int head = (int)(row - t * c.heads);
-        at[u] = -1;
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+            const Vec16<uint32_t> v = ld16_stream(reinterpret_cast<const uint32_t*>(p) + 4 * i);
 #pragma unroll
-        for (int e = 0; e < 8; e++) f[u][e] = 0.0f;
-        if (row < rows) {
-            while (b < s.seqs && __ldg(s.cu + b + 1) <= t) b++;
-            if (b < s.seqs && t >= __ldg(s.cu + b)) {
-                at[u] = pool_row(c, s, b, (int64_t)__ldg(s.lens + b) - __ldg(s.cu + b + 1) + t, head, status);
-                if (at[u] >= 0) load8(in.p[which] + t * in.token_stride[which] + head * in.head_stride[which] + word * 8, in.vec, f[u]);
-            }
+            for (int e = 0; e < 4; e++) r.w[4 * i + e] = v.v[e];
         }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) r.w[e] = reinterpret_cast<const uint32_t*>(p)[e];
+    } else {
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; e++) r.w[e] = (uint32_t)h[2 * e] | ((uint32_t)h[2 * e + 1] << 16);
     }
+}
+template <typename T> __device__ __forceinline__ float element(const Eight<T>& r, int e) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(r.w[e]);
+    else if constexpr (Elem<T>::kDtype == OXQ_BF16) return __uint_as_float(e & 1 ? r.w[e / 2] & 0xFFFF0000u : r.w[e / 2] << 16);
+    else return __half2float(__ushort_as_half((unsigned short)(r.w[e / 2] >> (16 * (e & 1)))));
+}
+// Whether an element is beyond f16's range (s and m are f16), infinite or NaN.
+template <typename T> __device__ __forceinline__ bool beyond(const Eight<T>& r) {
+    if constexpr (sizeof(T) == 4) {
+        bool any = false;
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        float lo = f[u][0], hi = f[u][0];
+        for (int e = 0; e < 8; e++) any |= !(fabsf(__uint_as_float(r.w[e])) <= 65504.0f);
+        return any;
+    } else {
+        uint32_t m = r.w[0] & 0x7FFF7FFFu;
 #pragma unroll
-        for (int e = 1; e < 8; e++) { lo = fminf(lo, f[u][e]); hi = fmaxf(hi, f[u][e]); }
+        for (int e = 1; e < 4; e++) m = __vmaxu2(m, r.w[e] & 0x7FFF7FFFu);
+        const uint32_t top = max(m & 0xFFFFu, m >> 16);
+        return top > (Elem<T>::kDtype == OXQ_BF16 ? 0x477Fu : 0x7BFFu);              // the largest bf16 below 65504, the largest f16
+    }
+}
+// Smallest and largest of the group that W neighbouring lanes hold eight elements of each.  16-bit types stay packed: the pair
+// (smallest, -largest) takes one shuffle and one packed minimum a step.
+template <typename T, int W> __device__ __forceinline__ void group_range(const Eight<T>& r, float& lo, float& hi) {
+    if constexpr (sizeof(T) == 4) {
+        lo = hi = __uint_as_float(r.w[0]);
 #pragma unroll
-        for (int o = 1; o < G / 8; o <<= 1) {
+        for (int e = 1; e < 8; e++) { lo = fminf(lo, __uint_as_float(r.w[e])); hi = fmaxf(hi, __uint_as_float(r.w[e])); }
+#pragma unroll
+        for (int o = 1; o < W; o <<= 1) {
             lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
             hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
-        const __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.0f)), mh = __float2half_rn(lo);
-        const float sc = __half2float(sh), m = __half2float(mh);
-        uint32_t codes = 0;
-        if (sc > 0.0f) {
-            const InvDiv d = make_invdiv(sc);
+    } else {
+        using T2 = typename Packed<T>::type;
+        const auto pack = [](uint32_t v) { return *reinterpret_cast<T2*>(&v); };
+        const auto bits = [](T2 v) { return *reinterpret_cast<uint32_t*>(&v); };
+        T2 l = __hmin2(__hmin2(pack(r.w[0]), pack(r.w[1])), __hmin2(pack(r.w[2]), pack(r.w[3])));
+        T2 h = __hmax2(__hmax2(pack(r.w[0]), pack(r.w[1])), __hmax2(pack(r.w[2]), pack(r.w[3])));
+        const uint32_t lb = bits(l), hb = bits(h) ^ 0x80008000u;
+        uint32_t v = bits(__hmin2(pack(__byte_perm(lb, hb, 0x5410)), pack(__byte_perm(lb, hb, 0x7632))));
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float q = fminf(fmaxf(rintf(div_exact_bounded(f[u][e] - m, d)), 0.0f), 15.0f);
-                codes |= (uint32_t)(int)q << (4 * e);
+        for (int o = 1; o < W; o <<= 1) v = bits(__hmin2(pack(v), pack(__shfl_xor_sync(0xffffffffu, v, o))));
+        Eight<T> e; e.w[0] = v;
+        lo = element(e, 0);
+        hi = -element(e, 1);
+    }
+}
+
+// D / 8 neighbouring lanes make a row, G / 8 of them a group; U words of a lane are in flight at once, `share` warps take turns
+// at the words of the same tokens.
+template <typename T, int D, int G, int U>
+__global__ void __launch_bounds__(256) kv4_append_kernel(Pool c, Batch s, Rows<T> in, int each, int share, FastDiv by_words, int32_t* status) {
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, which = blockIdx.y, words = by_words.d, warp = blockIdx.x * 8 + (threadIdx.x >> 5);          // words of a token
+    const int64_t first = (int64_t)(warp / share) * each;
+    if (first >= s.tokens) return;                                  // whole warps
+    const int64_t mine = place_of(c, s, first, each, status);
+    const int all = each * words;
+    const T* base = in.p[which] + first * in.token_stride[which];
+    for (int i0 = warp % share * 32 * U; i0 < all; i0 += 32 * U * share) {
+        Eight<T> x[U];
+        int64_t at[U];                                              // row in the pool, below 0: none
+        int word[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = i0 + 32 * u + lane, tok = by_words.div(i), rest = i - tok * words, head = rest / (D / 8);
+            word[u] = rest % (D / 8);
+            at[u] = __shfl_sync(0xffffffffu, mine, tok & 31);
+            if (i >= all) at[u] = NO_PLACE;
+#pragma unroll
+            for (int e = 0; e < (int)sizeof(T) * 2; e++) x[u].w[e] = 0;
+            if (at[u] >= 0) {
+                at[u] += (int64_t)head << c.page_shift;
+                load8(base + tok * in.token_stride[which] + head * in.head_stride[which] + word[u] * 8, in.vec, x[u]);
             }
         }
-        if (at[u] >= 0) {
-            uint8_t* row = (which ? c.vc : c.kc) + at[u] * (D / 2);
-            reinterpret_cast<uint32_t*>(row)[which ? value_place(word, D) : key_place(word, D)] = codes;
-            if (word % (G / 8) == 0)
-                (which ? c.vp : c.kp)[at[u] * (D / G) + word / (G / 8)] = (uint32_t)__half_as_ushort(sh) | ((uint32_t)__half_as_ushort(mh) << 16);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float lo, hi, f[8];
+            if (__any_sync(0xffffffffu, beyond(x[u]))) {            // NaN counts as 0, the rest is held to +-65504
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    f[e] = element(x[u], e);
+                    f[e] = f[e] != f[e] ? 0.0f : fminf(fmaxf(f[e], -65504.0f), 65504.0f);
+                    lo = e ? fminf(lo, f[e]) : f[e];
+                    hi = e ? fmaxf(hi, f[e]) : f[e];
+                }
+#pragma unroll
+                for (int o = 1; o < G / 8; o <<= 1) {
+                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[e] = element(x[u], e);
+                group_range<T, G / 8>(x[u], lo, hi);
+            }
+            const __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.0f)), mh = __float2half_rn(lo);
+            const float sc = __half2float(sh), m = __half2float(mh);
+            // (x - m) / s, correctly rounded by a shared reciprocal and one correction (s is 0 or in [2^-24, 8736]); held to
+            // [0, 15]; rounded half to even by adding 1.5 * 2^23; four codes make a number below 2^16, which f32 holds exactly.
+            const float y = __frcp_rn(sc);
+            float half[2] = {0.0f, 0.0f};
+            constexpr float kMagic = 12582912.0f, kPlace[4] = {1.0f, 16.0f, 256.0f, 4096.0f};
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float d = f[e] - m, q0 = d * y, q = fminf(fmaxf(fmaf(fmaf(-sc, q0, d), y, q0), 0.0f), 15.0f);
+                half[e >> 2] = fmaf((q + kMagic) - kMagic, kPlace[e & 3], half[e >> 2]);
+            }
+            uint32_t codes = (__float_as_uint(half[0] + 8388608.0f) & 0xFFFFu) | (__float_as_uint(half[1] + 8388608.0f) << 16);
+            if (!(sc > 0.0f)) codes = 0;
+            if (at[u] >= 0) {
+                uint32_t* row = reinterpret_cast<uint32_t*>((which ? c.vc : c.kc) + at[u] * (D / 2));
+                row[which ? value_place(word[u], D) : key_place(word[u], D)] = codes;
+                if (word[u] % (G / 8) == 0)
+                    (which ? c.vp : c.kp)[at[u] * (D / G) + word[u] / (G / 8)] = (uint32_t)__half_as_ushort(sh) | ((uint32_t)__half_as_ushort(mh) << 16);
+            }
         }
     }
 }
 
-// c * s + m in f32: c * s is exact (4 + 11 bits), so there is one rounding, and one more to T.
+// c * s + m in f32: c * s is exact (4 + 11 bits), so there is one rounding, and one more to T.  The words come out in the
+// order of the output's elements.
 template <typename T, int D, int G, int U>
-__global__ void __launch_bounds__(256) kv4_read_kernel(Pool c, Batch s, T* k_out, T* v_out, int32_t* status) {
+__global__ void __launch_bounds__(256) kv4_read_kernel(Pool c, Batch s, T* k_out, T* v_out, int each, int share, FastDiv by_words, int32_t* status) {
     pdl_trigger();
     pdl_wait();
-    constexpr int LANES = D / 8, PER_WARP = 32 / LANES;
-    const int lane = threadIdx.x & 31, word = lane % LANES;
-    const int which = blockIdx.y;
-    const int64_t rows = s.tokens * c.heads;
-    const int64_t first = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (PER_WARP * U);
-    if (first >= rows) return;
-    int b = sequence_of(s.cu, s.seqs, first / c.heads);
-    const int place = which ? value_place(word, D) : key_place(word, D);
-    uint32_t codes[U], sm[U];
-    bool have[U];
+    const int lane = threadIdx.x & 31, which = blockIdx.y, words = by_words.d, warp = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t first = (int64_t)(warp / share) * each;
+    if (first >= s.tokens) return;
+    const int64_t mine = place_of(c, s, first, each, status);
+    const int all = each * words;
+    const uint32_t* codes_at = reinterpret_cast<const uint32_t*>(which ? c.vc : c.kc);
+    const uint32_t* params_at = which ? c.vp : c.kp;
+    T* out = (which ? v_out : k_out) + first * words * 8;
+    for (int i0 = warp % share * 32 * U; i0 < all; i0 += 32 * U * share) {
+        uint32_t codes[U], sm[U];
+        bool write[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int64_t row = first + u * PER_WARP + lane / LANES;
-        const int64_t t = row / c.heads;
-        const int head = (int)(row - t * c.heads);
-        have[u] = false;
-        codes[u] = 0; sm[u] = 0;
-        if (row < rows) {
-            while (b < s.seqs && __ldg(s.cu + b + 1) <= t) b++;
-            if (b < s.seqs && t >= __ldg(s.cu + b)) {
-                have[u] = true;                                     // a token without a page of the pool reads as zeros
-                const int64_t at = pool_row(c, s, b, (int64_t)__ldg(s.lens + b) - __ldg(s.cu + b + 1) + t, head, status);
-                if (at >= 0) {
-                    codes[u] = __ldg(reinterpret_cast<const uint32_t*>((which ? c.vc : c.kc) + at * (D / 2)) + place);
-                    sm[u] = __ldg((which ? c.vp : c.kp) + at * (D / G) + word / (G / 8));
-                }
+        for (int u = 0; u < U; u++) {
+            const int i = i0 + 32 * u + lane, tok = by_words.div(i), rest = i - tok * words, head = rest / (D / 8), word = rest % (D / 8);
+            int64_t at = __shfl_sync(0xffffffffu, mine, tok & 31);
+            write[u] = i < all && at != NO_SEQUENCE;
+            codes[u] = 0; sm[u] = 0;                                // a token without a page of the pool reads as zeros
+            if (write[u] && at >= 0) {
+                at += (int64_t)head << c.page_shift;
+                codes[u] = __ldg(codes_at + at * (D / 8) + (which ? value_place(word, D) : key_place(word, D)));
+                sm[u] = __ldg(params_at + at * (D / G) + word / (G / 8));
             }
         }
-    }
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        if (!have[u]) continue;
-        const float sc = __half2float(__ushort_as_half((unsigned short)(sm[u] & 0xFFFFu))), m = __half2float(__ushort_as_half((unsigned short)(sm[u] >> 16)));
-        T* out = (which ? v_out : k_out) + (first + u * PER_WARP + lane / LANES) * D + word * 8;
-        constexpr int N = Vec16<T>::N;
+        for (int u = 0; u < U; u++) {
+            if (!write[u]) continue;
+            const __half2 h = *reinterpret_cast<const __half2*>(&sm[u]);
+            const float sc = __low2float(h), m = __high2float(h);
+            T* to = out + (int64_t)(i0 + 32 * u + lane) * 8;
+            constexpr int N = Vec16<T>::N;
 #pragma unroll
-        for (int i = 0; i < 8 / N; i++) {
-            Vec16<T> v;
+            for (int i = 0; i < 8 / N; i++) {
+                Vec16<T> v;
 #pragma unroll
-            for (int e = 0; e < N; e++) v.v[e] = Elem<T>::from_f32(fmaf((float)((codes[u] >> (4 * (i * N + e))) & 15u), sc, m));
-            *reinterpret_cast<uint4*>(out + i * N) = *reinterpret_cast<const uint4*>(&v);
+                for (int e = 0; e < N; e++) v.v[e] = Elem<T>::from_f32(fmaf((float)((codes[u] >> (4 * (i * N + e))) & 15u), sc, m));
+                *reinterpret_cast<uint4*>(to + i * N) = *reinterpret_cast<const uint4*>(&v);
+            }
         }
     }
 }
@@ -180,17 +255,34 @@ int32_t oxq_kv4_check(oxq_handle* h, const oxq_kv4_cache* c, const oxq_kv4_batch
     return OXQ_OK;
 }
 
-// Rows per thread: four keep enough loads in flight to stream; one where there are too few rows to fill the machine with
-// four (a decode step), so that more SMs take part.
-static int rows_per_thread(const oxq_handle* h, int64_t rows, int per_cta) { return rows >= (int64_t)h->sm_count * per_cta * 4 ? 4 : 1; }
+// Tokens per warp: what leaves about 32 warps on every SM for keys and for values, at least a word for every lane, at most 32
+// (a long copy pays for finding 32 places once).  Where even a token a warp leaves SMs without work -- a decode step -- up to
+// eight warps share the token's words, a word a lane at a time.
+struct Shape { int each, share; FastDiv by_words; dim3 grid; };
+static Shape shape_of(const oxq_handle* h, const Pool& c, const Batch& s, int dim) {
+    Shape f;
+    const int words = c.heads * (dim / 8), least = (32 + words - 1) / words;
+    const int64_t each = s.tokens / ((int64_t)h->sm_count * 32);
+    f.each = (int)(each < least ? least : each > 32 ? 32 : each);
+    int share = s.tokens < 8ll * h->sm_count ? f.each * words / 32 : 1;
+    f.share = share < 1 ? 1 : share > 8 ? 8 : share;
+    f.by_words.set(words);
+    f.grid = dim3((unsigned)(((s.tokens + f.each - 1) / f.each * f.share + 7) / 8), 2);
+    return f;
+}
 
 template <typename T, int D, int G>
 static cudaError_t launch_append(oxq_handle* h, const Pool& c, const Batch& s, const Rows<T>& in) {
-    const int64_t rows = s.tokens * c.heads;
-    constexpr int CTA = 8 * (32 / (D / 8));
-    if (rows_per_thread(h, rows, CTA) == 4)
-        return oxq_launch(kv4_append_kernel<T, D, G, 4>, dim3((unsigned)((rows + CTA * 4 - 1) / (CTA * 4)), 2), 256, 0, h->stream, c, s, in, h->dev_status);
-    return oxq_launch(kv4_append_kernel<T, D, G, 1>, dim3((unsigned)((rows + CTA - 1) / CTA), 2), 256, 0, h->stream, c, s, in, h->dev_status);
+    const Shape f = shape_of(h, c, s, D);
+    if (f.share > 1) return oxq_launch(kv4_append_kernel<T, D, G, 1>, f.grid, 256, 0, h->stream, c, s, in, f.each, f.share, f.by_words, h->dev_status);
+    return oxq_launch(kv4_append_kernel<T, D, G, 2>, f.grid, 256, 0, h->stream, c, s, in, f.each, 1, f.by_words, h->dev_status);
+}
+
+template <typename T, int D, int G>
+static cudaError_t launch_read(oxq_handle* h, const Pool& c, const Batch& s, void* k, void* v) {
+    const Shape f = shape_of(h, c, s, D);
+    if (f.share > 1) return oxq_launch(kv4_read_kernel<T, D, G, 1>, f.grid, 256, 0, h->stream, c, s, (T*)k, (T*)v, f.each, f.share, f.by_words, h->dev_status);
+    return oxq_launch(kv4_read_kernel<T, D, G, 4>, f.grid, 256, 0, h->stream, c, s, (T*)k, (T*)v, f.each, 1, f.by_words, h->dev_status);
 }
 
 template <typename T>
@@ -204,15 +296,6 @@ static int32_t append_t(oxq_handle* h, const oxq_kv4_cache* cc, const Pool& c, c
     else if (cc->group == 64) OXQ_CUDA(h, (launch_append<T, 128, 64>(h, c, s, in)));
     else OXQ_CUDA(h, (launch_append<T, 128, 128>(h, c, s, in)));
     return OXQ_OK;
-}
-
-template <typename T, int D, int G>
-static cudaError_t launch_read(oxq_handle* h, const Pool& c, const Batch& s, void* k, void* v) {
-    const int64_t rows = s.tokens * c.heads;
-    constexpr int CTA = 8 * (32 / (D / 8));
-    if (rows_per_thread(h, rows, CTA) == 4)
-        return oxq_launch(kv4_read_kernel<T, D, G, 4>, dim3((unsigned)((rows + CTA * 4 - 1) / (CTA * 4)), 2), 256, 0, h->stream, c, s, (T*)k, (T*)v, h->dev_status);
-    return oxq_launch(kv4_read_kernel<T, D, G, 1>, dim3((unsigned)((rows + CTA - 1) / CTA), 2), 256, 0, h->stream, c, s, (T*)k, (T*)v, h->dev_status);
 }
 
 template <typename T>

@@ -5,19 +5,6 @@
 namespace oxq {
 namespace kv4 {
 
-// n / d for 0 <= n < 2^31 by a product: mul = ceil(2^(32 + shift) / d) with 2^(shift + 1) >= d is exact in that range; d = 1 apart.
-struct FastDiv {
-    uint32_t mul; int shift, d;
-    void set(int div) {
-        d = div;
-        shift = 0;
-        while ((2ll << shift) < div) shift++;
-        mul = div == 1 ? 0u : (uint32_t)((((unsigned long long)1 << (32 + shift)) + (unsigned)div - 1) / (unsigned)div);
-    }
-    __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift); }
-    __device__ __forceinline__ int mod(int n) const { return n - div(n) * d; }
-};
-
 struct AttnParams {
     Pool c;
     Batch s;
