@@ -21,8 +21,25 @@ struct Rows {
     int vec;                            // 16-byte loads are aligned
 };
 
-// A warp takes `each` (at most 32) tokens.  Lane j finds the place of token first + j; the tokens' words are then one run of
-// each * heads * D / 8 words that the lanes walk side by side, each asking the token's lane for its place.
+// How the warps walk the call.  A warp takes `each` (at most 32) tokens; lane j finds the place of token first + j, and the lanes
+// ask it for that place.  A step is 32 words of one token, or the words of `beside` whole tokens where a token has fewer; a
+// token has `rounds` of them.  `share` warps take turns at the steps of the same tokens.
+struct Walk { int each, share, beside, rounds; };
+// A lane's part of every step: which of the tokens beside each other, its word of the row (the same in every round, 32 being a
+// multiple of a row's words) and the word's head and place in the token.
+template <int D> struct Lane {
+    int next_to, word, head, at;
+    bool real;
+    __device__ __forceinline__ Lane(const Walk& w, int words) {
+        const int lane = threadIdx.x & 31;
+        next_to = w.beside > 1 ? lane / words : 0;
+        at = lane - next_to * words;
+        word = at % (D / 8);
+        head = at / (D / 8);
+        real = next_to < w.beside;
+    }
+};
+
 constexpr int64_t NO_PLACE = -1, NO_SEQUENCE = -2;
 __device__ __forceinline__ int64_t place_of(const Pool& c, const Batch& s, int64_t first, int each, int32_t* status) {
     int b = sequence_of(s.cu, s.seqs, first);
@@ -100,125 +117,173 @@ template <typename T, int W> __device__ __forceinline__ void group_range(const E
     }
 }
 
-// D / 8 neighbouring lanes make a row, G / 8 of them a group; U words of a lane are in flight at once, `share` warps take turns
-// at the words of the same tokens.
-template <typename T, int D, int G, int U>
-__global__ void __launch_bounds__(256) kv4_append_kernel(Pool c, Batch s, Rows<T> in, int each, int share, FastDiv by_words, int32_t* status) {
-    pdl_trigger();
-    pdl_wait();
-    const int lane = threadIdx.x & 31, which = blockIdx.y, words = by_words.d, warp = blockIdx.x * 8 + (threadIdx.x >> 5);          // words of a token
-    const int64_t first = (int64_t)(warp / share) * each;
-    if (first >= s.tokens) return;                                  // whole warps
-    const int64_t mine = place_of(c, s, first, each, status);
-    const int all = each * words;
-    const T* base = in.p[which] + first * in.token_stride[which];
-    for (int i0 = warp % share * 32 * U; i0 < all; i0 += 32 * U * share) {
-        Eight<T> x[U];
-        int64_t at[U];                                              // row in the pool, below 0: none
-        int word[U];
+// Eight elements of a lane to a word of codes and, the same in all lanes of the group, its (s, m).
+template <typename T, int G> __device__ __forceinline__ void quantize8(const Eight<T>& x, uint32_t& codes, uint32_t& params) {
+    float lo, hi, f[8];
+    if (__any_sync(0xffffffffu, beyond(x))) {            // NaN counts as 0, the rest is held to +-65504
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int i = i0 + 32 * u + lane, tok = by_words.div(i), rest = i - tok * words, head = rest / (D / 8);
-            word[u] = rest % (D / 8);
-            at[u] = __shfl_sync(0xffffffffu, mine, tok & 31);
-            if (i >= all) at[u] = NO_PLACE;
-#pragma unroll
-            for (int e = 0; e < (int)sizeof(T) * 2; e++) x[u].w[e] = 0;
-            if (at[u] >= 0) {
-                at[u] += (int64_t)head << c.page_shift;
-                load8(base + tok * in.token_stride[which] + head * in.head_stride[which] + word[u] * 8, in.vec, x[u]);
-            }
+        for (int e = 0; e < 8; e++) {
+            f[e] = element(x, e);
+            f[e] = f[e] != f[e] ? 0.0f : fminf(fmaxf(f[e], -65504.0f), 65504.0f);
+            lo = e ? fminf(lo, f[e]) : f[e];
+            hi = e ? fmaxf(hi, f[e]) : f[e];
         }
 #pragma unroll
+        for (int o = 1; o < G / 8; o <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = element(x, e);
+        group_range<T, G / 8>(x, lo, hi);
+    }
+    // range / 15 and (x - m) / s, correctly rounded by a reciprocal and one correction (Markstein; see InvDiv; a range too
+    // small for that to hold is one that f16 rounds to 0, and s is 0 or in [2^-24, 8736]); the quotients held to
+    // [0, 15]; rounded half to even by adding 1.5 * 2^23; four codes make a number below 2^16, which f32 holds exactly.
+    const float range = hi - lo, fifteenth = 1.0f / 15.0f, s0 = range * fifteenth;
+    const __half sh = __float2half_rn(fmaf(fmaf(-15.0f, s0, range), fifteenth, s0)), mh = __float2half_rn(lo);
+    const float sc = __half2float(sh), m = __half2float(mh), y = __frcp_rn(sc);
+    float half[2] = {0.0f, 0.0f};
+    constexpr float kMagic = 12582912.0f, kPlace[4] = {1.0f, 16.0f, 256.0f, 4096.0f};
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float d = f[e] - m, q0 = d * y, q = fminf(fmaxf(fmaf(fmaf(-sc, q0, d), y, q0), 0.0f), 15.0f);
+        half[e >> 2] = fmaf((q + kMagic) - kMagic, kPlace[e & 3], half[e >> 2]);
+    }
+    codes = (__float_as_uint(half[0] + 8388608.0f) & 0xFFFFu) | (__float_as_uint(half[1] + 8388608.0f) << 16);
+    if (!(sc > 0.0f)) codes = 0;
+    params = (uint32_t)__half_as_ushort(sh) | ((uint32_t)__half_as_ushort(mh) << 16);
+}
+
+template <typename T, int D, int G, int U, bool KEYS>
+__device__ __forceinline__ void append_rows(const Pool& c, const Batch& s, const Rows<T>& in, const Walk& walk, int32_t* status) {
+    const int words = c.heads * (D / 8), warp = blockIdx.x * 8 + (threadIdx.x >> 5);          // words of a token
+    const int64_t first = (int64_t)(warp / walk.share) * walk.each;
+    if (first >= s.tokens) return;                                  // whole warps
+    const int64_t mine = place_of(c, s, first, walk.each, status);
+    const Lane<D> lane(walk, words);
+    const int64_t token_stride = in.token_stride[KEYS ? 0 : 1], round_stride = 256 / D * in.head_stride[KEYS ? 0 : 1];
+    const int64_t round_rows = (int64_t)(256 / D) << c.page_shift;  // rows of the pool from one round to the next
+    const T* base = in.p[KEYS ? 0 : 1] + (first + lane.next_to) * token_stride + lane.head * in.head_stride[KEYS ? 0 : 1] + lane.word * 8;
+    uint32_t* codes_at = reinterpret_cast<uint32_t*>(KEYS ? c.kc : c.vc) + (KEYS ? key_place(lane.word, D) : value_place(lane.word, D));
+    uint32_t* params_at = (KEYS ? c.kp : c.vp) + lane.word / (G / 8);
+    const bool leads = lane.word % (G / 8) == 0;
+    for (int j0 = 0, t0 = 0; t0 < walk.each; j0 += U, t0 += U * walk.beside) {
+        int64_t at[U];                                              // row in the pool, below 0: none
+        const T* from[U];
+#pragma unroll
         for (int u = 0; u < U; u++) {
-            float lo, hi, f[8];
-            if (__any_sync(0xffffffffu, beyond(x[u]))) {            // NaN counts as 0, the rest is held to +-65504
+            const int tok = t0 + u * walk.beside + lane.next_to;
+            at[u] = __shfl_sync(0xffffffffu, mine, tok & 31);
+            if (!lane.real || tok >= walk.each) at[u] = NO_PLACE;
+            if (at[u] >= 0) at[u] += (int64_t)lane.head << c.page_shift;
+            from[u] = base + (t0 + u * walk.beside) * token_stride;
+        }
+        // the rounds of a token; where several warps share the tokens, every share-th step is this one's
+        for (int k = 0; k < walk.rounds; k++) {
+            if (U == 1 && walk.share > 1 && (j0 * walk.rounds + k) % walk.share != warp % walk.share) continue;
+            const bool inside = lane.at + 32 * k < words;
+            Eight<T> x[U];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    f[e] = element(x[u], e);
-                    f[e] = f[e] != f[e] ? 0.0f : fminf(fmaxf(f[e], -65504.0f), 65504.0f);
-                    lo = e ? fminf(lo, f[e]) : f[e];
-                    hi = e ? fmaxf(hi, f[e]) : f[e];
-                }
+            for (int u = 0; u < U; u++) {
 #pragma unroll
-                for (int o = 1; o < G / 8; o <<= 1) {
-                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) f[e] = element(x[u], e);
-                group_range<T, G / 8>(x[u], lo, hi);
+                for (int e = 0; e < (int)sizeof(T) * 2; e++) x[u].w[e] = 0;
+                if (inside && at[u] >= 0) load8(from[u] + k * round_stride, in.vec, x[u]);
             }
-            const __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.0f)), mh = __float2half_rn(lo);
-            const float sc = __half2float(sh), m = __half2float(mh);
-            // (x - m) / s, correctly rounded by a shared reciprocal and one correction (s is 0 or in [2^-24, 8736]); held to
-            // [0, 15]; rounded half to even by adding 1.5 * 2^23; four codes make a number below 2^16, which f32 holds exactly.
-            const float y = __frcp_rn(sc);
-            float half[2] = {0.0f, 0.0f};
-            constexpr float kMagic = 12582912.0f, kPlace[4] = {1.0f, 16.0f, 256.0f, 4096.0f};
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float d = f[e] - m, q0 = d * y, q = fminf(fmaxf(fmaf(fmaf(-sc, q0, d), y, q0), 0.0f), 15.0f);
-                half[e >> 2] = fmaf((q + kMagic) - kMagic, kPlace[e & 3], half[e >> 2]);
-            }
-            uint32_t codes = (__float_as_uint(half[0] + 8388608.0f) & 0xFFFFu) | (__float_as_uint(half[1] + 8388608.0f) << 16);
-            if (!(sc > 0.0f)) codes = 0;
-            if (at[u] >= 0) {
-                uint32_t* row = reinterpret_cast<uint32_t*>((which ? c.vc : c.kc) + at[u] * (D / 2));
-                row[which ? value_place(word[u], D) : key_place(word[u], D)] = codes;
-                if (word[u] % (G / 8) == 0)
-                    (which ? c.vp : c.kp)[at[u] * (D / G) + word[u] / (G / 8)] = (uint32_t)__half_as_ushort(sh) | ((uint32_t)__half_as_ushort(mh) << 16);
+            for (int u = 0; u < U; u++) {
+                uint32_t codes, params;
+                quantize8<T, G>(x[u], codes, params);
+                if (inside && at[u] >= 0) {
+                    const int64_t row = at[u] + k * round_rows;
+                    codes_at[row * (D / 8)] = codes;
+                    if (leads) params_at[row * (D / G)] = params;
+                }
             }
         }
     }
 }
+template <typename T, int D, int G, int U>
+__global__ void __launch_bounds__(256) kv4_append_kernel(Pool c, Batch s, Rows<T> in, Walk walk, int32_t* status) {
+    pdl_trigger();
+    pdl_wait();
+    if (blockIdx.y == 0) append_rows<T, D, G, U, true>(c, s, in, walk, status);
+    else append_rows<T, D, G, U, false>(c, s, in, walk, status);
+}
 
 // c * s + m in f32: c * s is exact (4 + 11 bits), so there is one rounding, and one more to T.  The words come out in the
 // order of the output's elements.
-template <typename T, int D, int G, int U>
-__global__ void __launch_bounds__(256) kv4_read_kernel(Pool c, Batch s, T* k_out, T* v_out, int each, int share, FastDiv by_words, int32_t* status) {
-    pdl_trigger();
-    pdl_wait();
-    const int lane = threadIdx.x & 31, which = blockIdx.y, words = by_words.d, warp = blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t first = (int64_t)(warp / share) * each;
+template <typename T, int D, int G, int U, bool KEYS>
+__device__ __forceinline__ void read_rows(const Pool& c, const Batch& s, T* rows_out, const Walk& walk, int32_t* status) {
+    const int words = c.heads * (D / 8), warp = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t first = (int64_t)(warp / walk.share) * walk.each;
     if (first >= s.tokens) return;
-    const int64_t mine = place_of(c, s, first, each, status);
-    const int all = each * words;
-    const uint32_t* codes_at = reinterpret_cast<const uint32_t*>(which ? c.vc : c.kc);
-    const uint32_t* params_at = which ? c.vp : c.kp;
-    T* out = (which ? v_out : k_out) + first * words * 8;
-    for (int i0 = warp % share * 32 * U; i0 < all; i0 += 32 * U * share) {
-        uint32_t codes[U], sm[U];
+    const int64_t mine = place_of(c, s, first, walk.each, status);
+    const Lane<D> lane(walk, words);
+    const int64_t round_rows = (int64_t)(256 / D) << c.page_shift;
+    const uint32_t* codes_at = reinterpret_cast<const uint32_t*>(KEYS ? c.kc : c.vc) + (KEYS ? key_place(lane.word, D) : value_place(lane.word, D));
+    const uint32_t* params_at = (KEYS ? c.kp : c.vp) + lane.word / (G / 8);
+    T* out = rows_out + ((first + lane.next_to) * words + lane.at) * 8;
+    for (int j0 = 0, t0 = 0; t0 < walk.each; j0 += U, t0 += U * walk.beside) {
+        int64_t at[U];
         bool write[U];
+        T* to[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int i = i0 + 32 * u + lane, tok = by_words.div(i), rest = i - tok * words, head = rest / (D / 8), word = rest % (D / 8);
-            int64_t at = __shfl_sync(0xffffffffu, mine, tok & 31);
-            write[u] = i < all && at != NO_SEQUENCE;
-            codes[u] = 0; sm[u] = 0;                                // a token without a page of the pool reads as zeros
-            if (write[u] && at >= 0) {
-                at += (int64_t)head << c.page_shift;
-                codes[u] = __ldg(codes_at + at * (D / 8) + (which ? value_place(word, D) : key_place(word, D)));
-                sm[u] = __ldg(params_at + at * (D / G) + word / (G / 8));
-            }
+            const int tok = t0 + u * walk.beside + lane.next_to;
+            at[u] = __shfl_sync(0xffffffffu, mine, tok & 31);
+            write[u] = lane.real && tok < walk.each && at[u] != NO_SEQUENCE;
+            if (at[u] >= 0) at[u] += (int64_t)lane.head << c.page_shift;
+            to[u] = out + (t0 + u * walk.beside) * words * 8;
         }
+        for (int k = 0; k < walk.rounds; k++) {
+            if (U == 1 && walk.share > 1 && (j0 * walk.rounds + k) % walk.share != warp % walk.share) continue;
+            const bool inside = lane.at + 32 * k < words;
+            uint32_t codes[U], sm[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (!write[u]) continue;
-            const __half2 h = *reinterpret_cast<const __half2*>(&sm[u]);
-            const float sc = __low2float(h), m = __high2float(h);
-            T* to = out + (int64_t)(i0 + 32 * u + lane) * 8;
-            constexpr int N = Vec16<T>::N;
+            for (int u = 0; u < U; u++) {
+                codes[u] = 0; sm[u] = 0;                            // a token without a page of the pool reads as zeros
+                if (inside && write[u] && at[u] >= 0) {
+                    const int64_t row = at[u] + k * round_rows;
+                    codes[u] = __ldg(codes_at + row * (D / 8));
+                    sm[u] = __ldg(params_at + row * (D / G));
+                }
+            }
 #pragma unroll
-            for (int i = 0; i < 8 / N; i++) {
-                Vec16<T> v;
+            for (int u = 0; u < U; u++) {
+                if (!inside || !write[u]) continue;
+                const __half2 h = *reinterpret_cast<const __half2*>(&sm[u]);
+                const float sc = __low2float(h), m = __high2float(h);
+                // two codes at a time as f16: under the exponent of 1024 a nibble is 1024 + c, or 1024 + 16 c where it lies four bits up
+                const auto half2_of = [](uint32_t v) { return *reinterpret_cast<const __half2*>(&v); };
+                float f[8];
 #pragma unroll
-                for (int e = 0; e < N; e++) v.v[e] = Elem<T>::from_f32(fmaf((float)((codes[u] >> (4 * (i * N + e))) & 15u), sc, m));
-                *reinterpret_cast<uint4*>(to + i * N) = *reinterpret_cast<const uint4*>(&v);
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t w = e < 2 ? codes[u] : codes[u] >> 8;
+                    const __half2 c2 = e & 1 ? __hfma2(half2_of((w & 0x00F000F0u) | 0x64006400u), half2_of(0x2C002C00u), half2_of(0xD400D400u))
+                                             : __hsub2(half2_of((w & 0x000F000Fu) | 0x64006400u), half2_of(0x64006400u));
+                    f[e] = fmaf(__low2float(c2), sc, m);
+                    f[e + 4] = fmaf(__high2float(c2), sc, m);
+                }
+                constexpr int N = Vec16<T>::N;
+#pragma unroll
+                for (int i = 0; i < 8 / N; i++) {
+                    Vec16<T> v;
+#pragma unroll
+                    for (int e = 0; e < N; e++) v.v[e] = Elem<T>::from_f32(f[i * N + e]);
+                    *reinterpret_cast<uint4*>(to[u] + k * 256 + i * N) = *reinterpret_cast<const uint4*>(&v);
+                }
             }
         }
     }
+}
+template <typename T, int D, int G, int U>
+__global__ void __launch_bounds__(256) kv4_read_kernel(Pool c, Batch s, T* k_out, T* v_out, Walk walk, int32_t* status) {
+    pdl_trigger();
+    pdl_wait();
+    if (blockIdx.y == 0) read_rows<T, D, G, U, true>(c, s, k_out, walk, status);
+    else read_rows<T, D, G, U, false>(c, s, v_out, walk, status);
 }
 
 }  // namespace kv4
@@ -255,34 +320,40 @@ int32_t oxq_kv4_check(oxq_handle* h, const oxq_kv4_cache* c, const oxq_kv4_batch
     return OXQ_OK;
 }
 
-// Tokens per warp: what leaves about 32 warps on every SM for keys and for values, at least a word for every lane, at most 32
-// (a long copy pays for finding 32 places once).  Where even a token a warp leaves SMs without work -- a decode step -- up to
-// eight warps share the token's words, a word a lane at a time.
-struct Shape { int each, share; FastDiv by_words; dim3 grid; };
-static Shape shape_of(const oxq_handle* h, const Pool& c, const Batch& s, int dim) {
-    Shape f;
+// Tokens per warp: what leaves about 16 warps on every SM for keys and for values, at least a word for every lane, at most
+// eight (a read of 131k tokens: 125 us; with 32 a warp 150 us, for the last wave of CTAs is then long); whole fours, as four tokens' loads are in flight at once.  Where even a token
+// a warp leaves SMs without work -- a decode step -- up to eight warps share the token's words.
+static Walk walk_of(const oxq_handle* h, const Pool& c, const Batch& s, int dim, dim3* grid) {
+    Walk w;
     const int words = c.heads * (dim / 8), least = (32 + words - 1) / words;
-    const int64_t each = s.tokens / ((int64_t)h->sm_count * 32);
-    f.each = (int)(each < least ? least : each > 32 ? 32 : each);
-    int share = s.tokens < 8ll * h->sm_count ? f.each * words / 32 : 1;
-    f.share = share < 1 ? 1 : share > 8 ? 8 : share;
-    f.by_words.set(words);
-    f.grid = dim3((unsigned)(((s.tokens + f.each - 1) / f.each * f.share + 7) / 8), 2);
-    return f;
+    const int64_t each = s.tokens / ((int64_t)h->sm_count * 16);
+    w.each = (int)(each < least ? least : each > 8 && least <= 8 ? 8 : each > 32 ? 32 : each);
+    w.beside = words < 32 ? 32 / words : 1;
+    w.rounds = (words + 31) / 32;
+    const int share = s.tokens < 8ll * h->sm_count ? (w.each + w.beside - 1) / w.beside * w.rounds : 1;
+    w.share = share > 8 ? 8 : share;
+    if (w.share == 1) {
+        const int four = 4 * w.beside;
+        w.each = w.each + four - 1 < 32 ? (w.each + four - 1) / four * four : 32;
+    }
+    *grid = dim3((unsigned)(((s.tokens + w.each - 1) / w.each * w.share + 7) / 8), 2);
+    return w;
 }
 
 template <typename T, int D, int G>
 static cudaError_t launch_append(oxq_handle* h, const Pool& c, const Batch& s, const Rows<T>& in) {
-    const Shape f = shape_of(h, c, s, D);
-    if (f.share > 1) return oxq_launch(kv4_append_kernel<T, D, G, 1>, f.grid, 256, 0, h->stream, c, s, in, f.each, f.share, f.by_words, h->dev_status);
-    return oxq_launch(kv4_append_kernel<T, D, G, 2>, f.grid, 256, 0, h->stream, c, s, in, f.each, 1, f.by_words, h->dev_status);
+    dim3 grid;
+    const Walk w = walk_of(h, c, s, D, &grid);
+    if (w.share > 1) return oxq_launch(kv4_append_kernel<T, D, G, 1>, grid, 256, 0, h->stream, c, s, in, w, h->dev_status);
+    return oxq_launch(kv4_append_kernel<T, D, G, 4>, grid, 256, 0, h->stream, c, s, in, w, h->dev_status);
 }
 
 template <typename T, int D, int G>
 static cudaError_t launch_read(oxq_handle* h, const Pool& c, const Batch& s, void* k, void* v) {
-    const Shape f = shape_of(h, c, s, D);
-    if (f.share > 1) return oxq_launch(kv4_read_kernel<T, D, G, 1>, f.grid, 256, 0, h->stream, c, s, (T*)k, (T*)v, f.each, f.share, f.by_words, h->dev_status);
-    return oxq_launch(kv4_read_kernel<T, D, G, 4>, f.grid, 256, 0, h->stream, c, s, (T*)k, (T*)v, f.each, 1, f.by_words, h->dev_status);
+    dim3 grid;
+    const Walk w = walk_of(h, c, s, D, &grid);
+    if (w.share > 1) return oxq_launch(kv4_read_kernel<T, D, G, 1>, grid, 256, 0, h->stream, c, s, (T*)k, (T*)v, w, h->dev_status);
+    return oxq_launch(kv4_read_kernel<T, D, G, 4>, grid, 256, 0, h->stream, c, s, (T*)k, (T*)v, w, h->dev_status);
 }
 
 template <typename T>

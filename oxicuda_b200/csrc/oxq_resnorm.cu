@@ -3,7 +3,7 @@
 //   r' = residual + alpha t
 //   h  = rms(r'; weight), stored as it is, as E4M3 at a calibrated scale, or as INT8 with a scale per row
 // with rms(x; w) = x / sqrt(mean(x^2) + eps) * w.  All of it is f32; r' is normed before it is rounded to its own type.
-// A row is held in registers by TPR threads (NV items of eight elements each), so every input is read once and every
+// A row is held in registers by TPR threads (NV items of eight elements each, in their own type), so every input is read once and every
 // output written once; the sums of squares meet in shared memory, in a fixed order.
 #include "oxq_common.cuh"
 
@@ -26,14 +26,30 @@ struct Params {
     int mode;
 };
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-    constexpr int N = Vec16<T>::N;
+// Eight elements as they lie: a row waits in registers in its own type, not in f32.
+template <typename T> struct Eight { uint4 v[sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ Eight<T> load8(const T* p) {
+    Eight<T> r;
 #pragma unroll
-    for (int i = 0; i < 8 / N; i++) {
-        const Vec16<T> v = ld16_stream(p + i * N);
-#pragma unroll
-        for (int e = 0; e < N; e++) f[i * N + e] = Elem<T>::to_f32(v.v[e]);
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+        const Vec16<uint32_t> v = ld16_stream(reinterpret_cast<const uint32_t*>(p) + 4 * i);
+        r.v[i] = make_uint4(v.v[0], v.v[1], v.v[2], v.v[3]);
     }
+    return r;
+}
+template <typename T> __device__ __forceinline__ Eight<T> zero8() {
+    Eight<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) r.v[i] = make_uint4(0, 0, 0, 0);
+    return r;
+}
+template <typename T> __device__ __forceinline__ float element(const Eight<T>& r, int e) {
+    const uint4 v = r.v[sizeof(T) == 4 ? e >> 2 : 0];
+    const int i = sizeof(T) == 4 ? e & 3 : e >> 1;
+    const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+    else if constexpr (Elem<T>::kDtype == OXQ_BF16) return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
+    else return __half2float(__ushort_as_half((unsigned short)(w >> (16 * (e & 1)))));
 }
 template <typename T> __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
     constexpr int N = Vec16<T>::N;
@@ -81,15 +97,16 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_rmsnorm_kernel
     const int64_t row = live ? row0 : p.rows - 1;                   // idle threads of the last CTA meet the barriers
     const int64_t items = p.cols >> 3;
     const int lane = threadIdx.x % TPR;
-    float t[NV][8], r[NV][8];
+    Eight<T> y[NV], gate[NV];
+    Eight<R> res[NV];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const int64_t it = lane + i * TPR;
-#pragma unroll
-        for (int e = 0; e < 8; e++) { t[i][e] = 0.0f; r[i][e] = 0.0f; }
+        y[i] = zero8<T>(); gate[i] = zero8<T>(); res[i] = zero8<R>();
         if (it < items) {
-            load8((const T*)p.y + row * p.y_ld + it * 8, t[i]);
-            load8((const R*)p.residual + row * p.r_ld + it * 8, r[i]);
+            y[i] = load8((const T*)p.y + row * p.y_ld + it * 8);
+            res[i] = load8((const R*)p.residual + row * p.r_ld + it * 8);
+            if (p.gate) gate[i] = load8((const T*)p.gate + row * p.g_ld + it * 8);
         }
     }
     float k = p.alpha;
@@ -98,29 +115,32 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_rmsnorm_kernel
 #pragma unroll
         for (int i = 0; i < NV; i++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) ss = fmaf(t[i][e], t[i][e], ss);
+            for (int e = 0; e < 8; e++) ss = fmaf(element(y[i], e), element(y[i], e), ss);
         ss = row_reduce<TPR, false>(ss, red);
         k *= __fdiv_rn(1.0f, sqrtf(__fdiv_rn(ss, (float)p.cols) + p.eps));
     }
-    float ss = 0.0f;
+    float ss = 0.0f, r[NV][8];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const int64_t it = lane + i * TPR;
+#pragma unroll
+        for (int e = 0; e < 8; e++) r[i][e] = 0.0f;
         if (it < items) {
-            float w[8];
+            float t[8], w[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) t[e] = element(y[i], e);
             if (p.post) {
                 weight8(p.post + it * 8, w);
 #pragma unroll
-                for (int e = 0; e < 8; e++) t[i][e] *= w[e];
+                for (int e = 0; e < 8; e++) t[e] *= w[e];
             }
             if (p.gate) {
-                load8((const T*)p.gate + row * p.g_ld + it * 8, w);
 #pragma unroll
-                for (int e = 0; e < 8; e++) t[i][e] *= w[e];
+                for (int e = 0; e < 8; e++) t[e] *= element(gate[i], e);
             }
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                r[i][e] = fmaf(k, t[i][e], r[i][e]);
+                r[i][e] = fmaf(k, t[e], element(res[i], e));
                 ss = fmaf(r[i][e], r[i][e], ss);
             }
             if (live) store8((R*)p.residual_out + row * p.ro_ld + it * 8, r[i]);
@@ -177,18 +197,21 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_rmsnorm_kernel
     }
 }
 
-// Threads per row.  With rows enough to fill the machine, as few as hold the row at four items each: their loads are all
-// in flight at once and the meeting points stay cheap.  With fewer rows than that, one item a thread, for the latency.
+// Threads per row.  With rows enough to fill the machine, what holds the row at two items each: y, residual and gate of a row
+// are then all in flight at 64 registers a thread, 32 warps on an SM (8190 x 8192 bf16 with all parts: 173 us with half the
+// threads and four items).  With fewer rows than that, one item a thread, for the latency.
 template <typename T, typename R>
 static cudaError_t launch(oxq_handle* h, const Params& p) {
     const int64_t items = p.cols >> 3;
 #define OXQ_RN(TPR, NV) \
     oxq_launch(residual_rmsnorm_kernel<T, R, TPR, NV>, (unsigned)((p.rows + (TPR < 256 ? 256 / TPR : 1) - 1) / (TPR < 256 ? 256 / TPR : 1)), TPR < 256 ? 256 : TPR, 0, h->stream, p)
     if (p.rows >= 2 * (int64_t)h->sm_count) {
-        if (items <= 128) return OXQ_RN(32, 4);
-        if (items <= 512) return OXQ_RN(128, 4);
-        if (items <= 1024) return OXQ_RN(256, 4);
-        return OXQ_RN(512, 4);
+        if (items <= 64) return OXQ_RN(32, 2);
+        if (items <= 128) return OXQ_RN(64, 2);
+        if (items <= 256) return OXQ_RN(128, 2);
+        if (items <= 512) return OXQ_RN(256, 2);
+        if (items <= 1024) return OXQ_RN(512, 2);
+        return OXQ_RN(1024, 2);
     }
     if (items <= 128) return OXQ_RN(128, 1);
     if (items <= 512) return OXQ_RN(512, 1);
