@@ -9,9 +9,9 @@
 //
 // The shape: a CTA takes two blocks of 128 query rows (tokens and the query heads of one kv head, packed) and walks the keys
 // in tiles of 128.  tcgen05.mma: S from shared memory (Q and the tile's keys), O from P in tensor memory, written over the
-// scores, and the tile's values.  Roles: two warpgroups of softmax (one row a thread), one that turns codes into f16 tiles
-// (two stages each of keys and values), one warp that issues the products.  While one block's scores are in softmax the
-// tensor core works on the other block's.  Inside every eight elements of a head the order is 0 4 1 5 2 6 3 7, which is
+// scores, and the tile's values.  Roles: two warpgroups of softmax (one row a thread), two that turn codes into f16 tiles
+// (two stages each of keys and values), one warp that issues the products; registers go from the others to the softmax.
+// While one block's scores are in softmax the tensor core works on the other block's.  Inside every eight elements of a head the order is 0 4 1 5 2 6 3 7, which is
 // the order in which a word's nibbles come out in pairs; it is undone where O is stored.
 #include "oxq_kv4_attn.cuh"
 #include "oxq_tc.cuh"
@@ -52,6 +52,12 @@ __device__ __forceinline__ uint4 expand(uint32_t w, __half2 s, __half2 m) {
     o.w = as_u32(__hfma2(__hfma2(as_half2((w & 0x00F000F0u) | 0x64006400u), k16, k64), s, m));
     return o;
 }
+
+// Threads: warpgroups 0, 1 softmax, 2, 3 producers, 4 (its first warp) products.  Registers a thread after the split: launched with
+// 96 x 640 = 61440 in all, 2 x 128 x 144 + 2 x 128 x 64 + 128 x 64 = 61440.
+constexpr int THREADS = 640, PRODUCERS = 256, MMA_WARP = 16;
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // The CTA's item: sequence and pair of row blocks.  Items of a sequence come last rows first: they see the most keys.
 struct TileItem { int b, pair; SeqInfo q; };
@@ -98,7 +104,7 @@ __device__ __forceinline__ Walk walk_of(const AttnParams& p, const SeqInfo& q, i
 }
 
 template <typename T, int D, int NG>
-__global__ void __launch_bounds__(416, 1) kv4_attn_tiles_kernel(AttnParams p) {
+__global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p) {
     using L = TileSmem<D>;
     constexpr int NA = D / 64;
     extern __shared__ unsigned char smem_dyn[];
@@ -115,14 +121,14 @@ __global__ void __launch_bounds__(416, 1) kv4_attn_tiles_kernel(AttnParams p) {
     const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     unsigned char* smem = smem_dyn + (base - smem_u32(smem_dyn));
     const auto bar = [&](int i) { return base + L::BARS + 8 * i; };
-    if (warp == 12) {
+    if (warp == MMA_WARP) {
         if (lane == 0) {
             mbar_init(bar(BAR_Q), 256);
             mbar_init(bar(BAR_END), 1);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                mbar_init(bar(BAR_KFULL + i), 128); mbar_init(bar(BAR_KEMPTY + i), 1);
-                mbar_init(bar(BAR_VFULL + i), 128); mbar_init(bar(BAR_VEMPTY + i), 1);
+                mbar_init(bar(BAR_KFULL + i), PRODUCERS); mbar_init(bar(BAR_KEMPTY + i), 1);
+                mbar_init(bar(BAR_VFULL + i), PRODUCERS); mbar_init(bar(BAR_VEMPTY + i), 1);
                 mbar_init(bar(BAR_S + i), 1); mbar_init(bar(BAR_P + i), 128);
             }
             fence_barrier_init();
@@ -140,6 +146,7 @@ __global__ void __launch_bounds__(416, 1) kv4_attn_tiles_kernel(AttnParams p) {
 
     if (warp < 8) {
         // ------------------------------------------------------------------------------------ softmax: one row a thread
+        more_registers<144>();
         const int t = warp >> 2, r = (warp & 3) * 32 + lane;
         const int row = it.pair * 2 * BLOCK + t * BLOCK + r;
         const bool real = row < q.n * p.per;
@@ -308,14 +315,19 @@ __global__ void __launch_bounds__(416, 1) kv4_attn_tiles_kernel(AttnParams p) {
                 __syncwarp();
             }
         }
-    } else if (warp < 12) {
+    } else if (warp < MMA_WARP) {
         // ------------------------------------------------------------------------------------ codes to f16 tiles
+        fewer_registers<64>();
         constexpr int Q16 = D / 32;                                 // 16-byte pieces of a row
-        constexpr int ROUNDS = BLOCK * Q16 / 128, PER_ROUND = 128 / Q16;
+        constexpr int ROUNDS = BLOCK * Q16 / PRODUCERS, PER_ROUND = PRODUCERS / Q16;
         const int pt = tid - 256, piece = pt % Q16, tok0 = pt / Q16;
         const int32_t* table = p.s.table + (int64_t)it.b * p.s.width;
-        struct Raw { uint4 k[ROUNDS], v[ROUNDS]; uint32_t kp[ROUNDS][NG], vp[ROUNDS][NG]; } raw;
+        // One tile's codes wait in registers, keys and values apart: the next tile's keys are requested when this one's have
+        // been turned into f16, and are there when its values have; the table's entries are fetched a tile before that.
+        uint4 kraw[ROUNDS], vraw[ROUNDS];
+        uint32_t kpar[ROUNDS][NG], vpar[ROUNDS][NG];
         int page[ROUNDS];
+        bool gone[ROUNDS];                                          // a key without a page of the pool; one behind the end is masked by its position
         const auto get_pages = [&](int i) {
 #pragma unroll
             for (int u = 0; u < ROUNDS; u++) {
@@ -323,36 +335,37 @@ __global__ void __launch_bounds__(416, 1) kv4_attn_tiles_kernel(AttnParams p) {
                 page[u] = i < n && key < q.len ? __ldg(table + (key >> p.c.page_shift)) : -1;
             }
         };
-        // loads tile i; a key without a page of the pool counts as absent, one behind the end is masked by its position
-        const auto load = [&](int i) {
-            if (i >= n) return;
+        const auto load = [&](int i, const uint8_t* codes, const uint32_t* params, uint4 (&raw)[ROUNDS], uint32_t (&par)[ROUNDS][NG], bool keys) {
 #pragma unroll
             for (int u = 0; u < ROUNDS; u++) {
                 const int key = (walk.first + i) * BLOCK + tok0 + u * PER_ROUND;
-                raw.k[u] = make_uint4(0, 0, 0, 0); raw.v[u] = raw.k[u];
+                raw[u] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-                for (int g = 0; g < NG; g++) { raw.kp[u][g] = 0; raw.vp[u][g] = 0; }
-                bool good = key < q.len;
-                if (good && (page[u] < 0 || page[u] >= p.c.pages)) { good = false; if (piece == 0) *p.status = OXQ_ERR_INVALID_ARGUMENT; }
+                for (int g = 0; g < NG; g++) par[u][g] = 0;
+                const bool inside = i < n && key < q.len, good = inside && page[u] >= 0 && page[u] < p.c.pages;
+                if (keys) {
+                    gone[u] = inside && !good;
+                    if (gone[u] && piece == 0) *p.status = OXQ_ERR_INVALID_ARGUMENT;
+                }
                 if (good) {
                     const int64_t row = (((int64_t)page[u] * p.c.heads + head) << p.c.page_shift) + (key & ((1 << p.c.page_shift) - 1));
-                    raw.k[u] = __ldg(reinterpret_cast<const uint4*>(p.c.kc + row * (D / 2)) + piece);
-                    raw.v[u] = __ldg(reinterpret_cast<const uint4*>(p.c.vc + row * (D / 2)) + piece);
-#pragma unroll
-                    for (int g = 0; g < NG; g++) { raw.kp[u][g] = __ldg(p.c.kp + row * NG + g); raw.vp[u][g] = __ldg(p.c.vp + row * NG + g); }
+                    raw[u] = __ldg(reinterpret_cast<const uint4*>(codes + row * (D / 2)) + piece);
+                    if constexpr (NG == 2) {
+                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(params + row * 2));
+                        par[u][0] = v.x; par[u][1] = v.y;
+                    } else par[u][0] = __ldg(params + row);
                 }
             }
         };
-        const auto put = [&](uint32_t tile, bool keys) {
+        const auto put = [&](uint32_t tile, const uint4 (&raw)[ROUNDS], const uint32_t (&par)[ROUNDS][NG], bool keys) {
 #pragma unroll
             for (int u = 0; u < ROUNDS; u++) {
                 const int tok = tok0 + u * PER_ROUND;
-                const uint4 w4 = keys ? raw.k[u] : raw.v[u];
-                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
                 __half2 s[NG], m[NG];
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
-                    const __half2 sm = __hmul2(as_half2(keys ? raw.kp[u][g] : raw.vp[u][g]), as_half2(0x38003800u));        // halved
+                    const __half2 sm = __hmul2(as_half2(par[u][g]), as_half2(0x38003800u));        // halved
                     s[g] = __low2half2(sm); m[g] = __high2half2(sm);
                 }
 #pragma unroll
@@ -369,18 +382,14 @@ __global__ void __launch_bounds__(416, 1) kv4_attn_tiles_kernel(AttnParams p) {
             }
         };
         get_pages(0);
-        load(0);
+        load(0, p.c.kc, p.c.kp, kraw, kpar, true);
+        load(0, p.c.vc, p.c.vp, vraw, vpar, false);
+        get_pages(1);
         for (int i = 0; i < n; i++) {
             const int st = i & 1;
             const uint32_t ph = (i >> 1) & 1;
-            bool gone[ROUNDS];
-#pragma unroll
-            for (int u = 0; u < ROUNDS; u++) {
-                const int key = (walk.first + i) * BLOCK + tok0 + u * PER_ROUND;
-                gone[u] = key < q.len && (page[u] < 0 || page[u] >= p.c.pages);
-            }
             if (!mbar_wait_warp(bar(BAR_KEMPTY + st), ph ^ 1)) { if (lane == 0) fail(); break; }
-            put(base + L::K + st * L::OPERAND, true);
+            put(base + L::K + st * L::OPERAND, kraw, kpar, true);
 #pragma unroll
             for (int u = 0; u < ROUNDS; u++) {
                 const int tok = tok0 + u * PER_ROUND;
@@ -388,14 +397,17 @@ __global__ void __launch_bounds__(416, 1) kv4_attn_tiles_kernel(AttnParams p) {
             }
             fence_proxy_async();
             mbar_arrive(bar(BAR_KFULL + st));
+            load(i + 1, p.c.kc, p.c.kp, kraw, kpar, true);
             if (!mbar_wait_warp(bar(BAR_VEMPTY + st), ph ^ 1)) { if (lane == 0) fail(); break; }
-            put(base + L::V + st * L::OPERAND, false);
+            put(base + L::V + st * L::OPERAND, vraw, vpar, false);
             fence_proxy_async();
             mbar_arrive(bar(BAR_VFULL + st));
-            get_pages(i + 1);
-            load(i + 1);
+            load(i + 1, p.c.vc, p.c.vp, vraw, vpar, false);
+            get_pages(i + 2);
         }
     } else {
+        fewer_registers<64>();
+        if (warp == MMA_WARP) {
         // ------------------------------------------------------------------------------------ products (whole warp, one lane issues)
         constexpr uint32_t id_s = idesc_dense(1, 0, 0, BLOCK, BLOCK), id_o = idesc_dense(1, 0, 0, BLOCK, D) | idesc_majors(0, 1);
         const auto scores = [&](int t, int st) {
@@ -456,10 +468,11 @@ __global__ void __launch_bounds__(416, 1) kv4_attn_tiles_kernel(AttnParams p) {
             __syncwarp();
             mbar_wait_warp(bar(BAR_END), 0);
         }
+        }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == MMA_WARP) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -508,7 +521,7 @@ static int32_t launch_tiles(oxq_handle* h, const AttnParams& p, int64_t items) {
         ready.set(h->device, 1);
     }
     const dim3 grid((unsigned)(items * p.c.heads), (unsigned)p.parts);
-    OXQ_CUDA(h, oxq_launch(kernel, grid, 416, bytes, h->stream, p));
+    OXQ_CUDA(h, oxq_launch(kernel, grid, THREADS, bytes, h->stream, p));
     if (p.parts > 1) OXQ_CUDA(h, oxq_launch(kv4_tiles_join_kernel<T, D>, dim3(grid.x, 2 * BLOCK / (256 / (D / 4))), 256, 0, h->stream, p));
     return OXQ_OK;
 }
