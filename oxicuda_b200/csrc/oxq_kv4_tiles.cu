@@ -40,6 +40,25 @@ __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast
 __device__ __forceinline__ float lower(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v & 0xFFFFu))); }
 __device__ __forceinline__ float upper(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
 
+// two f32 operations in one instruction, and the largest of three
+__device__ __forceinline__ uint64_t two(float x, float y) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ void apart(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // Eight codes of a word to f16 c s + m, one rounding each, in the order 0 4 1 5 2 6 3 7.  A nibble under the exponent of 1024
 // is the number 1024 + c (or 1024 + 16 c where it is left four bits up), from which c is exact in one operation.
 __device__ __forceinline__ uint4 expand(uint32_t w, __half2 s, __half2 m) {
@@ -196,7 +215,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
         const int all_hi = __reduce_min_sync(0xffffffffu, real ? vhi : INT32_MAX), all_lo = __reduce_max_sync(0xffffffffu, real ? vlo : 0);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_col = tmem + t * BLOCK + lanes, o_col = tmem + 256 + t * BLOCK + lanes;
-        float M = -1e30f, l = 0.0f;
+        float M = -1e30f;
+        uint64_t l2 = 0;                        // the sum in two halves
+        const uint64_t a2 = two(a, a);
         bool ok = true;
         for (int i = 0; i < n; i++) {
             ok = mbar_wait_warp(bar(BAR_S + t), i & 1);
@@ -206,11 +227,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
             const uint32_t* valid = reinterpret_cast<const uint32_t*>(smem + L::VALID + (i & 3) * 8);
             const uint32_t v0 = valid[0], v1 = valid[1];
             const bool masked = t0 < all_lo || t0 + BLOCK > all_hi || (v0 & v1) != 0x01010101u;
+            uint32_t buf[2][32];                // a chunk of 32 keys, and the next one on its way
+            tmem_ld_32x32b_x32(s_col, buf[0]);
 #pragma unroll
             for (int ch = 0; ch < 4; ch++) {
-                uint32_t s[32];
-                tmem_ld_32x32b_x32(s_col + 32 * ch, s);
+                uint32_t (&s)[32] = buf[ch & 1];
                 tmem_ld_wait();
+                if (ch < 3) tmem_ld_32x32b_x32(s_col + 32 * (ch + 1), buf[(ch + 1) & 1]);
                 if (masked) {
                     const uint32_t vw = ch < 2 ? v0 : v1;
 #pragma unroll
@@ -220,17 +243,24 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
                         if (key < vlo || key >= vhi || !have) s[e] = 0xFF800000u;
                     }
                 }
-                float top = __uint_as_float(s[0]);
+                const auto at = [&](int e) { return __uint_as_float(s[e]); };
+                float top[4];
 #pragma unroll
-                for (int e = 1; e < 32; e++) top = fmaxf(top, __uint_as_float(s[e]));
-                top *= a;
-                const bool over = top > M + 8.0f;
+                for (int e = 0; e < 4; e++) top[e] = max3(at(e), at(4 + e), at(8 + e));
+#pragma unroll
+                for (int e = 12; e < 28; e += 8)
+#pragma unroll
+                    for (int f = 0; f < 4; f++) top[f] = max3(top[f], at(e + f), at(e + 4 + f));
+                const float most = fmaxf(max3(max3(top[0], top[1], at(28)), max3(top[2], top[3], at(29)), at(30)), at(31)) * a;
+                const bool over = most > M + 8.0f;
                 if (__any_sync(0xffffffffu, over)) {
                     // the reference moves: what was summed so far shrinks with it -- l, O (the last product into it is complete:
                     // it was issued before these scores), and the part of this tile's P that is already written
-                    const float to = over ? top : M, f = exp2_approx(M - to);
+                    const float to = over ? most : M, f = exp2_approx(M - to);
                     M = to;
-                    l *= f;
+                    float lx, ly;
+                    apart(l2, lx, ly);
+                    l2 = two(lx * f, ly * f);
                     if (i > 0) {
 #pragma unroll 1
                         for (int c0 = 0; c0 < D; c0 += 16) {
@@ -253,11 +283,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
                         tmem_st_32x32b_x16(s_col + 16 * c0, o);
                     }
                 }
+                const uint64_t m2 = two(-M, -M);
                 uint32_t o[16];
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    const float x = exp2_approx(fmaf(__uint_as_float(s[2 * e]), a, -M)), y = exp2_approx(fmaf(__uint_as_float(s[2 * e + 1]), a, -M));
-                    l += x + y;
+                    float x, y;
+                    apart(fma2(two(at(2 * e), at(2 * e + 1)), a2, m2), x, y);
+                    x = exp2_approx(x);
+                    y = exp2_approx(y);
+                    l2 = add2(l2, two(x, y));
                     o[e] = pack2(x, y);
                 }
                 tmem_st_32x32b_x16(s_col + 16 * ch, o);
@@ -271,6 +305,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
             if (!ok && lane == 0) fail();
             tc_fence_after();
         }
+        float l, l_odd;
+        apart(l2, l, l_odd);
+        l += l_odd;
         if (ok) {
             float* slot = p.parts > 1 ? p.ws + ((int64_t)blockIdx.x * p.parts + part) * (2 * BLOCK * (D + 2)) : nullptr;
             const float inv = l > 0.0f ? 2.0f / l : l != l ? l : 0.0f;                                    // 2: the values are halved
