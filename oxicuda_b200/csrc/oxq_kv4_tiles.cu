@@ -37,8 +37,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
-__device__ __forceinline__ float lower(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v & 0xFFFFu))); }
-__device__ __forceinline__ float upper(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
 
 // two f32 operations in one instruction, and the largest of three
 __device__ __forceinline__ uint64_t two(float x, float y) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
@@ -73,7 +71,7 @@ __device__ __forceinline__ uint4 expand(uint32_t w, __half2 s, __half2 m) {
 }
 
 // Threads: warpgroups 0, 1 softmax, 2, 3 producers, 4 (its first warp) products.  Registers a thread after the split: launched with
-// 96 x 640 = 61440 in all, 2 x 128 x 144 + 2 x 128 x 64 + 128 x 64 = 61440.
+// 96 x 640 = 61440 in all, 2 x 128 x 168 + 2 x 128 x 56 + 128 x 32 = 61440.
 constexpr int THREADS = 640, PRODUCERS = 256, MMA_WARP = 16;
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -165,7 +163,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
 
     if (warp < 8) {
         // ------------------------------------------------------------------------------------ softmax: one row a thread
-        more_registers<144>();
+        more_registers<168>();
         const int t = warp >> 2, r = (warp & 3) * 32 + lane;
         const int row = it.pair * 2 * BLOCK + t * BLOCK + r;
         const bool real = row < q.n * p.per;
@@ -216,7 +214,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_col = tmem + t * BLOCK + lanes, o_col = tmem + 256 + t * BLOCK + lanes;
         float M = -1e30f;
-        uint64_t l2 = 0;                        // the sum in two halves
+        uint64_t l2[2] = {0, 0};                // the sum in four parts
         const uint64_t a2 = two(a, a);
         bool ok = true;
         for (int i = 0; i < n; i++) {
@@ -227,71 +225,64 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
             const uint32_t* valid = reinterpret_cast<const uint32_t*>(smem + L::VALID + (i & 3) * 8);
             const uint32_t v0 = valid[0], v1 = valid[1];
             const bool masked = t0 < all_lo || t0 + BLOCK > all_hi || (v0 & v1) != 0x01010101u;
-            uint32_t buf[2][32];                // a chunk of 32 keys, and the next one on its way
-            tmem_ld_32x32b_x32(s_col, buf[0]);
+            uint32_t s[4][32];
 #pragma unroll
-            for (int ch = 0; ch < 4; ch++) {
-                uint32_t (&s)[32] = buf[ch & 1];
-                tmem_ld_wait();
-                if (ch < 3) tmem_ld_32x32b_x32(s_col + 32 * (ch + 1), buf[(ch + 1) & 1]);
-                if (masked) {
-                    const uint32_t vw = ch < 2 ? v0 : v1;
+            for (int ch = 0; ch < 4; ch++) tmem_ld_32x32b_x32(s_col + 32 * ch, s[ch]);
+            tmem_ld_wait();
+            if (masked) {
 #pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        const int key = t0 + 32 * ch + e;
-                        const bool have = (vw >> (8 * ((ch & 1) * 2 + (e >> 4)))) & 1u;
-                        if (key < vlo || key >= vhi || !have) s[e] = 0xFF800000u;
-                    }
+                for (int e = 0; e < 128; e++) {
+                    const int key = t0 + e;
+                    const bool have = ((e < 64 ? v0 : v1) >> (8 * ((e >> 4) & 3))) & 1u;
+                    if (key < vlo || key >= vhi || !have) s[e >> 5][e & 31] = 0xFF800000u;
                 }
-                const auto at = [&](int e) { return __uint_as_float(s[e]); };
-                float top[4];
+            }
+            const auto at = [&](int e) { return __uint_as_float(s[e >> 5][e & 31]); };
+            float top[8];
 #pragma unroll
-                for (int e = 0; e < 4; e++) top[e] = max3(at(e), at(4 + e), at(8 + e));
+            for (int e = 0; e < 8; e++) top[e] = max3(at(e), at(8 + e), at(16 + e));
 #pragma unroll
-                for (int e = 12; e < 28; e += 8)
+            for (int e = 24; e < 120; e += 16)
 #pragma unroll
-                    for (int f = 0; f < 4; f++) top[f] = max3(top[f], at(e + f), at(e + 4 + f));
-                const float most = fmaxf(max3(max3(top[0], top[1], at(28)), max3(top[2], top[3], at(29)), at(30)), at(31)) * a;
-                const bool over = most > M + 8.0f;
-                if (__any_sync(0xffffffffu, over)) {
-                    // the reference moves: what was summed so far shrinks with it -- l, O (the last product into it is complete:
-                    // it was issued before these scores), and the part of this tile's P that is already written
-                    const float to = over ? most : M, f = exp2_approx(M - to);
-                    M = to;
-                    float lx, ly;
-                    apart(l2, lx, ly);
-                    l2 = two(lx * f, ly * f);
-                    if (i > 0) {
+                for (int f = 0; f < 8; f++) top[f] = max3(top[f], at(e + f), at(e + 8 + f));
+#pragma unroll
+            for (int f = 0; f < 8; f++) top[f] = fmaxf(top[f], at(120 + f));
+            const float most = fmaxf(max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]), top[6]), top[7]) * a;
+            const bool over = most > M + 8.0f;
+            if (__any_sync(0xffffffffu, over)) {
+                // the reference moves: what was summed so far shrinks with it -- l, and O (the last product into it is
+                // complete: it was issued before these scores)
+                const float to = over ? most : M, f = exp2_approx(M - to);
+                M = to;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float x, y;
+                    apart(l2[h], x, y);
+                    l2[h] = two(x * f, y * f);
+                }
+                if (i > 0) {
 #pragma unroll 1
-                        for (int c0 = 0; c0 < D; c0 += 16) {
-                            uint32_t o[16];
-                            tmem_ld_32x32b_x16(o_col + c0, o);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            tmem_st_32x32b_x16(o_col + c0, o);
-                        }
-                    }
-#pragma unroll 1
-                    for (int c0 = 0; c0 < ch; c0++) {
+                    for (int c0 = 0; c0 < D; c0 += 16) {
                         uint32_t o[16];
-                        tmem_st_wait();
-                        tmem_ld_32x32b_x16(s_col + 16 * c0, o);
+                        tmem_ld_32x32b_x16(o_col + c0, o);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 16; e++) o[e] = pack2(lower(o[e]) * f, upper(o[e]) * f);
-                        tmem_st_32x32b_x16(s_col + 16 * c0, o);
+                        for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st_32x32b_x16(o_col + c0, o);
                     }
                 }
-                const uint64_t m2 = two(-M, -M);
+            }
+            const uint64_t m2 = two(-M, -M);
+#pragma unroll
+            for (int ch = 0; ch < 4; ch++) {
                 uint32_t o[16];
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     float x, y;
-                    apart(fma2(two(at(2 * e), at(2 * e + 1)), a2, m2), x, y);
+                    apart(fma2(two(at(32 * ch + 2 * e), at(32 * ch + 2 * e + 1)), a2, m2), x, y);
                     x = exp2_approx(x);
                     y = exp2_approx(y);
-                    l2 = add2(l2, two(x, y));
+                    l2[e & 1] = add2(l2[e & 1], two(x, y));
                     o[e] = pack2(x, y);
                 }
                 tmem_st_32x32b_x16(s_col + 16 * ch, o);
@@ -306,7 +297,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
             tc_fence_after();
         }
         float l, l_odd;
-        apart(l2, l, l_odd);
+        apart(add2(l2[0], l2[1]), l, l_odd);
         l += l_odd;
         if (ok) {
             float* slot = p.parts > 1 ? p.ws + ((int64_t)blockIdx.x * p.parts + part) * (2 * BLOCK * (D + 2)) : nullptr;
@@ -354,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
         }
     } else if (warp < MMA_WARP) {
         // ------------------------------------------------------------------------------------ codes to f16 tiles
-        fewer_registers<64>();
+        fewer_registers<56>();
         constexpr int Q16 = D / 32;                                 // 16-byte pieces of a row
         constexpr int ROUNDS = BLOCK * Q16 / PRODUCERS, PER_ROUND = PRODUCERS / Q16;
         const int pt = tid - 256, piece = pt % Q16, tok0 = pt / Q16;
@@ -443,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
             get_pages(i + 2);
         }
     } else {
-        fewer_registers<64>();
+        fewer_registers<32>();
         if (warp == MMA_WARP) {
         // ------------------------------------------------------------------------------------ products (whole warp, one lane issues)
         constexpr uint32_t id_s = idesc_dense(1, 0, 0, BLOCK, BLOCK), id_o = idesc_dense(1, 0, 0, BLOCK, D) | idesc_majors(0, 1);
