@@ -28,7 +28,7 @@ template <int D> struct TileSmem {
     static constexpr int OPERAND = ATOM * (D / 64);
     static constexpr int Q = 0, K = Q + 2 * OPERAND, V = K + 2 * OPERAND, BARS = V + 2 * OPERAND, VALID = BARS + 128, SLOT = VALID + 32, BYTES = SLOT + 16 + 1024;
 };
-enum { BAR_Q = 0, BAR_KFULL = 1, BAR_KEMPTY = 3, BAR_VFULL = 5, BAR_VEMPTY = 7, BAR_S = 9, BAR_P = 11, BAR_END = 13 };
+enum { BAR_Q = 0, BAR_KFULL = 1, BAR_KEMPTY = 3, BAR_VFULL = 5, BAR_VEMPTY = 7, BAR_S = 9, BAR_P = 11, BAR_END = 13, BAR_P2 = 14 };      // P in halves of 64 keys
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t r;
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
             for (int i = 0; i < 2; i++) {
                 mbar_init(bar(BAR_KFULL + i), PRODUCERS); mbar_init(bar(BAR_KEMPTY + i), 1);
                 mbar_init(bar(BAR_VFULL + i), PRODUCERS); mbar_init(bar(BAR_VEMPTY + i), 1);
-                mbar_init(bar(BAR_S + i), 1); mbar_init(bar(BAR_P + i), 128);
+                mbar_init(bar(BAR_S + i), 1); mbar_init(bar(BAR_P + i), 128); mbar_init(bar(BAR_P2 + i), 128);
             }
             fence_barrier_init();
         }
@@ -226,27 +226,36 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
             const uint32_t v0 = valid[0], v1 = valid[1];
             const bool masked = t0 < all_lo || t0 + BLOCK > all_hi || (v0 & v1) != 0x01010101u;
             uint32_t s[4][32];
-#pragma unroll
-            for (int ch = 0; ch < 4; ch++) tmem_ld_32x32b_x32(s_col + 32 * ch, s[ch]);
-            tmem_ld_wait();
-            if (masked) {
-#pragma unroll
-                for (int e = 0; e < 128; e++) {
-                    const int key = t0 + e;
-                    const bool have = ((e < 64 ? v0 : v1) >> (8 * ((e >> 4) & 3))) & 1u;
-                    if (key < vlo || key >= vhi || !have) s[e >> 5][e & 31] = 0xFF800000u;
-                }
-            }
             const auto at = [&](int e) { return __uint_as_float(s[e >> 5][e & 31]); };
             float top[8];
+            // the second half is on its way while the first one's largest is found
+            tmem_ld_32x32b_x32(s_col, s[0]);
+            tmem_ld_32x32b_x32(s_col + 32, s[1]);
+            tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 8; e++) top[e] = max3(at(e), at(8 + e), at(16 + e));
+            for (int h = 0; h < 2; h++) {
+                if (h == 0) {
+                    tmem_ld_32x32b_x32(s_col + 64, s[2]);
+                    tmem_ld_32x32b_x32(s_col + 96, s[3]);
+                } else {
+                    tmem_ld_wait();
+                }
+                if (masked) {
 #pragma unroll
-            for (int e = 24; e < 120; e += 16)
+                    for (int e = 64 * h; e < 64 * h + 64; e++) {
+                        const int key = t0 + e;
+                        const bool have = ((h ? v1 : v0) >> (8 * ((e >> 4) & 3))) & 1u;
+                        if (key < vlo || key >= vhi || !have) s[e >> 5][e & 31] = 0xFF800000u;
+                    }
+                }
 #pragma unroll
-                for (int f = 0; f < 8; f++) top[f] = max3(top[f], at(e + f), at(e + 8 + f));
+                for (int f = 0; f < 8; f++) {
+                    float x = h ? max3(top[f], at(64 + f), at(72 + f)) : fmaxf(at(f), at(8 + f));
 #pragma unroll
-            for (int f = 0; f < 8; f++) top[f] = fmaxf(top[f], at(120 + f));
+                    for (int e = 16; e < 64; e += 16) x = max3(x, at(64 * h + e + f), at(64 * h + e + 8 + f));
+                    top[f] = x;
+                }
+            }
             const float most = fmaxf(max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]), top[6]), top[7]) * a;
             const bool over = most > M + 8.0f;
             if (__any_sync(0xffffffffu, over)) {
@@ -286,10 +295,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
                     o[e] = pack2(x, y);
                 }
                 tmem_st_32x32b_x16(s_col + 16 * ch, o);
+                if (ch & 1) {                       // the product with the first half need not wait for the second
+                    tmem_st_wait();
+                    tc_fence_before();
+                    mbar_arrive(bar((ch == 1 ? BAR_P : BAR_P2) + t));
+                }
             }
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(bar(BAR_P + t));
         }
         if (ok && n > 0) {
             ok = mbar_wait_warp(bar(BAR_S + t), n & 1);         // the last product into O
@@ -447,10 +458,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
                 for (int kk = 0; kk < 4; kk++) mma_f16(tmem + t * BLOCK, ad + kk * 2, bd + kk * 2, id_s, (at | kk) != 0);
             }
         };
-        const auto sums = [&](int t, int st, bool more) {
+        const auto sums = [&](int t, int st, bool more, int half) {
             const uint64_t bd = smem_desc_mn_sw128(base + L::V + st * L::OPERAND, ATOM);
 #pragma unroll
-            for (int kk = 0; kk < BLOCK / 16; kk++) mma_f16_ts(tmem + 256 + t * BLOCK, tmem + t * BLOCK + kk * 8, bd + kk * 128, id_o, more || kk != 0);
+            for (int kk = half * (BLOCK / 32); kk < (half + 1) * (BLOCK / 32); kk++) mma_f16_ts(tmem + 256 + t * BLOCK, tmem + t * BLOCK + kk * 8, bd + kk * 128, id_o, more || kk != 0);
         };
         bool ok = true;
         if (n > 0) {
@@ -468,27 +479,29 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
         }
         for (int i = 0; i < n && ok; i++) {
             const int st = i & 1, nx = (i + 1) & 1;
-            ok = mbar_wait_warp(bar(BAR_VFULL + st), (i >> 1) & 1) && mbar_wait_warp(bar(BAR_P), i & 1);
-            if (ok && i + 1 < n) ok = mbar_wait_warp(bar(BAR_KFULL + nx), ((i + 1) >> 1) & 1);
-            if (!ok) { if (lane == 0) fail(); break; }
-            tc_fence_after();
-            if (elect_one()) {
-                sums(0, st, i > 0);
-                if (i + 1 < n) scores(0, nx);
-                tc_commit(bar(BAR_S));
+            ok = mbar_wait_warp(bar(BAR_VFULL + st), (i >> 1) & 1);
+            for (int t = 0; t < 2 && ok; t++) {
+                ok = mbar_wait_warp(bar(BAR_P + t), i & 1);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) sums(t, st, i > 0, 0);
+                __syncwarp();
+                if (t == 0 && i + 1 < n) ok = mbar_wait_warp(bar(BAR_KFULL + nx), ((i + 1) >> 1) & 1);
+                ok = ok && mbar_wait_warp(bar(BAR_P2 + t), i & 1);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    sums(t, st, true, 1);
+                    if (i + 1 < n) scores(t, nx);
+                    tc_commit(bar(BAR_S + t));
+                    if (t == 1) {
+                        tc_commit(bar(BAR_VEMPTY + st));
+                        if (i + 1 < n) tc_commit(bar(BAR_KEMPTY + nx));
+                    }
+                }
+                __syncwarp();
             }
-            __syncwarp();
-            ok = mbar_wait_warp(bar(BAR_P + 1), i & 1);
             if (!ok) { if (lane == 0) fail(); break; }
-            tc_fence_after();
-            if (elect_one()) {
-                sums(1, st, i > 0);
-                if (i + 1 < n) scores(1, nx);
-                tc_commit(bar(BAR_S + 1));
-                tc_commit(bar(BAR_VEMPTY + st));
-                if (i + 1 < n) tc_commit(bar(BAR_KEMPTY + nx));
-            }
-            __syncwarp();
         }
         if (!ok) {
             // Something did not arrive.  What was issued still has to end, with a limit, before tensor memory is given back.
