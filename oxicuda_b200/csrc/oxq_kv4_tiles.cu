@@ -138,32 +138,19 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
     const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     unsigned char* smem = smem_dyn + (base - smem_u32(smem_dyn));
     const auto bar = [&](int i) { return base + L::BARS + 8 * i; };
-    if (warp == MMA_WARP) {
-        if (lane == 0) {
-            mbar_init(bar(BAR_Q), 256);
-            mbar_init(bar(BAR_END), 1);
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                mbar_init(bar(BAR_KFULL + i), PRODUCERS); mbar_init(bar(BAR_KEMPTY + i), 1);
-                mbar_init(bar(BAR_VFULL + i), PRODUCERS); mbar_init(bar(BAR_VEMPTY + i), 1);
-                mbar_init(bar(BAR_S + i), 1); mbar_init(bar(BAR_P + i), 128); mbar_init(bar(BAR_P2 + i), 128);
-            }
-            fence_barrier_init();
-        }
-        __syncwarp();
-        tmem_alloc(base + L::SLOT, 512);
-        tmem_relinquish();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    pdl_trigger();                              // only now: a kernel that starts early must not find tensor memory before this one
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::SLOT);
+    // Each role asks for its first data, then meets the others: barriers and tensor memory are set up by the last one.
+    uint32_t tmem = 0;
+    const auto ready = [&]() {
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        pdl_trigger();                          // only now: a kernel that starts early must not find tensor memory before this one
+        tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::SLOT);
+    };
     const auto fail = [&]() { *p.status = OXQ_ERR_DEVICE_TIMEOUT; };
 
     if (warp < 8) {
         // ------------------------------------------------------------------------------------ softmax: one row a thread
-        more_registers<168>();
         const int t = warp >> 2, r = (warp & 3) * 32 + lane;
         const int row = it.pair * 2 * BLOCK + t * BLOCK + r;
         const bool real = row < q.n * p.per;
@@ -186,6 +173,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
                     raw[i] = real ? (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(src) + 2 * i) |
                                         ((uint32_t)__ldg(reinterpret_cast<const unsigned short*>(src) + 2 * i + 1) << 16) : 0u;
             }
+            ready();
+            more_registers<168>();
             const auto value = [&](int e) {
                 const unsigned short h = (unsigned short)(raw[e >> 1] >> (16 * (e & 1)));
                 if constexpr (Elem<T>::kDtype == OXQ_BF16) return __uint_as_float((uint32_t)h << 16);
@@ -225,7 +214,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
             const uint32_t* valid = reinterpret_cast<const uint32_t*>(smem + L::VALID + (i & 3) * 8);
             const uint32_t v0 = valid[0], v1 = valid[1];
             const bool masked = t0 < all_lo || t0 + BLOCK > all_hi || (v0 & v1) != 0x01010101u;
-            uint32_t s[4][32];
+            uint32_t s[4][32];                  // loaded below, in two halves
             const auto at = [&](int e) { return __uint_as_float(s[e >> 5][e & 31]); };
             float top[8];
             // the second half is on its way while the first one's largest is found
@@ -356,7 +345,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
         }
     } else if (warp < MMA_WARP) {
         // ------------------------------------------------------------------------------------ codes to f16 tiles
-        fewer_registers<56>();
         constexpr int Q16 = D / 32;                                 // 16-byte pieces of a row
         constexpr int ROUNDS = BLOCK * Q16 / PRODUCERS, PER_ROUND = PRODUCERS / Q16;
         const int pt = tid - 256, piece = pt % Q16, tok0 = pt / Q16;
@@ -424,6 +412,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
         load(0, p.c.kc, p.c.kp, kraw, kpar, true);
         load(0, p.c.vc, p.c.vp, vraw, vpar, false);
         get_pages(1);
+        ready();
+        fewer_registers<56>();
         for (int i = 0; i < n; i++) {
             const int st = i & 1;
             const uint32_t ph = (i >> 1) & 1;
@@ -445,6 +435,23 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
             get_pages(i + 2);
         }
     } else {
+        if (warp == MMA_WARP) {
+            if (lane == 0) {
+                mbar_init(bar(BAR_Q), 256);
+                mbar_init(bar(BAR_END), 1);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    mbar_init(bar(BAR_KFULL + i), PRODUCERS); mbar_init(bar(BAR_KEMPTY + i), 1);
+                    mbar_init(bar(BAR_VFULL + i), PRODUCERS); mbar_init(bar(BAR_VEMPTY + i), 1);
+                    mbar_init(bar(BAR_S + i), 1); mbar_init(bar(BAR_P + i), 128); mbar_init(bar(BAR_P2 + i), 128);
+                }
+                fence_barrier_init();
+            }
+            __syncwarp();
+            tmem_alloc(base + L::SLOT, 512);
+            tmem_relinquish();
+        }
+        ready();
         fewer_registers<32>();
         if (warp == MMA_WARP) {
         // ------------------------------------------------------------------------------------ products (whole warp, one lane issues)
