@@ -479,10 +479,10 @@ OXQ_API int32_t oxq_residual_rmsnorm_int8_rows(oxq_handle* h, const oxq_residual
  * The batch: sequence b owns the call's tokens cu_tokens[b] .. cu_tokens[b + 1] (not decreasing; seqs + 1 offsets), and they
  * are its last ones: with them it has seq_lens[b] tokens, the last at position seq_lens[b] - 1.  Position p lives in page
  * block_table[b][p / page_size].  All three arrays are device memory and are read when the kernels run; `tokens` is the number
- * of rows of the token arrays.  Rows behind the last sequence are not read, and left as they were.  Two sequences may
+ * of rows of the token arrays.  A table row covers at most 2^30 positions.  Rows behind the last sequence are not read, and left as they were.  Two sequences may
  * share pages that are only read; two tokens of one append must not share a place (its contents are then unspecified).  A
  * table entry that names no page of the pool, or a position behind the table's end, is never followed: an append skips the
- * token, a read gives zeros, attention leaves the keys out, and oxq_device_status() then returns
+ * token, a read gives zeros, attention leaves the keys out (the queries' positions stay those of seq_lens), and oxq_device_status() then returns
  * OXQ_ERR_INVALID_ARGUMENT.  A token before position 0 (more tokens than seq_lens) is skipped, reads as zeros, sees no key.
  *
  * oxq_kv4_append  keys and values [tokens][heads][dim] of `dtype` with any token and head strides (in elements; elements of a
@@ -494,7 +494,7 @@ OXQ_API int32_t oxq_residual_rmsnorm_int8_rows(oxq_handle* h, const oxq_residual
  *                 A query that sees no key gives zeros.  lse (f32 [tokens][q_heads], may be NULL) receives
  *                 ln(sum(exp(scale * q . k))), -inf where nothing is seen.  max_tokens: the most tokens that a sequence has in
  *                 this call (0: not known); it chooses kernels and sizes the workspace, results are right whatever it says.
- *                 Out rows have strides like q's and are 4-byte aligned.  Scores, the softmax's statistics and the sums
+ *                 Out rows have strides like q's, are 4-byte aligned and overlap no input.  Scores, the softmax's statistics and the sums
  *                 are f32.  The workspace (oxq_kv4_attention_workspace_bytes of the same call; the batch's arrays are not looked
  *                 at; 16-byte aligned) needs no initial value and holds nothing between calls; calls that may overlap need one
  *                 each. */

@@ -307,7 +307,7 @@ int32_t oxq_kv4_check(oxq_handle* h, const oxq_kv4_cache* c, const oxq_kv4_batch
         OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4: null pool pointer, or one that is not 16-byte aligned");
     if (s->seqs < 0 || s->tokens < 0 || s->table_width < 0 || s->seqs > (1 << 24) || s->table_width > (1 << 27) || s->tokens > INT32_MAX)
         OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4: %lld sequences, %lld tokens, a table of %lld columns", (long long)s->seqs, (long long)s->tokens, (long long)s->table_width);
-    if (s->table_width * c->page_size > INT32_MAX)
+    if (s->table_width * c->page_size > (1 << 30))
         OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4: a table row covers %lld tokens", (long long)(s->table_width * c->page_size));
     if (s->seqs > 0 && s->tokens > 0 && ((!s->block_table && s->table_width > 0) || !s->seq_lens || !s->cu_tokens))
         OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4: null block table, lengths or token offsets");

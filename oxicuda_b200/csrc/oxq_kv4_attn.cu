@@ -65,8 +65,8 @@ struct Span { int first, tiles; int lo, hi; };          // first tile, how many 
 __device__ __forceinline__ Span item_span(const AttnParams& p, const SeqInfo& q, int rt, int nr) {
     Span s;
     const int j0 = p.by_per.div(rt * nr), j1 = p.by_per.div(min((rt + 1) * nr, q.n * p.per) - 1);
-    s.hi = p.causal ? min(q.len, q.len - q.asked + j1 + 1) : q.len;
-    s.lo = p.window > 0 ? max(0, q.len - q.asked + j0 + 1 - p.window) : 0;
+    s.hi = p.causal ? min(q.len, q.before + j1 + 1) : q.len;
+    s.lo = p.window > 0 ? max(0, q.before + j0 + 1 - p.window) : 0;
     s.hi = max(s.hi, 0);
     s.first = min(s.lo, s.hi) / TILE;
     s.tiles = max(1, (s.hi + TILE - 1) / TILE - s.first);
@@ -101,6 +101,7 @@ struct Where { int b, at; };            // sequence, and the line's position of 
 __device__ __forceinline__ Line find_part(const AttnParams& p, int nr, int ctas, int k, int* red, Where* found) {
     Line line;
     int want = -1;
+    if (threadIdx.x == 0) *found = Where{0, 0};
     for (int pass = 0; pass < 2; pass++) {
         int base = 0, mine = 0, start = 0;
         for (int b0 = 0; b0 < p.s.seqs; b0 += 256) {
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
     __syncthreads();                                                  // the barriers are set up
     if (more) prime(wk);
     for (int turn = 0; more; turn ^= 1) {
-        const int ta = wk.ta, tb = wk.tb, len = wk.seq.len, before = wk.seq.len - wk.seq.asked, first = wk.it.span.first;
+        const int ta = wk.ta, tb = wk.tb, len = wk.seq.len, before = wk.seq.before, first = wk.it.span.first;
         const int row0 = wk.it.rt * ROWS;
         // keys that every row of the block sees need no mask
         const int pos0 = before + p.by_per.div(row0), pos1 = before + p.by_per.div(min(row0 + ROWS, wk.seq.n * p.per) - 1);
@@ -613,7 +614,7 @@ __global__ void __launch_bounds__(512) kv4_attn_join_kernel(AttnParams p) {
     pdl_trigger();
     pdl_wait();
     const int4 note = *reinterpret_cast<const int4*>(reinterpret_cast<const Cut*>(p.ws) + blockIdx.x);
-    const int first = blockIdx.x, last = note.w;
+    const int first = blockIdx.x, last = min(note.w, (int)gridDim.x - 1);
     if (last < 0) return;
     const SeqInfo seq = {note.x, note.y, 0, 0};
     const int blocks = row_blocks(p, seq, ROWS), head = note.z / blocks, row0 = (note.z - head * blocks) * ROWS, rows = min(ROWS, seq.n * p.per - row0);
@@ -753,7 +754,8 @@ int32_t oxq_kv4_attention(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_k
     const int64_t per = a->q_heads / p.c.heads;
     if (p.s.tokens * per > INT32_MAX / 2) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 attention: too many query rows");
     const Plan plan = make_plan(h, cache, batch, per, a->max_tokens);
-    if (!workspace || workspace_bytes < plan.bytes || ((uintptr_t)workspace & 15u))
+    if (plan.items * p.c.heads * plan.parts > INT32_MAX) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 attention: more row blocks than one call counts");
+    if ((plan.bytes && !workspace) || workspace_bytes < plan.bytes || ((uintptr_t)workspace & 15u))
         OXQ_FAIL(h, OXQ_ERR_BUFFER_TOO_SMALL, "kv4 attention: workspace of %zu bytes (16-byte aligned), got %zu", plan.bytes, workspace ? workspace_bytes : (size_t)0);
     if (int32_t rc = oxq_require_sm100(h)) return rc;
     OxqDeviceGuard guard(h->device);

@@ -22,19 +22,19 @@ struct AttnParams {
     int32_t* status;
 };
 
-// Sequence b: its first query token, how many of its tokens are in the call's rows, how many it asks for (the positions
-// count from that), how many keys it has.  Offsets and lengths come from the device and are held to their arrays here.
-struct SeqInfo { int start, n, asked, len; };
+// Sequence b: its first query token, how many of its tokens are in the call's rows, the position before its first one's, and
+// how many keys the table can give.  Offsets and lengths come from the device and are held to their arrays here.
+struct SeqInfo { int start, n, before, len; };
 __device__ __forceinline__ SeqInfo seq_info(const AttnParams& p, int b) {
     SeqInfo q;
-    const int a = __ldg(p.s.cu + b), e = __ldg(p.s.cu + b + 1);
+    const int a = __ldg(p.s.cu + b), e = __ldg(p.s.cu + b + 1), len = max(__ldg(p.s.lens + b), 0);
+    const bool sound = a >= 0 && e >= a;
     q.start = a;
-    q.asked = max(e - a, 0);
-    q.n = a < 0 || a >= p.s.tokens ? 0 : min((int64_t)q.asked, p.s.tokens - a);
-    if (a < 0 || e < a) q.asked = 0, q.n = 0;
-    const int len = max(__ldg(p.s.lens + b), 0);
+    q.n = sound && a < p.s.tokens ? (int)min((int64_t)(e - a), p.s.tokens - a) : 0;
+    q.before = len - (sound ? e - a : 0);
     const int64_t most = p.s.width << p.c.page_shift;
     q.len = len > most ? (int)most : len;
+    if (len > most && q.n > 0) *p.status = OXQ_ERR_INVALID_ARGUMENT;
     return q;
 }
 

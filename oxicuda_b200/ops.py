@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import threading
 
 import torch
 
@@ -31,6 +32,7 @@ class Handle:
             stream = torch.cuda.current_stream().cuda_stream
             raise_for_status(self.lib.oxq_handle_create(self.device, C.c_void_p(stream), C.byref(self._h)))
         self._stream = stream
+        self._lock = threading.Lock()
 
     def close(self):
         if self._h:
@@ -51,10 +53,12 @@ class Handle:
             self._stream = s
 
     def call(self, name: str, *args):
-        self.sync_stream()
-        rc = getattr(self.lib, name)(self._h, *args)
+        with self._lock:                      # the stream is the handle's: threads that share it take turns from setting it to the launch
+            self.sync_stream()
+            rc = getattr(self.lib, name)(self._h, *args)
+            error = self.lib.oxq_last_error_string(self._h).decode() if rc else ""
         if rc:
-            raise_for_status(rc, self.lib.oxq_last_error_string(self._h).decode())
+            raise_for_status(rc, error)
 
     def device_status(self) -> int:
         v = C.c_int32(0)

@@ -512,6 +512,56 @@ def test_places_that_the_table_does_not_give():
     h.device_status()
 
 
+@pytest.mark.parametrize("new", [2, 40])
+def test_a_table_shorter_than_the_lengths(new):
+    """Keys behind the table are left out; the queries keep the positions that the lengths give them, with window and without."""
+    from oxicuda_b200 import ops
+    for window in (0, 30):
+        c = Case([100, 60], [new, new], 2, 128, 64, 16)
+        c.fill()
+        q = c.normal(c.tokens, 8, 128, dtype=torch.bfloat16)
+        short = c.table[:, :5].contiguous()             # 80 positions
+        out, lse = ops.kv4_attention(q, c.cache, short, c.lens, c.cu, window=window, want_lse=True)
+        assert ops.handle().device_status() == 15
+        drop = [torch.arange(200, device="cuda") >= 80 for _ in range(2)]
+        check(c, q, out, lse, 128 ** -0.5, True, window, drop)
+
+
+def test_workspace_and_threads():
+    """A given workspace of the stated size serves; a smaller one is refused; threads with streams of their own share the library's handle."""
+    import threading
+    from oxicuda_b200 import ops
+    from oxicuda_b200.errors import BlasError
+    c = Case([5000, 33], [1, 1], 2, 128, 64, 16)
+    c.fill()
+    qs = [c.normal(2, 8, 128, dtype=torch.bfloat16) for _ in range(4)]
+    want = [attend(c, q)[0] for q in qs]
+    n = ops.kv4_attention_workspace_bytes(c.cache, c.table, c.lens, c.cu, 2, 8, 1)
+    assert n > 0
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    assert torch.equal(attend(c, qs[0], workspace=ws)[0], want[0])
+    with pytest.raises(BlasError) as e:
+        attend(c, qs[0], workspace=ws[:-16])
+    assert e.value.variant == "BufferTooSmall"
+    torch.cuda.synchronize()
+    got = [[] for _ in qs]
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(30):
+                got[i].append(attend(c, qs[i])[0])
+        s.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for w, outs in zip(want, got):
+        assert len(outs) == 30 and all(torch.equal(o, w) for o in outs)
+
+
 def test_nothing_to_do():
     from oxicuda_b200 import ops
     c = Case([5], [0], 2, 64, 64, 16)
