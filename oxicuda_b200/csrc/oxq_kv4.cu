@@ -117,6 +117,13 @@ template <typename T, int W> __device__ __forceinline__ void group_range(const E
     }
 }
 
+// two f32 operations in one instruction
+__device__ __forceinline__ uint64_t pair(float x, float y) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ void split(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) { uint64_t r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+
 // Eight elements of a lane to a word of codes and, the same in all lanes of the group, its (s, m).
 template <typename T, int G> __device__ __forceinline__ void quantize8(const Eight<T>& x, uint32_t& codes, uint32_t& params) {
     float lo, hi, f[8];
@@ -144,13 +151,20 @@ template <typename T, int G> __device__ __forceinline__ void quantize8(const Eig
     const float range = hi - lo, fifteenth = 1.0f / 15.0f, s0 = range * fifteenth;
     const __half sh = __float2half_rn(fmaf(fmaf(-15.0f, s0, range), fifteenth, s0)), mh = __float2half_rn(lo);
     const float sc = __half2float(sh), m = __half2float(mh), y = __frcp_rn(sc);
-    float half[2] = {0.0f, 0.0f};
-    constexpr float kMagic = 12582912.0f, kPlace[4] = {1.0f, 16.0f, 256.0f, 4096.0f};
+    constexpr float kMagic = 12582912.0f;
+    const uint64_t m2 = pair(-m, -m), y2 = pair(y, y), s2 = pair(-sc, -sc), up = pair(kMagic, kMagic), down = pair(-kMagic, -kMagic);
+    uint64_t sum[2] = {0, 0};
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float d = f[e] - m, q0 = d * y, q = fminf(fmaxf(fmaf(fmaf(-sc, q0, d), y, q0), 0.0f), 15.0f);
-        half[e >> 2] = fmaf((q + kMagic) - kMagic, kPlace[e & 3], half[e >> 2]);
+    for (int e = 0; e < 8; e += 2) {
+        const uint64_t d = add2(pair(f[e], f[e + 1]), m2), q0 = mul2(d, y2);
+        float a, b;
+        split(fma2(fma2(s2, q0, d), y2, q0), a, b);
+        const uint64_t r = add2(add2(pair(fminf(fmaxf(a, 0.0f), 15.0f), fminf(fmaxf(b, 0.0f), 15.0f)), up), down);
+        sum[e >> 2] = fma2(r, e & 2 ? pair(256.0f, 4096.0f) : pair(1.0f, 16.0f), sum[e >> 2]);
     }
+    float half[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) { float a, b; split(sum[h], a, b); half[h] = a + b; }
     codes = (__float_as_uint(half[0] + 8388608.0f) & 0xFFFFu) | (__float_as_uint(half[1] + 8388608.0f) << 16);
     if (!(sc > 0.0f)) codes = 0;
     params = (uint32_t)__half_as_ushort(sh) | ((uint32_t)__half_as_ushort(mh) << 16);
@@ -320,21 +334,23 @@ int32_t oxq_kv4_check(oxq_handle* h, const oxq_kv4_cache* c, const oxq_kv4_batch
     return OXQ_OK;
 }
 
-// Tokens per warp: what leaves about 16 warps on every SM for keys and for values, at least a word for every lane, at most
-// eight (a read of 131k tokens: 125 us; with 32 a warp 150 us, for the last wave of CTAs is then long); whole fours, as four tokens' loads are in flight at once.  Where even a token
-// a warp leaves SMs without work -- a decode step -- up to eight warps share the token's words.
-static Walk walk_of(const oxq_handle* h, const Pool& c, const Batch& s, int dim, dim3* grid) {
+// Tokens per warp: what leaves about `warps` warps on every SM for keys and for values, at least a word for every lane, at most
+// eight (a read of 131k tokens: 125 us; with 32 a warp 150 us, for the last wave of CTAs is then long); a multiple of the tokens
+// whose loads are in flight at once.  Where even a token a warp leaves SMs without work -- a decode step -- up to eight warps
+// share the token's words.  Reading streams: 16 warps, four tokens at once.  Appending computes: 32 warps and two (8192 tokens
+// of 8 heads: 18.1 us; 16 and four 22.8, 64 and one 23.7).
+static Walk walk_of(const oxq_handle* h, const Pool& c, const Batch& s, int dim, int warps, int at_once, dim3* grid) {
     Walk w;
     const int words = c.heads * (dim / 8), least = (32 + words - 1) / words;
-    const int64_t each = s.tokens / ((int64_t)h->sm_count * 16);
+    const int64_t each = s.tokens / ((int64_t)h->sm_count * warps);
     w.each = (int)(each < least ? least : each > 8 && least <= 8 ? 8 : each > 32 ? 32 : each);
     w.beside = words < 32 ? 32 / words : 1;
     w.rounds = (words + 31) / 32;
     const int share = s.tokens < 8ll * h->sm_count ? (w.each + w.beside - 1) / w.beside * w.rounds : 1;
     w.share = share > 8 ? 8 : share;
     if (w.share == 1) {
-        const int four = 4 * w.beside;
-        w.each = w.each + four - 1 < 32 ? (w.each + four - 1) / four * four : 32;
+        const int whole = at_once * w.beside;
+        w.each = w.each + whole - 1 < 32 ? (w.each + whole - 1) / whole * whole : 32;
     }
     *grid = dim3((unsigned)(((s.tokens + w.each - 1) / w.each * w.share + 7) / 8), 2);
     return w;
@@ -343,15 +359,15 @@ static Walk walk_of(const oxq_handle* h, const Pool& c, const Batch& s, int dim,
 template <typename T, int D, int G>
 static cudaError_t launch_append(oxq_handle* h, const Pool& c, const Batch& s, const Rows<T>& in) {
     dim3 grid;
-    const Walk w = walk_of(h, c, s, D, &grid);
+    const Walk w = walk_of(h, c, s, D, 32, 2, &grid);
     if (w.share > 1) return oxq_launch(kv4_append_kernel<T, D, G, 1>, grid, 256, 0, h->stream, c, s, in, w, h->dev_status);
-    return oxq_launch(kv4_append_kernel<T, D, G, 4>, grid, 256, 0, h->stream, c, s, in, w, h->dev_status);
+    return oxq_launch(kv4_append_kernel<T, D, G, 2>, grid, 256, 0, h->stream, c, s, in, w, h->dev_status);
 }
 
 template <typename T, int D, int G>
 static cudaError_t launch_read(oxq_handle* h, const Pool& c, const Batch& s, void* k, void* v) {
     dim3 grid;
-    const Walk w = walk_of(h, c, s, D, &grid);
+    const Walk w = walk_of(h, c, s, D, 16, 4, &grid);
     if (w.share > 1) return oxq_launch(kv4_read_kernel<T, D, G, 1>, grid, 256, 0, h->stream, c, s, (T*)k, (T*)v, w, h->dev_status);
     return oxq_launch(kv4_read_kernel<T, D, G, 4>, grid, 256, 0, h->stream, c, s, (T*)k, (T*)v, w, h->dev_status);
 }
