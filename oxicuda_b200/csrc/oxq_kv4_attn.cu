@@ -29,7 +29,7 @@ namespace kv4 {
 
 constexpr int TILE = 128;               // keys per tile: 4 warps x 32
 constexpr int MIN_TILES = 2;            // tiles a CTA takes at least: a join of many small parts costs more than it brings
-constexpr int SETUP = 3;                // what an item costs besides its tiles, in tiles: 3.3 us against 1.2 us a tile, measured
+constexpr int SETUP = 6;                // what an item costs besides its tiles, in tiles (six ragged batches at 3, 4, 5, 6, 8: 79.1, 76.4, 76.9, 75.9, 77.2 us for the first)
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -688,7 +688,9 @@ static int32_t launch_dims(oxq_handle* h, const oxq_kv4_cache* cc, const AttnPar
 
 // Which kernels a call needs.  Up to ROWS_MOST query rows per sequence and kv head go to the kernel above, more to the tiles of
 // oxq_kv4_tiles.cu.  A batch may hold both kinds, and only the device knows its sequences, so with more than one both kernels
-// are launched and each takes its own; a single sequence goes whole to the one that its bound asks for.
+// are launched and each takes its own; a single sequence goes whole to the one that its bound asks for, and so does a batch
+// whose sequences must all be as long as the longest, by the number of tokens (3 x 1000 tokens: 218 us with the second kernel, 211
+// without).
 constexpr int64_t ROWS_MOST = 64;
 struct Plan {
     int nt;                             // blocks of 8 or 16 query rows: 16 where a sequence has more than 8, because the codes are unpacked once for all of them
@@ -701,12 +703,13 @@ static Plan make_plan(const oxq_handle* h, const oxq_kv4_cache* cc, const oxq_kv
     const int64_t all_rows = s->tokens * per, max_rows = (max_tokens > 0 && max_tokens < s->tokens ? max_tokens : s->tokens) * per;
     f.nt = max_rows <= 8 ? 1 : 2;
     f.tiles = max_rows > ROWS_MOST;
-    f.rows = !f.tiles || s->seqs > 1;
+    const bool alike = s->seqs == 1 || (max_tokens > 0 && s->tokens / max_tokens >= s->seqs);
+    f.rows = !f.tiles || !alike;
     f.rows_bytes = f.rows ? (size_t)attn_ctas(h, f.nt) * 2 * (f.nt == 1 ? Slot<1>::floats(cc->dim) : Slot<2>::floats(cc->dim)) * sizeof(float) + attn_ctas(h, f.nt) * sizeof(Cut) : 0;
     f.items = 0; f.parts = 1;
     if (f.tiles) {
         const int64_t with = all_rows / (ROWS_MOST + 1) < s->seqs ? all_rows / (ROWS_MOST + 1) : s->seqs;
-        f.items = s->seqs == 1 ? (all_rows + 255) / 256 : all_rows / 256 + with;
+        f.items = s->seqs == 1 ? (all_rows + 255) / 256 : all_rows / 256 + (f.rows ? with : s->seqs);
         // too few CTAs for the machine: several share an item's keys (at least four tiles each of the longest the table allows)
         const int64_t ctas = f.items * cc->heads, most = s->table_width * cc->page_size / (4 * TILE);
         int64_t parts = ctas * 2 <= h->sm_count ? h->sm_count / ctas : 1;

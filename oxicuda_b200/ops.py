@@ -656,7 +656,7 @@ def _residual_norm_args(y, residual, weight, post_weight, gate, alpha, eps, resi
         gate_ptr = gate.data_ptr()
     r_ld = _row_stride(residual, shape)
     if residual_out is None:
-        residual_out, ro_ld = residual.new_empty(shape), cols
+        residual_out, ro_ld = torch.empty_like(residual) if r_ld == cols else residual.new_empty(shape), cols
     else:
         if residual_out.shape != shape or residual_out.dtype != residual.dtype or residual_out.get_device() != index:
             raise QuantError("DimensionMismatch", f"residual_out {tuple(residual_out.shape)} {residual_out.dtype} for {tuple(shape)} {residual.dtype} on {y.device}", 4)
@@ -672,7 +672,7 @@ def residual_rmsnorm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
     residual_out may be residual itself.  y, residual, residual_out and gate may be row-strided views."""
     r_out, args = _residual_norm_args(y, residual, weight, post_weight, gate, alpha, eps, residual_out)
     if out is None:
-        out = y.new_empty(y.shape)
+        out = torch.empty_like(y) if y.is_contiguous() else y.new_empty(y.shape)
     else:
         _chk(out, y.dtype)
         if out.shape != y.shape or out.device != y.device:
@@ -843,7 +843,7 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, block_table: torch.Tensor, s
     tokens, heads = shape[0], shape[1]
     qt, qh = _kv4_rows(q, heads, cache, "q", _HALVES)
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
         ot, oh = heads * cache.dim, cache.dim
     else:
         ot, oh = _kv4_rows(out, heads, cache, "out", (q.dtype,))

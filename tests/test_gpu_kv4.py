@@ -364,6 +364,16 @@ def test_a_mixed_batch():
         check(c, q, out, lse, 128 ** -0.5, True, 0)
 
 
+def test_a_batch_that_looks_alike():
+    """As many tokens as sequences times the longest run: all go to one kernel, whatever the offsets then say."""
+    for new in ([40, 40, 40], [118, 1, 1], [0, 119, 1]):
+        c = Case([300, 119, 77], new, 2, 128, 64, 32)
+        c.fill()
+        q = c.normal(c.tokens, 8, 128, dtype=torch.bfloat16)
+        out, lse = attend(c, q, max_tokens=40)
+        check(c, q, out, lse, 128 ** -0.5, True, 0)
+
+
 @pytest.mark.parametrize("heads,per,lens,new", [(1, 4, [9000], [20]), (2, 4, [5000, 3000], [80, 40]), (1, 1, [20000], [100])])
 @pytest.mark.parametrize("dim,group", DIMS)
 def test_few_blocks_share_their_keys(heads, per, lens, new, dim, group):
