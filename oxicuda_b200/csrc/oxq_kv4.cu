@@ -5,6 +5,9 @@
 // The codes are computed from the rounded s and m, the numbers the reader uses, so rounding them costs no accuracy in the
 // codes.  s and m stay f16 (4 bytes a group): the offset is a float, not a zero-point in code units, because a group whose
 // values all lie on one side of zero must keep its four bits for its own range.
+//
+// What bounds them: appending, the quantizer's instructions (8192 tokens of 8 heads, keys and values: 18 us, the
+// bytes need 6.6); reading, memory (131k tokens: 125 us = 5.6 TB/s, 0.86 of the copy rate).
 #include "oxq_kv4.cuh"
 
 namespace oxq {

@@ -7,10 +7,11 @@
 // the codes; the offsets' sum is kept beside it in f32.  A code is used as the f16 number with those bits, the subnormal
 // c * 2^-24 (16 c * 2^-24 for a nibble that is left where it lies): one AND per two codes, exact, and the power of two is
 // taken out again in f32.  q enters as f16 scaled per row by a power of two, so that the row's largest element lies in
-// [2^11, 2^12): exact for f16 and bf16 values down to 2^-25 of the row's largest.
+// [2^11, 2^12): exact, but for elements below 2^-21 of the row's largest, which are off by at most 2^-32 of it.
 // The running reference M of a row is the maximum over its keys of x + log2(largest s of the value rows of the key and of
-// its three companions 8, 16 and 24 places apart, rounded down, at least -15), so that w stays in f16's range whatever the scales are; it moves only when a key exceeds it by 2^8 (w <= 2^9),
-// which one vote per 32 keys finds out.  l = sum p, the offsets' sum and all accumulators are f32.
+// its three companions 8, 16 and 24 places apart, rounded down, at least -15), so that w stays in f16's range whatever the
+// scales are; it moves only when a key exceeds it by 2^8 (w <= 2^9), which one vote per 32 keys finds out.  l = sum p, the
+// offsets' sum and all accumulators are f32.  bf16 outputs take w rounded once to f16 (2^-11, an eighth of their own step).
 // f16 outputs are finer than one f16 rounding of w; for them w is split into two f16 terms (two products).
 //
 // The shape.  mma.sync m16n8k16 with the keys as the 16 rows and 8 query rows as the columns (a kv head's query heads, and
@@ -21,6 +22,10 @@
 // CTAs cut into equal parts (lengths are known on the device only).  An item that lies inside one part is finished there; of a
 // cut one every CTA leaves o, M and l in the workspace and a second kernel joins them, in the order of the keys, so
 // results do not depend on timing.
+//
+// What bounds it: about 300 instructions per 16 keys at 16 warps on an SM, half of them on the logic pipe, which issues at
+// half rate (32 sequences of 50 to 16000 keys, 8 kv heads of 128: 76 us, the tiles alone stream in 56, their bytes need 47;
+// 4 x 131072 keys: 110, 87, 80).  A single short call is latency: 3.5 us to find the work, 2 to the first tiles, 4 for the join.
 #include "oxq_kv4_attn.cuh"
 #include "oxq_tc.cuh"
 
