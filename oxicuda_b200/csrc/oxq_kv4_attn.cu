@@ -757,7 +757,17 @@ int32_t oxq_kv4_attention(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_k
     if (!a->q || !a->out) OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: null queries or output");
     if (a->q_token_stride < 0 || a->q_head_stride < 0 || a->out_token_stride < 0 || a->out_head_stride < 0)
         OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: negative stride");
-    if (((uintptr_t)a->out | (uintptr_t)(a->out_token_stride * 2) | (uintptr_t)(a->out_head_stride * 2)) & 3u)
+    // the strides of a single token or head are never used
+    const int64_t q_ts = p.s.tokens > 1 ? a->q_token_stride : 0, q_hs = a->q_heads > 1 ? a->q_head_stride : 0;
+    const int64_t o_ts = p.s.tokens > 1 ? a->out_token_stride : 0, o_hs = a->q_heads > 1 ? a->out_head_stride : 0;
+    // output rows that lie over one another would be written by several CTAs at once: the far stride has to pass all near rows
+    const bool heads_near = p.s.tokens == 1 || (a->q_heads > 1 && o_hs <= o_ts);
+    const int64_t near_rows = heads_near ? a->q_heads : p.s.tokens, near_stride = heads_near ? o_hs : o_ts;
+    const int64_t far_rows = heads_near ? p.s.tokens : a->q_heads, far_stride = heads_near ? o_ts : o_hs;
+    if ((near_rows > 1 && near_stride < cache->dim) ||
+        (far_rows > 1 && (far_stride < cache->dim || (near_rows > 1 && (far_stride - cache->dim) / (near_rows - 1) < near_stride))))
+        OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: output rows overlap");
+    if (((uintptr_t)a->out | (uintptr_t)(o_ts * 2) | (uintptr_t)(o_hs * 2)) & 3u)
         OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: output rows must be 4-byte aligned");
     const int64_t per = a->q_heads / p.c.heads;
     if (p.s.tokens * per > INT32_MAX / 2) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 attention: too many query rows");
@@ -767,15 +777,15 @@ int32_t oxq_kv4_attention(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_k
         OXQ_FAIL(h, OXQ_ERR_BUFFER_TOO_SMALL, "kv4 attention: workspace of %zu bytes (16-byte aligned), got %zu", plan.bytes, workspace ? workspace_bytes : (size_t)0);
     if (int32_t rc = oxq_require_sm100(h)) return rc;
     OxqDeviceGuard guard(h->device);
-    p.q = a->q; p.q_ts = a->q_token_stride; p.q_hs = a->q_head_stride;
-    p.q_vec = (((uintptr_t)a->q | (uintptr_t)(a->q_token_stride * 2) | (uintptr_t)(a->q_head_stride * 2)) & 15u) == 0;
-    p.out = a->out; p.o_ts = a->out_token_stride; p.o_hs = a->out_head_stride; p.lse = a->lse;
+    p.q = a->q; p.q_ts = q_ts; p.q_hs = q_hs;
+    p.q_vec = (((uintptr_t)a->q | (uintptr_t)(q_ts * 2) | (uintptr_t)(q_hs * 2)) & 15u) == 0;
+    p.out = a->out; p.o_ts = o_ts; p.o_hs = o_hs; p.lse = a->lse;
     p.by_per.set((int)per);
     p.per = (int)per; p.q_heads = (int)a->q_heads;
     p.scale_log2 = a->scale * 1.44269504088896340736f;
     p.causal = a->causal ? 1 : 0;
     p.window = a->window > INT32_MAX ? INT32_MAX : (int)a->window;
-    p.out_vec = (((uintptr_t)a->out | (uintptr_t)(a->out_token_stride * 2) | (uintptr_t)(a->out_head_stride * 2)) & 15u) == 0;
+    p.out_vec = (((uintptr_t)a->out | (uintptr_t)(o_ts * 2) | (uintptr_t)(o_hs * 2)) & 15u) == 0;
     p.status = h->dev_status;
     // the most tiles that there can be for the row kernel: every row block of every sequence over a whole table row
     const int nt = plan.nt;

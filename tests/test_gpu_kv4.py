@@ -487,6 +487,26 @@ def test_strided_queries_and_outputs():
     check(c, q, out, lse, 128 ** -0.5, True, 0)
 
 
+def test_one_token_whose_stride_means_nothing():
+    c = Case([100], [1], 2, 128, 128, 16)
+    c.fill()
+    q = torch.as_strided(c.normal(8 * 128, dtype=torch.bfloat16), (1, 8, 128), (1, 128, 1))
+    home = torch.zeros(8 * 128, dtype=torch.bfloat16, device="cuda")
+    out, lse = attend(c, q, out=torch.as_strided(home, (1, 8, 128), (3, 128, 1)))
+    check(c, q, out, lse, 128 ** -0.5, True, 0)
+
+
+@pytest.mark.parametrize("shape,strides", [((4, 8, 128), (0, 128, 1)), ((4, 8, 128), (1024, 0, 1)), ((4, 8, 128), (1022, 128, 1)), ((4, 8, 128), (128, 510, 1))])
+def test_outputs_whose_rows_overlap_are_refused(shape, strides):
+    from oxicuda_b200.errors import BlasError
+    c = Case([100], [4], 2, 128, 128, 16)
+    c.fill()
+    home = torch.zeros(8 * 1024, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(BlasError, match="overlap"):
+        attend(c, c.normal(*shape, dtype=torch.bfloat16), out=torch.as_strided(home, shape, strides))
+    assert (home == 0).all()
+
+
 def test_places_that_the_table_does_not_give():
     """A page number outside the pool and a position behind the table are left out, never followed, and reported once."""
     from oxicuda_b200 import ops

@@ -85,6 +85,21 @@ def test_attention(lib, fake, key, value, status):
     assert lib.oxq_kv4_attention(fake, c, b, a, 0x10000, 1 << 30) == status
 
 
+@pytest.mark.parametrize("tokens,heads,strides,status", [
+    (3, 8, (1024, 128), 13), (3, 8, (128, 384), 13), (3, 8, (1152, 132), 13),     # rows apart, in either order
+    (3, 8, (0, 128), 15), (3, 8, (1024, 0), 15), (3, 8, (1024, 64), 15), (3, 8, (1022, 128), 15), (3, 8, (128, 382), 15), (3, 8, (128, 128), 15),
+    (1, 8, (1, 128), 13), (1, 8, (0, 128), 13), (1, 8, (1024, 64), 15), (3, 2, (256, 128), 13), (3, 2, (254, 128), 15), (3, 2, ((1 << 62), 128), 13),
+    (3, 2, (128, 1 << 62), 13), (1, 2, (0, 126), 15)])
+def test_output_rows_that_overlap(lib, fake, tokens, heads, strides, status):
+    c, b, a = _descs(tokens=tokens, q_heads=heads, out_token_stride=strides[0], out_head_stride=strides[1])
+    assert lib.oxq_kv4_attention(fake, c, b, a, 0x10000, 1 << 30) == status
+
+
+def test_the_strides_of_one_token_and_one_head_are_not_looked_at(lib, fake):
+    c, b, a = _descs(tokens=1, heads=1, q_heads=1, q_token_stride=7, q_head_stride=5, out_token_stride=3, out_head_stride=1)
+    assert lib.oxq_kv4_attention(fake, c, b, a, 0x10000, 1 << 30) == OK_BUT_NO_DEVICE
+
+
 def test_attention_window_and_workspace(lib, fake):
     c, b, a = _descs(window=4, causal=0)
     assert lib.oxq_kv4_attention(fake, c, b, a, 0x10000, 1 << 30) == 15
