@@ -5,8 +5,12 @@
 // so the product runs on the codes themselves and scale and offset are applied to its result in f32: the keys are never
 // rounded.  Likewise o = sum p v^ = sum (p s) c + sum p m: the second product's left factor is w = p s, its right factor
 // the codes; the offsets' sum is kept beside it in f32.  A code is used as the f16 number with those bits, the subnormal
-// c * 2^-24 (16 c * 2^-24 for a nibble that is left where it lies): one AND per two codes, exact, and the power of two is
-// taken out again in f32.  q enters as f16 scaled per row by a power of two, so that the row's largest element lies in
+// c * 2^-24 (16 c * 2^-24 for a nibble four bits up): one AND per two codes, exact, and the power of two is taken out again
+// in f32.  The matrix instruction lines products up by the operands' exponent fields, where a subnormal has the least normal
+// one, and cuts them 2^-25 below that: the higher a code lies in the mantissa, the more of the other factor's bits are kept.
+// So the keys' codes lie two bits up, 4 c * 2^-24 and 64 c * 2^-24: one shift a word more (1.4% of the large calls), and the
+// log-sum-exp is off by 2e-7 of itself in place of 1.3e-6 (f16 queries, 4 keys; an f32 product of unpacked keys: 1.3e-7).
+// The values' lie so for f16 outputs only; bf16's own step hides what is cut.  q enters as f16 scaled per row by a power of two, so that the row's largest element lies in
 // [2^11, 2^12): exact, but for elements below 2^-21 of the row's largest, which are off by at most 2^-32 of it.
 // The running reference M of a row is the maximum over its keys of x + log2(largest s of the value rows of the key and of
 // its three companions 8, 16 and 24 places apart, rounded down, at least -15), so that w stays in f16's range whatever the
@@ -24,8 +28,8 @@
 // results do not depend on timing.
 //
 // What bounds it: about 300 instructions per 16 keys at 16 warps on an SM, half of them on the logic pipe, which issues at
-// half rate (32 sequences of 50 to 16000 keys, 8 kv heads of 128: 76 us, the tiles alone stream in 56, their bytes need 47;
-// 4 x 131072 keys: 110, 87, 80).  A single short call is latency: 3.5 us to find the work, 2 to the first tiles, 4 for the join.
+// half rate (32 sequences of 50 to 16000 keys, 8 kv heads of 128: 77 us, the tiles alone stream in 56, their bytes need 47;
+// 4 x 131072 keys: 111, 87, 80).  A single short call is latency: 3.5 us to find the work, 2 to the first tiles, 4 for the join.
 #include "oxq_kv4_attn.cuh"
 #include "oxq_tc.cuh"
 
@@ -200,7 +204,7 @@ struct Smem {
     unsigned char ring[STAGES][Stage<D, NG>::BYTES];
     __half q[ROWS * QPAD];              // per eight elements in the order 0 4 1 5 2 6 3 7, the odd ones / 16
     float slab[4][ROWS * (D + 8)];
-    float a[ROWS], bsum[ROWS][NG];      // scale log2(e) 2^(24 + e - 11), scale log2(e) * sum of q
+    float a[ROWS], bsum[ROWS][NG];      // scale log2(e) 2^(22 + e - 11), scale log2(e) * sum of q
     float m[8][ROWS], l[8][ROWS];
     uint64_t bars[2 * STAGES];
     unsigned char there[STAGES][8];
@@ -331,7 +335,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
             o.x = pack_f16(f[0] * up, f[4] * up); o.y = pack_f16(f[1] * up * 0.0625f, f[5] * up * 0.0625f);
             o.z = pack_f16(f[2] * up, f[6] * up); o.w = pack_f16(f[3] * up * 0.0625f, f[7] * up * 0.0625f);
             *reinterpret_cast<uint4*>(&sm.q[row * QPAD + g * 8]) = o;
-            if (g == 0) sm.a[row] = p.scale_log2 * pow2_of(min(24 - 11 + ex, 127));
+            if (g == 0) sm.a[row] = p.scale_log2 * pow2_of(min(22 - 11 + ex, 127));
             if (g % (D / 8 / NG) == 0) sm.bsum[row][g / (D / 8 / NG)] = p.scale_log2 * sum;
         }
         if (tid == 0) sm.work[turn] = wk;
@@ -392,12 +396,12 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
 #pragma unroll
                         for (int i2 = 0; i2 < NB / NG; i2++) {
                             const int blk = g * (NB / NG) + i2;
-                            const uint32_t w0 = k[0][blk], w1 = k[1][blk], u0 = w0 >> 8, u1 = w1 >> 8;
+                            const uint32_t w0 = k[0][blk] << 2, w1 = k[1][blk] << 2, u0 = k[0][blk] >> 6, u1 = k[1][blk] >> 6;
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
                                 const uint4 qf = *reinterpret_cast<const uint4*>(&sm.q[(nt * 8 + r) * QPAD + blk * 32 + c * 8]);
-                                mma_16816(s4[nt], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf.x, qf.y);
-                                mma_16816(s4[nt], u0 & 0x000F000Fu, u1 & 0x000F000Fu, u0 & 0x00F000F0u, u1 & 0x00F000F0u, qf.z, qf.w);
+                                mma_16816(s4[nt], w0 & 0x003C003Cu, w1 & 0x003C003Cu, w0 & 0x03C003C0u, w1 & 0x03C003C0u, qf.x, qf.y);
+                                mma_16816(s4[nt], u0 & 0x003C003Cu, u1 & 0x003C003Cu, u0 & 0x03C003C0u, u1 & 0x03C003C0u, qf.z, qf.w);
                             }
                         }
 #pragma unroll
@@ -489,7 +493,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                         }
                     }
                 }
-                // ---- O^T: rows r and r + 8 of block (s, j) are elements 64 s + 8 r + 2 j and + 1, the second one times 16
+                // ---- O^T: rows r and r + 8 of block (s, j) are elements 64 s + 8 r + 2 j and + 1, the second one times 16 (or the first, where the values are two bits down)
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     uint32_t v[4][NS];
@@ -501,8 +505,10 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                         for (int j = 0; j < 4; j++) {
                             constexpr uint32_t kSel[4] = {0x4400u, 0x5511u, 0x6622u, 0x7733u};
                             const int g = NG == 1 ? 0 : s;
-                            const uint32_t b0 = __byte_perm(v[0][s], v[1][s], kSel[j]), b1 = __byte_perm(v[2][s], v[3][s], kSel[j]);
-                            const uint32_t a0 = b0 & 0x000F000Fu, a1 = b0 & 0x00F000F0u, a2 = b1 & 0x000F000Fu, a3 = b1 & 0x00F000F0u;
+                            // every byte is there twice in its half; two bits down, its low nibble lies at the top of the mantissa
+                            constexpr uint32_t kLow = SPLIT ? 0x03C003C0u : 0x000F000Fu, kHigh = SPLIT ? 0x003C003Cu : 0x00F000F0u;
+                            const uint32_t b0 = __byte_perm(v[0][s], v[1][s], kSel[j]) >> (SPLIT ? 2 : 0), b1 = __byte_perm(v[2][s], v[3][s], kSel[j]) >> (SPLIT ? 2 : 0);
+                            const uint32_t a0 = b0 & kLow, a1 = b0 & kHigh, a2 = b1 & kLow, a3 = b1 & kHigh;
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
                                 mma_16816(acc[s * 4 + j][nt], a0, a1, a2, a3, wb[nt][g][2 * u], wb[nt][g][2 * u + 1]);
@@ -567,8 +573,8 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                             for (int j = 0; j < 4; j++) {
                                 float2& at = *reinterpret_cast<float2*>(&sm.slab[warp & 3][row * OPAD + 64 * s + 8 * r + 2 * j]);
                                 float2 o;
-                                o.x = fmaf(acc[s * 4 + j][nt][e] * 0x1p24f, f, off);
-                                o.y = fmaf(acc[s * 4 + j][nt][e + 2] * 0x1p20f, f, off);
+                                o.x = fmaf(acc[s * 4 + j][nt][e] * (SPLIT ? 0x1p18f : 0x1p24f), f, off);
+                                o.y = fmaf(acc[s * 4 + j][nt][e + 2] * (SPLIT ? 0x1p22f : 0x1p20f), f, off);
                                 if (half) { o.x += at.x; o.y += at.y; }
                                 at = o;
                             }

@@ -487,6 +487,32 @@ def test_strided_queries_and_outputs():
     check(c, q, out, lse, 128 ** -0.5, True, 0)
 
 
+@pytest.mark.parametrize("dim,group", DIMS)
+def test_log_sum_exp_of_few_keys(dim, group):
+    """The products are cut, not rounded, where the tensor core lines them up; what that costs stays below two f32 roundings of the terms' sum
+    X = sum of |scale q| (15 s + |m|), each 2^-24 X / sqrt(12) in the root mean square at most: together below 2^-25 X."""
+    c = Case([1 + i % 5 for i in range(60)], [1] * 60, 8, dim, group, 16)
+    c.fill()
+    q = c.normal(c.tokens, 24, dim, dtype=torch.float16)
+    _, lse = attend(c, q)
+    _, ref, _, _, x = reference(c, q, dim ** -0.5, True, 0)
+    rms = lambda t: t.double().square().mean().sqrt()  # noqa: E731
+    assert rms(lse.double() - ref) <= 2.0 ** -25 * rms(x)
+
+
+@pytest.mark.parametrize("dim,group", DIMS)
+def test_f16_outputs_are_off_by_their_own_rounding(dim, group):
+    """Scores of standard deviation 2.5: most weights are far below the largest.  w is good to 2^-21 and the rest is f32, so the error is that of
+    the final rounding to f16 (a tenth is left for all else)."""
+    c = Case([3000, 700], [4, 4], 3, dim, group, 16)
+    c.fill()
+    q = (c.normal(c.tokens, 6, dim) * 2.5).to(torch.float16)
+    out, _ = attend(c, q)
+    ref = reference(c, q, dim ** -0.5, True, 0)[0]
+    rms = lambda t: t.double().square().mean().sqrt()  # noqa: E731
+    assert rms(out.double() - ref) <= 1.1 * rms(ref.to(torch.float16).double() - ref)
+
+
 def test_one_token_whose_stride_means_nothing():
     c = Case([100], [1], 2, 128, 128, 16)
     c.fill()
