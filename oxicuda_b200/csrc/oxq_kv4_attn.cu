@@ -723,7 +723,7 @@ static Plan make_plan(const oxq_handle* h, const oxq_kv4_cache* cc, const oxq_kv
         f.items = s->seqs == 1 ? (all_rows + 255) / 256 : all_rows / 256 + (f.rows ? with : s->seqs);
         // too few CTAs for the machine: several share an item's keys (at least four tiles each of the longest the table allows)
         const int64_t ctas = f.items * cc->heads, most = s->table_width * cc->page_size / (4 * TILE);
-        int64_t parts = ctas * 2 <= h->sm_count ? h->sm_count / ctas : 1;
+        int64_t parts = ctas > 0 && ctas * 2 <= h->sm_count ? h->sm_count / ctas : 1;
         if (parts > most) parts = most;
         if (parts > 16) parts = 16;
         f.parts = parts < 1 ? 1 : (int)parts;
@@ -742,7 +742,7 @@ int32_t oxq_kv4_attention_workspace_bytes(oxq_handle* h, const oxq_kv4_cache* ca
     if (!bytes_out) OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "null size");
     if (q_heads <= 0 || q_heads % c.heads != 0) OXQ_FAIL(h, OXQ_ERR_DIMENSION_MISMATCH, "kv4 attention: %lld query heads over %d kv heads", (long long)q_heads, c.heads);
     if (max_tokens < 0) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 attention: negative max_tokens");
-    *bytes_out = make_plan(h, cache, batch, q_heads / c.heads, max_tokens).bytes;
+    *bytes_out = s.tokens == 0 || s.seqs == 0 ? 0 : make_plan(h, cache, batch, q_heads / c.heads, max_tokens).bytes;       // such a call does nothing
     return OXQ_OK;
 }
 

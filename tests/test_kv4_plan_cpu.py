@@ -1,0 +1,35 @@
+"""CPU tests of the sizes that attention over the 4-bit cache asks for.  A handle is faked as zeroed memory: a machine of no SMs."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+ROWS = [1, 64, 65, 127, 128, 255, 256, 300, 70000]
+
+# in a process of its own: a division by zero on the host would end this one
+CHILD = """
+import ctypes as C
+from oxicuda_b200 import _ffi
+lib, fake, n = _ffi.load(), C.create_string_buffer(4096), C.c_size_t(0)
+cache = _ffi.kv4_cache(0x1000, 0x2000, 0x3000, 0x4000, 8, 16, 2, 128, 64)
+for tokens in %r:
+    for most in (0, 1, 20, tokens):
+        for width in (0, 4, 4096):
+            n.value = 7
+            batch = _ffi.kv4_batch(0x5000, width, 0x6000, 0x7000, %d, tokens)
+            assert lib.oxq_kv4_attention_workspace_bytes(fake, cache, batch, 2, most, C.byref(n)) == 0
+            if %d == 0 or tokens == 0:
+                assert n.value == 0
+print("done")
+"""
+
+
+@pytest.mark.parametrize("seqs", [0, 1, 3])
+def test_workspace_of_any_number_of_sequences(seqs):
+    """A call without sequences (or without tokens) needs no workspace, however many query rows it has."""
+    from oxicuda_b200 import _build
+    _build.build()
+    r = subprocess.run([sys.executable, "-c", CHILD % ([0] + ROWS, seqs, seqs)], capture_output=True, text=True, cwd=ROOT)
+    assert r.returncode == 0 and r.stdout.strip() == "done", (r.returncode, r.stderr[-2000:])
