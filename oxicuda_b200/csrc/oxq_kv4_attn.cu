@@ -415,11 +415,12 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                     }
                 }
                 if (t0 < all_lo || t0 + 32 > all_hi || there != 0x0101u) {
+                    const int lo = *reinterpret_cast<volatile int*>(&sm.work[turn].it.span.lo);        // the first key that the block sees; kept out of registers
 #pragma unroll
                     for (int h = 0; h < 4; h++) {
                         const int t = t0 + r + 8 * h;
-                        const bool have = t < len && (there >> (8 * (h >> 1)) & 1u);
-                        if (!have)                                    // places behind the last key, and absent ones, hold anything
+                        const bool have = t < len && t >= lo && (there >> (8 * (h >> 1)) & 1u);
+                        if (!have)                                    // places behind the last key, in front of the first one seen, and absent ones, hold anything
 #pragma unroll
                             for (int g = 0; g < NG; g++) vp[h][g] = 0;
 #pragma unroll

@@ -114,8 +114,9 @@ __device__ __forceinline__ bool find_pair(const AttnParams& p, int want, TileIte
     return false;
 }
 
-// What the rows row0 .. of an item see together: tiles [first, first + n), this CTA's part of them.
-struct Walk { int first, n; };
+// What the rows row0 .. of an item see together: positions [lo, hi), and this CTA's part of the tiles that hold them,
+// [first, first + n).  Places outside [lo, hi) are not looked at: pages in front of a window may have been given back.
+struct Walk { int first, n, lo, hi; };
 __device__ __forceinline__ Walk walk_of(const AttnParams& p, const SeqInfo& q, int pair, int part) {
     const int row0 = pair * 2 * BLOCK;
     const int j0 = p.by_per.div(row0), j1 = p.by_per.div(min(row0 + 2 * BLOCK, q.n * p.per) - 1);
@@ -123,7 +124,7 @@ __device__ __forceinline__ Walk walk_of(const AttnParams& p, const SeqInfo& q, i
     const int lo = min(hi, p.window > 0 ? max(0, q.before + j0 + 1 - p.window) : 0);
     const int first = lo / BLOCK, all = (hi + BLOCK - 1) / BLOCK - first;
     const int a = (int)((int64_t)all * part / p.parts), e = (int)((int64_t)all * (part + 1) / p.parts);
-    return {first + a, e - a};
+    return {first + a, e - a, lo, hi};
 }
 
 template <typename T, int D, int NG>
@@ -360,12 +361,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
         uint4 kraw[ROUNDS], vraw[ROUNDS];
         uint32_t kpar[ROUNDS][NG], vpar[ROUNDS][NG];
         int page[ROUNDS];
-        bool gone[ROUNDS];                                          // a key without a page of the pool; one behind the end is masked by its position
+        bool gone[ROUNDS];                                          // a key without a page of the pool; those that no row sees are masked by their positions
+        const auto wanted = [&](int i, int key) { return i < n && key >= walk.lo && key < walk.hi; };
         const auto get_pages = [&](int i) {
 #pragma unroll
             for (int u = 0; u < ROUNDS; u++) {
                 const int key = (walk.first + i) * BLOCK + tok0 + u * PER_ROUND;
-                page[u] = i < n && key < q.len ? __ldg(table + (key >> p.c.page_shift)) : -1;
+                page[u] = wanted(i, key) ? __ldg(table + (key >> p.c.page_shift)) : -1;
             }
         };
         const auto load = [&](int i, const uint8_t* codes, const uint32_t* params, uint4 (&raw)[ROUNDS], uint32_t (&par)[ROUNDS][NG], bool keys) {
@@ -375,7 +377,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
                 raw[u] = make_uint4(0, 0, 0, 0);
 #pragma unroll
                 for (int g = 0; g < NG; g++) par[u][g] = 0;
-                const bool inside = i < n && key < q.len, good = inside && page[u] >= 0 && page[u] < p.c.pages;
+                const bool inside = wanted(i, key), good = inside && page[u] >= 0 && page[u] < p.c.pages;
                 if (keys) {
                     gone[u] = inside && !good;
                     if (gone[u] && piece == 0) *p.status = OXQ_ERR_INVALID_ARGUMENT;
