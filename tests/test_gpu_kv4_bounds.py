@@ -1,0 +1,50 @@
+"""GPU tests of attention over the 4-bit cache against what its roundings may be off by, row by row and all rows together."""
+import pytest
+import torch
+
+from kv4_bounds import Expected, rows_of
+from test_gpu_kv4 import DIMS, DT, Case, attend
+from test_kv4_bounds_cpu import SHAPES
+
+pytestmark = pytest.mark.gpu
+
+
+def held(c, q, scale, causal, window, max_tokens=None):
+    out, lse = attend(c, q, scale=scale, causal=causal, window=window, max_tokens=max_tokens)
+    worst = Expected(rows_of(c), c.new_l, q, scale, causal, window, max_tokens=max_tokens).worst(out, lse)
+    assert worst <= 1, f"{worst:.3f} of the bound"
+
+
+@pytest.mark.parametrize("dim,group", DIMS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("per,lens,new,causal,window", SHAPES)
+def test_rows_are_off_by_their_roundings(dim, group, dtype, per, lens, new, causal, window):
+    c = Case(lens, new, 2, dim, group, 32, seed=per + len(lens))
+    c.fill()
+    q = c.normal(c.tokens, 2 * per, dim, dtype=DT[dtype])
+    held(c, q, dim ** -0.5, causal, window)
+
+
+@pytest.mark.parametrize("max_tokens", [0, 1, 40, 200])
+def test_mixed_batches_are_off_by_their_roundings(max_tokens):
+    new = [1, 200, 0, 3, 16, 17, 1, 90]
+    c = Case([900, 200, 50, 3, 1000, 400, 1, 2000], new, 2, 128, 64, 32)
+    c.fill()
+    held(c, c.normal(c.tokens, 8, 128, dtype=torch.bfloat16), 128 ** -0.5, True, 0, max_tokens)
+
+
+@pytest.mark.parametrize("dim,group", DIMS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("per,lens,new,window", [(1, [300, 77], [5, 1], 0), (4, [300, 77], [5, 2], 50), (4, [500], [300], 0), (4, [500, 130], [300, 20], 129), (2, [900], [128], 128)])
+def test_the_edges_of_the_mask(dim, group, dtype, per, lens, new, window):
+    """Scores that rise by 8 from key to key: a row's output is the last value that it sees, and a row that saw one key more or less would give
+    another one.  Falling ones: the first value that it sees, which is the window's edge."""
+    for falling in (False, True):
+        c = Case(lens, new, 2, dim, group, 16, seed=dim)
+        c.fill()
+        for b, n in enumerate(lens):
+            at = torch.arange(n, device="cuda")
+            pg, sl = c.place(b, at)
+            c.cache.k_params[pg, :, sl] = torch.stack([torch.zeros_like(at), -at if falling else at], -1).half()[:, None, None]
+        q = torch.ones(c.tokens, 2 * per, dim, dtype=DT[dtype], device="cuda")
+        held(c, q, 8 / dim, True, window)
