@@ -495,7 +495,8 @@ OXQ_API int32_t oxq_residual_rmsnorm_int8_rows(oxq_handle* h, const oxq_residual
  *                 ln(sum(exp(scale * q . k))), -inf where nothing is seen.  max_tokens: the most tokens that a sequence has in
  *                 this call (0: not known); it chooses kernels and sizes the workspace, results are right whatever it says.
  *                 Out rows have strides like q's, are 4-byte aligned and overlap neither one another nor an input.  Scores, the
- *                 softmax's statistics and the sums are f32.  The workspace (oxq_kv4_attention_workspace_bytes of the same call; the batch's arrays are not looked
+ *                 softmax's statistics and the sums are f32.  Keys and values are used as stored, or, where a sequence has more
+ *                 than 64 query rows per kv head, rounded once to f16 (above 65504: 65504).  The workspace (oxq_kv4_attention_workspace_bytes of the same call; the batch's arrays are not looked
  *                 at; 16-byte aligned) needs no initial value and holds nothing between calls; calls that may overlap need one
  *                 each. */
 typedef struct oxq_kv4_cache {

@@ -2,8 +2,8 @@
 //
 // The mathematics is the usual one: S = Q K^T, a running reference M per row (moved only when a score exceeds it by 2^8, as
 // all exponents are taken in base 2), P = 2^(S - M), O += P V, l += row sums of P, o = O / l at the end.  Keys and values
-// become f16 numbers rounded once from c s + m (halved, so that none overflows: the factor is taken out again in f32), P is
-// f16, everything else f32.  f16 rather than bf16 operands, for either type of the queries: their rounding is eight times
+// become f16 numbers rounded once from c s + m (a number below 2^-13 is a multiple of 2^-24 and not rounded at all; one that
+// the rounding of s has lifted above 65504, by 64 at most, counts as 65504), P is f16, everything else f32.  f16 rather than bf16 operands, for either type of the queries: their rounding is eight times
 // finer.  A query row enters scaled by a power of two so that its largest element lies in [2^11, 2^12): exact, but for
 // elements below 2^-25 of it, which are off by at most 2^-36 of it; the row's factor goes into the softmax.  l is summed from
 // the unrounded p.
@@ -17,7 +17,7 @@
 //
 // What bounds it: a block's softmax and its products take turns (of 4300 cycles a tile and block: 1900 waiting for products,
 // 1650 exponentials, 450 fetching scores, 400 finding their maximum, before P was handed over in halves) and the two blocks
-// fill each other's gaps in part only; a prompt of 8192 tokens with 32 query heads on 8 takes 553 us = 994 TFLOP/s, 0.59 of
+// fill each other's gaps in part only; a prompt of 8192 tokens with 32 query heads on 8 takes 558 us = 985 TFLOP/s, 0.58 of
 // cuBLAS's rate (0.52 in a long run under the power cap), the products alone 401.  A CTA's set-up is 10 us.
 #include "oxq_kv4_attn.cuh"
 #include "oxq_tc.cuh"
@@ -64,15 +64,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // Eight codes of a word to f16 c s + m, one rounding each, in the order 0 4 1 5 2 6 3 7.  A nibble under the exponent of 1024
-// is the number 1024 + c (or 1024 + 16 c where it is left four bits up), from which c is exact in one operation.
+// is the number 1024 + c (or 1024 + 16 c where it is left four bits up), from which c is exact in one operation.  s is not
+// negative and m finite, so that overflow has one side only; a NaN stays one.
 __device__ __forceinline__ uint4 expand(uint32_t w, __half2 s, __half2 m) {
     const __half2 k1024 = as_half2(0x64006400u), k16 = as_half2(0x2C002C00u), k64 = as_half2(0xD400D400u);    // 1024, 1 / 16, -64
+    const auto value = [&](__half2 c) { return as_u32(__hmin2_nan(__hfma2(c, s, m), as_half2(0x7BFF7BFFu))); };
     uint4 o;
-    o.x = as_u32(__hfma2(__hsub2(as_half2((w & 0x000F000Fu) | 0x64006400u), k1024), s, m));
-    o.y = as_u32(__hfma2(__hfma2(as_half2((w & 0x00F000F0u) | 0x64006400u), k16, k64), s, m));
+    o.x = value(__hsub2(as_half2((w & 0x000F000Fu) | 0x64006400u), k1024));
+    o.y = value(__hfma2(as_half2((w & 0x00F000F0u) | 0x64006400u), k16, k64));
     w >>= 8;
-    o.z = as_u32(__hfma2(__hsub2(as_half2((w & 0x000F000Fu) | 0x64006400u), k1024), s, m));
-    o.w = as_u32(__hfma2(__hfma2(as_half2((w & 0x00F000F0u) | 0x64006400u), k16, k64), s, m));
+    o.z = value(__hsub2(as_half2((w & 0x000F000Fu) | 0x64006400u), k1024));
+    o.w = value(__hfma2(as_half2((w & 0x00F000F0u) | 0x64006400u), k16, k64));
     return o;
 }
 
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
             const int ex = max((int)(__float_as_uint(top) >> 23) - 127, -100);
             // a negative scale goes into the sign of the queries, a zero one into their magnitude, so that a > 0 below
             const float up = p.scale_log2 == 0.0f ? 0.0f : copysignf(pow2_of(max(11 - ex, -126)), p.scale_log2);
-            a = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2) * pow2_of(min(ex - 11 + 1, 127));       // + 1: the keys are halved
+            a = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2) * pow2_of(ex - 11);
             unsigned char* dst = smem + L::Q + t * L::OPERAND + r * 128;
 #pragma unroll
             for (int i = 0; i < D / 8; i++) {
@@ -308,7 +310,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
         l += l_odd;
         if (ok) {
             float* slot = p.parts > 1 ? p.ws + ((int64_t)blockIdx.x * p.parts + part) * (2 * BLOCK * (D + 2)) : nullptr;
-            const float inv = l > 0.0f ? 2.0f / l : l != l ? l : 0.0f;                                    // 2: the values are halved
+            const float inv = l > 0.0f ? 1.0f / l : l != l ? l : 0.0f;
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
                 uint32_t o[32];
@@ -326,8 +328,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
 #pragma unroll
                         for (int e = 0; e < 32; e += 4)
                             *reinterpret_cast<float4*>(dst + e) = make_float4(
-                                2.0f * __uint_as_float(o[(e & ~7) + kAt[e & 7]]), 2.0f * __uint_as_float(o[(e & ~7) + kAt[(e & 7) + 1]]),
-                                2.0f * __uint_as_float(o[(e & ~7) + kAt[(e & 7) + 2]]), 2.0f * __uint_as_float(o[(e & ~7) + kAt[(e & 7) + 3]]));
+                                __uint_as_float(o[(e & ~7) + kAt[e & 7]]), __uint_as_float(o[(e & ~7) + kAt[(e & 7) + 1]]),
+                                __uint_as_float(o[(e & ~7) + kAt[(e & 7) + 2]]), __uint_as_float(o[(e & ~7) + kAt[(e & 7) + 3]]));
                         if (c0 == 0) { slot[2 * BLOCK * D + t * BLOCK + r] = M; slot[2 * BLOCK * (D + 1) + t * BLOCK + r] = l; }
                     } else {
                         T* dst = (T*)p.out + (int64_t)(q.start + tok) * p.o_ts + (int64_t)qh * p.o_hs + c0;
@@ -400,8 +402,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
                 __half2 s[NG], m[NG];
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
-                    const __half2 sm = __hmul2(as_half2(par[u][g]), as_half2(0x38003800u));        // halved
-                    s[g] = __low2half2(sm); m[g] = __high2half2(sm);
+                    s[g] = __low2half2(as_half2(par[u][g])); m[g] = __high2half2(as_half2(par[u][g]));
                 }
 #pragma unroll
                 for (int i = 0; i < 4; i++) {

@@ -48,3 +48,32 @@ def test_the_edges_of_the_mask(dim, group, dtype, per, lens, new, window):
             c.cache.k_params[pg, :, sl] = torch.stack([torch.zeros_like(at), -at if falling else at], -1).half()[:, None, None]
         q = torch.ones(c.tokens, 2 * per, dim, dtype=DT[dtype], device="cuda")
         held(c, q, 8 / dim, True, window)
+
+
+@pytest.mark.parametrize("dim,group", DIMS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,new", [([500], [300]), ([5000], [40]), ([500, 70], [5, 2])])
+def test_small_keys_and_values(dim, group, dtype, lens, new):
+    """Steps and offsets below f16's normal range, down to a step of 2^-24, are held as they are: what comes out is as good as for large ones."""
+    from oxicuda_b200 import ops
+    for kf, vf in ((1.0, 2.0 ** -10), (2.0 ** -12, 2.0 ** -14), (2.0 ** -16, 2.0 ** -16), (2.0 ** -18, 2.0 ** -18), (1.0, 2.0 ** -21), (2.0 ** -21, 1.0)):
+        c = Case(lens, new, 2, dim, group, 32, seed=dim, dirty=False)
+        k, v = c.normal(sum(lens), 2, dim) * 2 * kf, c.normal(sum(lens), 2, dim) * vf
+        all_ = torch.tensor([0] + list(torch.tensor(lens).cumsum(0)), dtype=torch.int32, device="cuda")
+        ops.kv4_append(c.cache, k, v, c.table, c.lens, all_)
+        q = c.normal(c.tokens, 8, dim, dtype=DT[dtype])
+        held(c, q, dim ** -0.5 / kf, True, 0)
+        held(c, q, dim ** -0.5 / kf, True, 60)
+
+
+def test_values_at_the_end_of_f16():
+    """A group that spans f16's whole range: the largest value, which the rounding of the step lifts to 65536, counts as at least 65504."""
+    from oxicuda_b200 import ops
+    for new in (1, 200):
+        c = Case([200], [new], 1, 128, 64, 16, dirty=False)
+        x = torch.full((200, 2, 128), 65504.0, device="cuda")
+        x[:, :, ::2] = -65504.0
+        x[:, 0] *= 1e-4
+        ops.kv4_append(c.cache, x[:, :1], x[:, 1:], c.table, c.lens, torch.tensor([0, 200], dtype=torch.int32, device="cuda"))
+        out, _ = attend(c, c.normal(new, 1, 128, dtype=torch.bfloat16))
+        assert (out[..., ::2] == -65536.0).all() and (out[..., 1::2] == 65536.0).all()       # to the nearest bf16
