@@ -451,7 +451,8 @@ OXQ_API int32_t oxq_gptq_quantize_layer(oxq_handle* h, const float* weights_dev,
  * and out have `dtype` (OXQ_F32 / OXQ_BF16 / OXQ_F16), residual and residual_out `residual_dtype`: the same, or OXQ_F32.
  * Rows are `*_ld` elements apart (multiples of 8, at least cols; gate_ld 0: one gate row for all); out, q and the codes are
  * dense.  cols % 8 == 0, cols <= 16384; pointers 16-byte aligned (q: 8).  Apart from residual_out == residual (with the
- * same leading dimension) no output may overlap an input.  A row with a NaN or an infinity gives NaNs in that row only. */
+ * same leading dimension) no output may overlap an input.  A row with a NaN or an infinity gives NaNs in that row only;
+ * the INT8 form has them in the row's scale, and the row's codes then mean nothing. */
 typedef struct oxq_residual_norm {
     const void* y; int64_t y_ld; int32_t dtype;
     const void* residual; int64_t residual_ld; int32_t residual_dtype;

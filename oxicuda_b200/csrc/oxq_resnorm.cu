@@ -67,12 +67,19 @@ __device__ __forceinline__ void weight8(const float* p, float (&f)[8]) {
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
+// the larger one, or NaN where one is NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // Over the TPR threads of a row; `red` holds a word per warp of the CTA.
 template <int TPR, bool MAX> __device__ __forceinline__ float row_reduce(float v, float* red) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float w = __shfl_xor_sync(0xffffffffu, v, o);
-        v = MAX ? fmaxf(v, w) : v + w;
+        v = MAX ? max_nan(v, w) : v + w;
     }
     if constexpr (TPR > 32) {
         constexpr int W = TPR / 32;
@@ -82,7 +89,7 @@ template <int TPR, bool MAX> __device__ __forceinline__ float row_reduce(float v
         __syncthreads();
         v = red[first];
 #pragma unroll
-        for (int i = 1; i < W; i++) v = MAX ? fmaxf(v, red[first + i]) : v + red[first + i];
+        for (int i = 1; i < W; i++) v = MAX ? max_nan(v, red[first + i]) : v + red[first + i];
     }
     return v;
 }
@@ -159,14 +166,14 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_rmsnorm_kernel
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 r[i][e] = r[i][e] * inv * w[e];
-                top = fmaxf(top, fabsf(r[i][e]));
+                top = max_nan(top, fabsf(r[i][e]));
             }
         }
     }
     InvDiv d;
     if (p.mode == OUT_INT8) {
         top = row_reduce<TPR, true>(top, red);
-        const float sc = __fdiv_rn(fmaxf(top, 1e-8f), 127.0f);
+        const float sc = __fdiv_rn(max_nan(top, 1e-8f), 127.0f);        // a NaN or an infinity in the row has made an h NaN: so is then the scale, codes have no NaN
         if (live && lane == 0) p.row_scales[row] = sc;
         d = make_invdiv(sc);
     } else if (p.mode == OUT_FP8) {
