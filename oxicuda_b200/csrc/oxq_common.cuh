@@ -174,6 +174,23 @@ __device__ __forceinline__ Vec16<T> ld16_stream(const T* p) {
     *reinterpret_cast<uint4*>(&r) = u;
     return r;
 }
+// The same two for data that an earlier kernel of the stream, or this one, writes.  A kernel that was launched early is resident
+// while the one before it still writes, and the read-only path of the two above is for data that nobody writes meanwhile.
+template <typename T>
+__device__ __forceinline__ Vec16<T> ld16_written(const T* p) {
+    Vec16<T> r;
+    *reinterpret_cast<uint4*>(&r) = *reinterpret_cast<const uint4*>(p);
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ Vec16<T> ld16_written_stream(const T* p) {
+    Vec16<T> r;
+    uint4 u;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+    *reinterpret_cast<uint4*>(&r) = u;
+    return r;
+}
 
 __device__ __forceinline__ float round_mode(float v, int rounding) {
     // HALF_EVEN: rintf (cvt.rni).  HALF_AWAY: roundf, the reference's f32::round.

@@ -48,9 +48,9 @@ __device__ __forceinline__ int64_t place_of(const Pool& c, const Batch& s, int64
     int b = sequence_of(s.cu, s.seqs, first);
     const int64_t t = first + (threadIdx.x & 31);
     if ((int)(threadIdx.x & 31) >= each || t >= s.tokens) return NO_SEQUENCE;
-    while (b < s.seqs && __ldg(s.cu + b + 1) <= t) b++;
-    if (b >= s.seqs || t < __ldg(s.cu + b)) return NO_SEQUENCE;
-    return pool_row(c, s, b, (int64_t)__ldg(s.lens + b) - __ldg(s.cu + b + 1) + t, 0, status);
+    while (b < s.seqs && s.cu[b + 1] <= t) b++;
+    if (b >= s.seqs || t < s.cu[b]) return NO_SEQUENCE;
+    return pool_row(c, s, b, (int64_t)s.lens[b] - s.cu[b + 1] + t, 0, status);
 }
 
 // Eight elements as they lie.
@@ -59,7 +59,7 @@ template <typename T> __device__ __forceinline__ void load8(const T* p, int vec,
     if (vec) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; i++) {
-            const Vec16<uint32_t> v = ld16_stream(reinterpret_cast<const uint32_t*>(p) + 4 * i);
+            const Vec16<uint32_t> v = ld16_written_stream(reinterpret_cast<const uint32_t*>(p) + 4 * i);
 #pragma unroll
             for (int e = 0; e < 4; e++) r.w[4 * i + e] = v.v[e];
         }
@@ -263,8 +263,8 @@ __device__ __forceinline__ void read_rows(const Pool& c, const Batch& s, T* rows
                 codes[u] = 0; sm[u] = 0;                            // a token without a page of the pool reads as zeros
                 if (inside && write[u] && at[u] >= 0) {
                     const int64_t row = at[u] + k * round_rows;
-                    codes[u] = __ldg(codes_at + row * (D / 8));
-                    sm[u] = __ldg(params_at + row * (D / G));
+                    codes[u] = codes_at[row * (D / 8)];
+                    sm[u] = params_at[row * (D / G)];
                 }
             }
 #pragma unroll

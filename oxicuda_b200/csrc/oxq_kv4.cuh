@@ -8,6 +8,9 @@
 //           the score product in one 16-byte load, and a matrix instruction never mixes two scale groups;
 //   values  word 8 i + r lies at place r * (D / 64) + i: lane row r finds its elements of every 64-element block of the
 //           weighted sum in one load.
+//
+// None of the kernels reads through the read-only path: the pool, the queries and the batch's arrays are what earlier kernels of
+// the stream write, and with programmatic launches a kernel is resident while they do.
 #pragma once
 #include "oxq_common.cuh"
 
@@ -51,7 +54,7 @@ __device__ __forceinline__ int value_place(int word, int dim) { return (word & 7
 __device__ __forceinline__ int64_t pool_row(const Pool& c, const Batch& s, int b, int64_t pos, int head, int32_t* status) {
     const int64_t entry = pos >> c.page_shift;
     int64_t page = -1;
-    if (pos >= 0 && entry < s.width) page = __ldg(s.table + (int64_t)b * s.width + entry);
+    if (pos >= 0 && entry < s.width) page = s.table[(int64_t)b * s.width + entry];
     if (page < 0 || page >= c.pages) {
         if (pos >= 0 && status) *status = OXQ_ERR_INVALID_ARGUMENT;
         return -1;
@@ -66,7 +69,7 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int seqs, int64_t 
     while (hi > lo) {
         const int step = (hi - lo + 31) >> 5;
         const int i = lo + lane * step + step - 1;
-        const bool before = i < hi && __ldg(cu + i + 1) <= t;
+        const bool before = i < hi && cu[i + 1] <= t;
         const int c = __popc(__ballot_sync(0xffffffffu, before));
         const int nlo = min(hi, lo + c * step);
         hi = min(hi, nlo + step - 1);

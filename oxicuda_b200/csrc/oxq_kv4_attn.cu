@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
     struct { const int32_t* table; int head, first, lo, hi, tb; } src;                // of the piece whose tiles are being brought
     const auto fetch_page = [&](int i) {
         const int key = (src.first + i) * TILE + off;
-        if (i < src.tb && off < TILE && key < src.hi && key + chunk > src.lo) page = __ldg(src.table + (key >> p.c.page_shift));
+        if (i < src.tb && off < TILE && key < src.hi && key + chunk > src.lo) page = src.table[key >> p.c.page_shift];
     };
     const auto bring = [&](int i, uint32_t number) {
         const int key = (src.first + i) * TILE + off, slot = number % STAGES;
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
         *reinterpret_cast<uint4*>(&query) = make_uint4(0, 0, 0, 0);
         if (tid < ROWS * (D / 8) && row < wk.seq.n * p.per) {
             const T* src = (const T*)p.q + (int64_t)(wk.seq.start + p.by_per.div(row)) * p.q_ts + (int64_t)(wk.it.head * p.per + p.by_per.mod(row)) * p.q_hs + tid % (D / 8) * 8;
-            if (p.q_vec) query = ld16(src);
+            if (p.q_vec) query = ld16_written(src);
             else
 #pragma unroll
                 for (int e = 0; e < 8; e++) query.v[e] = src[e];

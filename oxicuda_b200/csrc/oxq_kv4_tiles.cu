@@ -173,14 +173,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
             if (real && p.q_vec) {
 #pragma unroll
                 for (int i = 0; i < D / 8; i++) {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+                    const uint4 v = reinterpret_cast<const uint4*>(src)[i];
                     raw[4 * i] = v.x; raw[4 * i + 1] = v.y; raw[4 * i + 2] = v.z; raw[4 * i + 3] = v.w;
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < D / 2; i++)
-                    raw[i] = real ? (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(src) + 2 * i) |
-                                        ((uint32_t)__ldg(reinterpret_cast<const unsigned short*>(src) + 2 * i + 1) << 16) : 0u;
+                    raw[i] = real ? (uint32_t)reinterpret_cast<const unsigned short*>(src)[2 * i] |
+                                        ((uint32_t)reinterpret_cast<const unsigned short*>(src)[2 * i + 1] << 16) : 0u;
             }
             ready();
             more_registers<168>();
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
 #pragma unroll
             for (int u = 0; u < ROUNDS; u++) {
                 const int key = (walk.first + i) * BLOCK + tok0 + u * PER_ROUND;
-                page[u] = wanted(i, key) ? __ldg(table + (key >> p.c.page_shift)) : -1;
+                page[u] = wanted(i, key) ? table[key >> p.c.page_shift] : -1;
             }
         };
         const auto load = [&](int i, const uint8_t* codes, const uint32_t* params, uint4 (&raw)[ROUNDS], uint32_t (&par)[ROUNDS][NG], bool keys) {
@@ -386,11 +386,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
                 }
                 if (good) {
                     const int64_t row = (((int64_t)page[u] * p.c.heads + head) << p.c.page_shift) + (key & ((1 << p.c.page_shift) - 1));
-                    raw[u] = __ldg(reinterpret_cast<const uint4*>(codes + row * (D / 2)) + piece);
+                    raw[u] = reinterpret_cast<const uint4*>(codes + row * (D / 2))[piece];
                     if constexpr (NG == 2) {
-                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(params + row * 2));
+                        const uint2 v = *reinterpret_cast<const uint2*>(params + row * 2);
                         par[u][0] = v.x; par[u][1] = v.y;
-                    } else par[u][0] = __ldg(params + row);
+                    } else par[u][0] = params[row];
                 }
             }
         };

@@ -6,6 +6,7 @@
 // A row is held in registers by TPR threads (NV items of eight elements each, in their own type), so every input is read once and every
 // output written once; the sums of squares meet in shared memory, in a fixed order.  Bound by memory: 8190 x 8192 bf16 with all
 // parts 123 us = 5.5 TB/s, 0.83 of the copy rate.
+// The weights alone are read through the read-only path: the rest is what earlier kernels write, or this one in place.
 #include "oxq_common.cuh"
 
 namespace oxq {
@@ -33,7 +34,7 @@ template <typename T> __device__ __forceinline__ Eight<T> load8(const T* p) {
     Eight<T> r;
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; i++) {
-        const Vec16<uint32_t> v = ld16_stream(reinterpret_cast<const uint32_t*>(p) + 4 * i);
+        const Vec16<uint32_t> v = ld16_written_stream(reinterpret_cast<const uint32_t*>(p) + 4 * i);
         r.v[i] = make_uint4(v.v[0], v.v[1], v.v[2], v.v[3]);
     }
     return r;
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_rmsnorm_kernel
         if (live && lane == 0) p.row_scales[row] = sc;
         d = make_invdiv(sc);
     } else if (p.mode == OUT_FP8) {
-        d = make_invdiv(__ldg(p.scale));
+        d = make_invdiv(*p.scale);
     }
 #pragma unroll
     for (int i = 0; i < NV; i++) {

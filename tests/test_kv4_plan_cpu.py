@@ -1,5 +1,6 @@
 """CPU tests of the sizes that attention over the 4-bit cache asks for.  A handle is faked as zeroed memory: a machine of no SMs."""
 import os
+import re
 import subprocess
 import sys
 
@@ -33,3 +34,16 @@ def test_workspace_of_any_number_of_sequences(seqs):
     _build.build()
     r = subprocess.run([sys.executable, "-c", CHILD % ([0] + ROWS, seqs, seqs)], capture_output=True, text=True, cwd=ROOT)
     assert r.returncode == 0 and r.stdout.strip() == "done", (r.returncode, r.stderr[-2000:])
+
+
+READ_ONLY = re.compile(r"__ldg\s*\(|\bld16\s*\(|\bld16_stream\s*\(|\.nc\b|__restrict__")
+
+
+@pytest.mark.parametrize("name", ["oxq_kv4.cu", "oxq_kv4.cuh", "oxq_kv4_attn.cu", "oxq_kv4_attn.cuh", "oxq_kv4_tiles.cu", "oxq_resnorm.cu"])
+def test_nothing_that_kernels_write_is_read_through_the_read_only_path(name):
+    """A kernel that starts early is resident while the one before it writes the pool, the queries or the residual; the read-only path is for data
+    that nobody writes then.  The norm's weights are."""
+    with open(os.path.join(ROOT, "oxicuda_b200", "csrc", name)) as f:
+        lines = [line.split("//")[0] for line in f]
+    found = [line.strip() for line in lines if READ_ONLY.search(line)]
+    assert all("reinterpret_cast<const float4*>(p)" in line and name == "oxq_resnorm.cu" for line in found), found
