@@ -13,8 +13,11 @@
 // The values' lie so for f16 outputs only; bf16's own step hides what is cut.  q enters as f16 scaled per row by a power of two, so that the row's largest element lies in
 // [2^11, 2^12): exact, but for elements below 2^-21 of the row's largest, which are off by at most 2^-32 of it.
 // The running reference M of a row is the maximum over its keys of x + log2(largest s of the value rows of the key and of
-// its three companions 8, 16 and 24 places apart, rounded down, at least -15), so that w stays in f16's range whatever the
-// scales are; it moves only when a key exceeds it by 2^8 (w <= 2^9), which one vote per 32 keys finds out.  l = sum p, the
+// its three companions 8, 16 and 24 places apart, rounded down, at least -15); it moves only when a key exceeds it by 2^5, which
+// one vote per 32 keys finds out.  p is taken 2^10 above it: w stays below 2^16 whatever the scales are (s ends 2^-11 short of
+// the next power of two, so at 65504 at most), and a group or a key whose s is small beside the others' keeps bits of its w.
+// w is off by 2^-25, 2^-35 of the largest, at worst, and as much again is cut from each product: a group 2^-19 of the other
+// one is as good as if it stood alone (tested; in the root mean square, bf16 outputs).  l = sum p, the
 // offsets' sum and all accumulators are f32.  bf16 outputs take w rounded once to f16 (2^-11, an eighth of their own step).
 // f16 outputs are finer than one f16 rounding of w; for them w is split into two f16 terms (two products).
 //
@@ -38,6 +41,7 @@ namespace kv4 {
 
 constexpr int TILE = 128;               // keys per tile: 4 warps x 32
 constexpr int MIN_TILES = 2;            // tiles a CTA takes at least: a join of many small parts costs more than it brings
+constexpr float ABOVE = 10.0f, MOVES = 5.0f;    // log2: how far above the reference p is taken, and by how much the reference may be exceeded
 constexpr int SETUP = 6;                // what an item costs besides its tiles, in tiles (six ragged batches at 3, 4, 5, 6, 8: 79.1, 76.4, 76.9, 75.9, 77.2 us for the first)
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -435,7 +439,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                 }
                 // ---- the rows' reference
                 float large = log2_floor(vp);                         // of this lane's four keys
-                const float most = 8.0f - large;
+                const float most = ABOVE + MOVES - large;
                 bool over = false;
                 float2 y[NT][4];
 #pragma unroll
@@ -459,7 +463,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
                             top.x = fmaxf(top.x, __shfl_xor_sync(0xffffffffu, top.x, o));
                             top.y = fmaxf(top.y, __shfl_xor_sync(0xffffffffu, top.y, o));
                         }
-                        top = make_float2(fmaxf(top.x, M[nt].x), fmaxf(top.y, M[nt].y));
+                        top = make_float2(fmaxf(top.x - ABOVE, M[nt].x), fmaxf(top.y - ABOVE, M[nt].y));
                         const float2 f = make_float2(exp2_approx(M[nt].x - top.x), exp2_approx(M[nt].y - top.y));
                         M[nt] = top;
                         l[nt].x *= f.x; l[nt].y *= f.y;
@@ -530,9 +534,12 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
         more = wk.next(p, ROWS);
         if (more) fetch_rows(wk);
 
-        // ---- join the warps: common reference, then four slabs, two warps each one after the other
+        // ---- join the warps: common reference (M was ABOVE below it), then four slabs, two warps each one after the other
+        constexpr float kDown = 0x1p-10f, kLow = (SPLIT ? 0x1p18f : 0x1p24f) * kDown, kHigh = (SPLIT ? 0x1p22f : 0x1p20f) * kDown;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
+            M[nt].x += ABOVE; M[nt].y += ABOVE;
+            l[nt].x *= kDown; l[nt].y *= kDown;
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
                 l[nt].x += __shfl_xor_sync(0xffffffffu, l[nt].x, o);
@@ -569,13 +576,13 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
 #pragma unroll
                         for (int s = 0; s < NS; s++) {
                             const float2 pg = po[nt][NG == 1 ? 0 : s];
-                            const float off = (e ? pg.y : pg.x) * f;
+                            const float off = (e ? pg.y : pg.x) * (f * kDown);
 #pragma unroll
                             for (int j = 0; j < 4; j++) {
                                 float2& at = *reinterpret_cast<float2*>(&sm.slab[warp & 3][row * OPAD + 64 * s + 8 * r + 2 * j]);
                                 float2 o;
-                                o.x = fmaf(acc[s * 4 + j][nt][e] * (SPLIT ? 0x1p18f : 0x1p24f), f, off);
-                                o.y = fmaf(acc[s * 4 + j][nt][e + 2] * (SPLIT ? 0x1p22f : 0x1p20f), f, off);
+                                o.x = fmaf(acc[s * 4 + j][nt][e] * kLow, f, off);
+                                o.y = fmaf(acc[s * 4 + j][nt][e + 2] * kHigh, f, off);
                                 if (half) { o.x += at.x; o.y += at.y; }
                                 at = o;
                             }

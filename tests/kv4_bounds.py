@@ -73,12 +73,12 @@ class Expected:
                 self.cut[mine, h] = 2.0 ** -22 * (pt @ v.abs() + o.abs() * pt.sum(1, keepdim=True)) + (length / 16 + 32) * 2.0 ** -24 * (p @ v.abs())
                 self.lse_cut[mine, h] = 2.0 ** -22 * pt.sum(1) + self.lse[mine, h].abs().nan_to_num(posinf=0.0) * 2.0 ** -22 + (math.sqrt(length) + 16) * 2.0 ** -24
 
-    def worst(self, out, lse=None):
-        """The largest of error / bound over the rows of `out`, all of it, and the rows of lse."""
+    def worst(self, out, lse=None, dims=slice(None)):
+        """The largest of error / bound over the rows of `out` (of its elements `dims`), all of it, and the rows of lse."""
         rms = lambda x, d=None: x.square().mean() ** 0.5 if d is None else x.square().mean(d).sqrt()  # noqa: E731
         live = slice(0, self.live)
-        o, var, cut = self.o[live], self.var[live], self.cut[live]
-        e = out[live].double() - o
+        o, var, cut = (x[live, :, dims] for x in (self.o, self.var, self.cut))
+        e = out[live, :, dims].double() - o
         if not torch.isfinite(e).all():
             return math.inf
         info = torch.finfo(self.dtype)

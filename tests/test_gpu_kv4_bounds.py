@@ -77,3 +77,22 @@ def test_values_at_the_end_of_f16():
         ops.kv4_append(c.cache, x[:, :1], x[:, 1:], c.table, c.lens, torch.tensor([0, 200], dtype=torch.int32, device="cuda"))
         out, _ = attend(c, c.normal(new, 1, 128, dtype=torch.bfloat16))
         assert (out[..., ::2] == -65536.0).all() and (out[..., 1::2] == 65536.0).all()       # to the nearest bf16
+
+
+@pytest.mark.parametrize("dtype,ratio", [("bf16", 19), ("f16", 15)])
+@pytest.mark.parametrize("lens,new", [([500], [1]), ([900, 70], [4, 2]), ([3000], [16]), ([400], [60])])
+def test_groups_whose_steps_are_far_apart(dtype, ratio, lens, new):
+    """The second group of every value row is 2^-ratio of the first, and is held to its own outputs' roundings.  p is taken 2^10 above the reference,
+    so the second group's largest w is 2^(10 - ratio) and off by 2^-25 at worst: 2^(ratio - 35) of itself, below the 2^-11 of its rounding (bf16) and
+    a quarter of a step of the output (f16, 2^-13)."""
+    c = Case(lens, new, 2, 128, 64, 32, seed=ratio)
+    c.fill()
+    first = 2.0 ** 6 if dtype == "bf16" else 2.0 ** 9
+    c.cache.v_params[..., 0, :].mul_(first)
+    c.cache.v_params[..., 1, :].mul_(first * 2.0 ** -ratio)
+    q = c.normal(c.tokens, 8, 128, dtype=DT[dtype])
+    out, lse = attend(c, q)
+    e = Expected(rows_of(c), new, q, 128 ** -0.5)
+    for dims in (slice(0, 64), slice(64, 128)):
+        worst = e.worst(out, lse, dims)
+        assert worst <= 1, f"{worst:.3f} of the bound for elements from {dims.start} on"
