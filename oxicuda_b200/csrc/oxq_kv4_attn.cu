@@ -79,7 +79,7 @@ __device__ __forceinline__ Span item_span(const AttnParams& p, const SeqInfo& q,
     Span s;
     const int j0 = p.by_per.div(rt * nr), j1 = p.by_per.div(min((rt + 1) * nr, q.n * p.per) - 1);
     s.hi = p.causal ? min(q.len, q.before + j1 + 1) : q.len;
-    s.lo = p.window > 0 ? max(0, q.before + j0 + 1 - p.window) : 0;
+    s.lo = max(0, window_start(p, q.before + j0));
     s.hi = max(s.hi, 0);
     s.first = min(s.lo, s.hi) / TILE;
     s.tiles = max(1, (s.hi + TILE - 1) / TILE - s.first);
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
         const int row0 = wk.it.rt * ROWS;
         // keys that every row of the block sees need no mask
         const int pos0 = before + p.by_per.div(row0), pos1 = before + p.by_per.div(min(row0 + ROWS, wk.seq.n * p.per) - 1);
-        const int all_hi = p.causal ? min(len, pos0 + 1) : len, all_lo = p.window > 0 ? pos1 + 1 - p.window : 0;
+        const int all_hi = p.causal ? min(len, pos0 + 1) : len, all_lo = window_start(p, pos1);
 
         // ---- the query rows
         __syncthreads();
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
 #pragma unroll
                             for (int e = 0; e < 2; e++) {
                                 const int pos = before + p.by_per.div(row0 + nt * 8 + 2 * c + e);      // the row's own position
-                                const int vhi = p.causal ? min(len, pos + 1) : len, vlo = p.window > 0 ? pos + 1 - p.window : 0;
+                                const int vhi = p.causal ? min(len, pos + 1) : len, vlo = window_start(p, pos);
                                 if (t < vlo || t >= vhi || !have) (e ? x[nt][h].y : x[nt][h].x) = -INFINITY;
                             }
                     }

@@ -46,6 +46,10 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnParams& p, int b) {
     return q;
 }
 
+// The first position that the window of a query at `pos` holds (0 and less: all).  A query before position 0 sees nothing, wherever
+// its window begins; it must only not wrap around.
+__device__ __forceinline__ int window_start(const AttnParams& p, int pos) { return p.window > 0 ? max(pos + 1, 0) - p.window : 0; }
+
 __device__ __forceinline__ float exp2_approx(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

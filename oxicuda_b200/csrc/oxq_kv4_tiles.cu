@@ -123,7 +123,7 @@ __device__ __forceinline__ Walk walk_of(const AttnParams& p, const SeqInfo& q, i
     const int row0 = pair * 2 * BLOCK;
     const int j0 = p.by_per.div(row0), j1 = p.by_per.div(min(row0 + 2 * BLOCK, q.n * p.per) - 1);
     const int hi = max(0, p.causal ? min(q.len, q.before + j1 + 1) : q.len);
-    const int lo = min(hi, p.window > 0 ? max(0, q.before + j0 + 1 - p.window) : 0);
+    const int lo = min(hi, max(0, window_start(p, q.before + j0)));
     const int first = lo / BLOCK, all = (hi + BLOCK - 1) / BLOCK - first;
     const int a = (int)((int64_t)all * part / p.parts), e = (int)((int64_t)all * (part + 1) / p.parts);
     return {first + a, e - a, lo, hi};
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
         const bool real = row < q.n * p.per;
         const int tok = p.by_per.div(row), qh = head * p.per + p.by_per.mod(row);
         const int pos = q.before + tok;
-        const int vhi = !real ? 0 : p.causal ? min(q.len, pos + 1) : q.len, vlo = p.window > 0 ? pos + 1 - p.window : 0;
+        const int vhi = !real ? 0 : p.causal ? min(q.len, pos + 1) : q.len, vlo = window_start(p, pos);
         float a;                                // scores to units of log2
         {
             const T* src = (const T*)p.q + (int64_t)(q.start + tok) * p.q_ts + (int64_t)qh * p.q_hs;

@@ -96,3 +96,14 @@ def test_groups_whose_steps_are_far_apart(dtype, ratio, lens, new):
     for dims in (slice(0, 64), slice(64, 128)):
         worst = e.worst(out, lse, dims)
         assert worst <= 1, f"{worst:.3f} of the bound for elements from {dims.start} on"
+
+
+@pytest.mark.parametrize("per,lens,new", [(1, [300], [350]), (4, [300, 40], [350, 3]), (1, [5, 60], [9, 61]), (2, [20], [30])])
+@pytest.mark.parametrize("window", [2 ** 31 - 2 ** 6, 2 ** 31 - 5, 2 ** 31 - 1, 2 ** 40])
+def test_the_widest_windows_with_queries_before_the_first_position(per, lens, new, window):
+    """A call may have more tokens than positions; a window that holds everything hides nothing, whatever its width."""
+    c = Case(lens, new, 2, 128, 64, 16, seed=per)
+    c.fill()
+    q = c.normal(c.tokens, 2 * per, 128, dtype=torch.bfloat16)
+    held(c, q, 128 ** -0.5, True, window)
+    assert torch.equal(attend(c, q, window=window)[0], attend(c, q)[0])
