@@ -333,13 +333,13 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) kv4_attn_rows_kernel(Att
             for (int o = 1; o < D / 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
             for (int o = 1; o < D / 8 / NG; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            const int ex = max((int)(__float_as_uint(top) >> 23) - 127, -100);
+            const int ex = max((int)(__float_as_uint(top) >> 23) - 127, -116);                      // 2^(11 - ex) has to be a number
             const float up = pow2_of(max(11 - ex, -126));
             uint4 o;
             o.x = pack_f16(f[0] * up, f[4] * up); o.y = pack_f16(f[1] * up * 0.0625f, f[5] * up * 0.0625f);
             o.z = pack_f16(f[2] * up, f[6] * up); o.w = pack_f16(f[3] * up * 0.0625f, f[7] * up * 0.0625f);
             *reinterpret_cast<uint4*>(&sm.q[row * QPAD + g * 8]) = o;
-            if (g == 0) sm.a[row] = p.scale_log2 * pow2_of(min(22 - 11 + ex, 127));
+            if (g == 0) sm.a[row] = p.scale_log2 * pow2_of(min(ex, 127)) * 0x1p11f;       // 2^(22 - 11 + ex) itself may be beyond f32
             if (g % (D / 8 / NG) == 0) sm.bsum[row][g / (D / 8 / NG)] = p.scale_log2 * sum;
         }
         if (tid == 0) sm.work[turn] = wk;

@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attn_tiles_kernel(AttnParams p
             float top = 0.0f;
 #pragma unroll
             for (int e = 0; e < D; e++) top = fmaxf(top, fabsf(value(e)));
-            const int ex = max((int)(__float_as_uint(top) >> 23) - 127, -100);
+            const int ex = max((int)(__float_as_uint(top) >> 23) - 127, -116);                      // 2^(11 - ex) has to be a number
             // a negative scale goes into the sign of the queries, a zero one into their magnitude, so that a > 0 below
             const float up = p.scale_log2 == 0.0f ? 0.0f : copysignf(pow2_of(max(11 - ex, -126)), p.scale_log2);
             a = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2) * pow2_of(ex - 11);

@@ -107,3 +107,19 @@ def test_the_widest_windows_with_queries_before_the_first_position(per, lens, ne
     q = c.normal(c.tokens, 2 * per, 128, dtype=torch.bfloat16)
     held(c, q, 128 ** -0.5, True, window)
     assert torch.equal(attend(c, q, window=window)[0], attend(c, q)[0])
+
+
+@pytest.mark.parametrize("new", [1, 3, 90])
+@pytest.mark.parametrize("power", [-110, -60, 60, 110, 118])
+def test_queries_of_any_size(new, power):
+    """Queries and scale by a power of two up and down: the same scores, so the same bits."""
+    c = Case([300], [new], 1, 128, 64, 16)
+    c.fill()
+    q = c.normal(new, 4, 128, dtype=torch.bfloat16)
+    q[:, 1, :64] *= 2.0 ** -12
+    scaled = q * 2.0 ** power
+    # 2^-110 takes elements of 2^-16 and less below bf16's normal range, 2^-126, where the product above loses bits of them; the way back up loses none
+    q = (scaled.float() * 2.0 ** -power).bfloat16()
+    want, want_lse = attend(c, q, scale=0.1)
+    out, lse = attend(c, scaled, scale=0.1 * 2.0 ** -power)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
