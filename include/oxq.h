@@ -488,7 +488,7 @@ OXQ_API int32_t oxq_residual_rmsnorm_int8_rows(oxq_handle* h, const oxq_residual
  *
  * oxq_kv4_append  keys and values [tokens][heads][dim] of `dtype` with any token and head strides (in elements; elements of a
  *                 row are adjacent): the columns of a fused projection need no copy.
- * oxq_kv4_read    the same tokens back as dense [tokens][heads][dim] of `dtype`.
+ * oxq_kv4_read    the same tokens back as dense [tokens][heads][dim] of `dtype`, keys and values apart from one another.
  * oxq_kv4_attention  q [tokens][q_heads][dim] (bf16 or f16), q_heads a multiple of heads; query head i reads kv head
  *                 i / (q_heads / heads).  o = softmax(scale * q . k) v over the keys that the query sees: with `causal` those up
  *                 to its own position, and with window > 0 of them the last `window`; without, all of the sequence.

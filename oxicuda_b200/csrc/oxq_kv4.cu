@@ -425,6 +425,8 @@ int32_t oxq_kv4_read(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_kv4_ba
     if (s.tokens == 0 || s.seqs == 0) return OXQ_OK;
     if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out)) OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 read: null output, or one that is not 16-byte aligned");
     if (s.tokens * c.heads > INT32_MAX) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 read: %lld tokens of %d heads", (long long)s.tokens, c.heads);
+    const uint64_t bytes = (uint64_t)s.tokens * c.heads * cache->dim * (dtype == OXQ_F32 ? 4 : 2), ka = (uintptr_t)k_out, va = (uintptr_t)v_out;
+    if ((ka < va ? va - ka : ka - va) < bytes) OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 read: the outputs overlap");
     if (int32_t rc = oxq_require_sm100(h)) return rc;
     OxqDeviceGuard guard(h->device);
     switch (dtype) {

@@ -1,4 +1,5 @@
 """CPU tests of the sizes that attention over the 4-bit cache asks for.  A handle is faked as zeroed memory: a machine of no SMs."""
+import ctypes as C
 import os
 import re
 import subprocess
@@ -47,3 +48,16 @@ def test_nothing_that_kernels_write_is_read_through_the_read_only_path(name):
         lines = [line.split("//")[0] for line in f]
     found = [line.strip() for line in lines if READ_ONLY.search(line)]
     assert all("reinterpret_cast<const float4*>(p)" in line and name == "oxq_resnorm.cu" for line in found), found
+
+
+@pytest.mark.parametrize("apart,dtype,status", [(0, 1, 15), (16, 1, 15), (3 * 2 * 128 * 2 - 16, 1, 15), (3 * 2 * 128 * 2, 1, 13), (3 * 2 * 128 * 2, 0, 15),
+                                                (3 * 2 * 128 * 4, 0, 13), (3 * 2 * 128 * 2, 2, 13)])
+def test_read_into_outputs_that_overlap(apart, dtype, status):
+    """13: all is right but for the machine, which has compute capability 0.0."""
+    from oxicuda_b200 import _build, _ffi
+    _build.build()
+    lib, fake = _ffi.load(), C.create_string_buffer(4096)
+    cache = _ffi.kv4_cache(0x1000, 0x2000, 0x3000, 0x4000, 8, 16, 2, 128, 64)
+    batch = _ffi.kv4_batch(0x5000, 4, 0x6000, 0x7000, 2, 3)
+    for k, v in ((0x100000, 0x100000 + apart), (0x100000 + apart, 0x100000)):
+        assert lib.oxq_kv4_read(fake, cache, batch, k, v, dtype) == status
