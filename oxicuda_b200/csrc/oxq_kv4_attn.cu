@@ -769,6 +769,7 @@ int32_t oxq_kv4_attention(oxq_handle* h, const oxq_kv4_cache* cache, const oxq_k
     if (a->max_tokens < 0) OXQ_FAIL(h, OXQ_ERR_INVALID_DIMENSION, "kv4 attention: negative max_tokens");
     if (p.s.tokens == 0 || p.s.seqs == 0) return OXQ_OK;
     if (!a->q || !a->out) OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: null queries or output");
+    if (a->q == a->out) OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: the output lies over the queries, which other CTAs may still read");
     if (a->q_token_stride < 0 || a->q_head_stride < 0 || a->out_token_stride < 0 || a->out_head_stride < 0)
         OXQ_FAIL(h, OXQ_ERR_INVALID_ARGUMENT, "kv4 attention: negative stride");
     // the strides of a single token or head are never used

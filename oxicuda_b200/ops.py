@@ -835,7 +835,8 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, block_table: torch.Tensor, s
     dim ** -0.5 unless given, over the keys up to each query's own position (causal; the last `window` of them if window > 0) or all of its sequence.
     A query that sees no key gives zeros (and -inf in lse).  max_tokens: the most tokens a sequence has in this call, 0 if it is not known; it
     only chooses kernels.  Returns out, or (out, lse f32 [tokens, q_heads]) if want_lse or lse is given.  Rows behind the last sequence
-    are left as they were.  `workspace` (uint8, kv4_attention_workspace_bytes) may be given to allocate nothing; overlapping calls need one each."""
+    are left as they were.  `out` must not lie over the queries.  `workspace` (uint8, kv4_attention_workspace_bytes) may be given to allocate nothing;
+    overlapping calls need one each."""
     shape = q.shape
     if len(shape) != 3 or shape[1] == 0 or cache.heads == 0 or shape[1] % cache.heads != 0:
         from .errors import QuantError

@@ -61,3 +61,15 @@ def test_read_into_outputs_that_overlap(apart, dtype, status):
     batch = _ffi.kv4_batch(0x5000, 4, 0x6000, 0x7000, 2, 3)
     for k, v in ((0x100000, 0x100000 + apart), (0x100000 + apart, 0x100000)):
         assert lib.oxq_kv4_read(fake, cache, batch, k, v, dtype) == status
+
+
+def test_attention_in_place():
+    """An item's rows are read by every CTA that has a part of its keys, so its output cannot take their place."""
+    from oxicuda_b200 import _build, _ffi
+    _build.build()
+    lib, fake = _ffi.load(), C.create_string_buffer(4096)
+    cache = _ffi.kv4_cache(0x1000, 0x2000, 0x3000, 0x4000, 8, 16, 2, 128, 64)
+    batch = _ffi.kv4_batch(0x5000, 4, 0x6000, 0x7000, 2, 3)
+    for out, status in ((0x8000, 15), (0x18000, 13)):
+        args = _ffi.kv4_attention_args(0x8000, 1024, 128, out, 1024, 128, 0, 8, 0, 0, 0.1, 1, 1)
+        assert lib.oxq_kv4_attention(fake, cache, batch, args, 0x10000, 1 << 30) == status
