@@ -5,8 +5,8 @@ spread).  Sequences of more than 64 query rows per kv head (many rows): keys, va
     o is off by  sum p v (d_p + d_v) + sum p dx (v - o),   dx = scale * sum q k d_k,   each d independent of the others,
 and the log of the sum by sum p dx.  Others (few rows): keys and values are exact, and for bf16 outputs w = p s is one f16 number: sum p s c d_w.
 A row of an output is held to four standard deviations of this and half a step of its own rounding; all rows together to a tenth more than what
-this and the rounding of the reference itself come to.  What f32 does besides is small and bounded: the products are cut 2^-22 of their terms' sum
-short, the sums of N keys lose 2^-24 at each of N / 16 steps."""
+this and the rounding of the reference itself come to.  What f32 does besides is small and bounded: a score is cut 2^-22 of the sum of its terms' sizes
+short -- q k for many rows, q c s and q m, which may cancel, for few -- and the sums of N keys lose 2^-24 at each of N / 16 steps."""
 import math
 
 import torch
@@ -14,16 +14,17 @@ import torch
 U = 2.0 ** -11 / math.sqrt(3)
 
 
-def goes_to_many_rows(new, per, max_tokens):
-    """Per sequence: whether the kernel for many query rows takes it."""
-    tokens = sum(new)
+def goes_to_many_rows(new, per, max_tokens, tokens=None):
+    """Per sequence: whether the kernel for many query rows takes it, in a call of `tokens` rows (those behind the last sequence among them)."""
+    tokens = tokens or sum(new)
     tiles = min(max_tokens or tokens, tokens) * per > 64
     alike = len(new) == 1 or (max_tokens > 0 and tokens // max_tokens >= len(new))
     return [tiles and (alike or n * per > 64) for n in new]
 
 
 class Expected:
-    """o, lse and what they may be off by, per query row [tokens, q_heads, ...].  rows[b] = (k, v, s c) of sequence b, [len, heads, dim] in f64."""
+    """o, lse and what they may be off by, per query row [tokens, q_heads, ...].  rows[b] = (k, v, s c of v, |s c| + |m| of k) of sequence b,
+    [len, heads, dim] in f64."""
 
     def __init__(self, rows, new, q, scale, causal=True, window=0, max_tokens=None, see=None):
         t, hq, dim = q.shape
@@ -35,7 +36,7 @@ class Expected:
         self.o, self.lse = z(t, hq, dim), torch.full((t, hq), -math.inf, dtype=torch.float64, device=dev)
         self.var, self.cut = z(t, hq, dim), z(t, hq, dim)               # variance in units of u^2; what f32 may add
         self.lse_var, self.lse_cut = z(t, hq), z(t, hq)
-        many = goes_to_many_rows(new, per, max(new) if max_tokens is None else max_tokens)
+        many = goes_to_many_rows(new, per, max(new) if max_tokens is None else max_tokens, t)
         at0 = 0
         for b, n in enumerate(new):
             length = rows[b][0].shape[0]
@@ -52,7 +53,7 @@ class Expected:
                 continue
             any_ = sees.any(1)
             for h in range(hq):
-                k, v, sc = (r[:, h // per] for r in rows[b])
+                k, v, sc, size = (r[:, h // per] for r in rows[b])
                 qq = q[mine, h].double()
                 x = qq @ k.T * scale
                 x[~sees] = -math.inf
@@ -62,7 +63,7 @@ class Expected:
                 o = p @ v
                 self.o[mine, h] = o
                 p2 = p * p
-                terms = abs(scale) * (qq.abs() @ k.abs().T)              # of a score
+                terms = abs(scale) * (qq.abs() @ (k.abs() if many[b] else size).T)
                 if many[b]:
                     w2 = p2 * (scale * scale) * (qq.square() @ k.square().T)
                     self.var[mine, h] = 2 * (p2 @ v.square()) + (w2 @ v.square() - 2 * o * (w2 @ v) + o * o * w2.sum(1, keepdim=True)).clamp(min=0)
@@ -103,6 +104,6 @@ def rows_of(c):
     for b, n in enumerate(c.lens_l):
         k, v = c.rows(b, True), c.rows(b, False)
         pg, sl = c.place(b, torch.arange(max(n, 0), device=c.table.device))
-        m = c.cache.v_params[pg, :, sl][..., 1].double()
-        out.append((k, v, v - m.repeat_interleave(c.group, -1)))
+        km, vm = (p[pg, :, sl][..., 1].double().repeat_interleave(c.group, -1) for p in (c.cache.k_params, c.cache.v_params))
+        out.append((k, v, v - vm, (k - km).abs() + km.abs()))
     return out

@@ -25,8 +25,8 @@ def make(per, lens, new, dim=64, group=64, seed=0):
             x[:, :, 3] *= 6.0
             c, p = quantize(x, group)
             s, m = (p[..., i].double().repeat_interleave(group, -1) for i in (0, 1))
-            kv += [c * s + m, c * s]
-        rows.append((kv[0], kv[2], kv[3]))
+            kv += [c * s + m, c * s, m]
+        rows.append((kv[0], kv[3], kv[4], kv[1].abs() + kv[2].abs()))
     return rows, torch.randn(sum(new), per, dim, generator=g)
 
 
@@ -46,7 +46,7 @@ def as_the_kernels_round(rows, new, q, scale, see, many, dtype, g):
     f16 = lambda x: x.half().double()  # noqa: E731
     at = 0
     for b, n in enumerate(new):
-        k, v, sc = (r[:, 0] for r in rows[b])
+        k, v, sc, _ = (r[:, 0] for r in rows[b])
         if many[b]:
             k, v = f16(k), f16(v)
         for h in range(q.shape[1]):
