@@ -6,8 +6,10 @@
 // codes.  s and m stay f16 (4 bytes a group): the offset is a float, not a zero-point in code units, because a group whose
 // values all lie on one side of zero must keep its four bits for its own range.
 //
-// What bounds them: appending, the quantizer's instructions (8192 tokens of 8 heads, keys and values: 18 us, the
-// bytes need 6.6); reading, memory (131k tokens: 125 us = 5.6 TB/s, 0.86 of the copy rate).
+// What bounds them: appending, 8192 tokens of 8 heads, keys and values, takes 18 us where the bytes need 6.6.  No pipe is full
+// (issue 0.67 of the cycles, logic 0.53): an instruction takes 9.9 cycles of a warp, 3.0 of them waits for rows, and 26 of 64
+// warps are there; what is missing are rows on their way.  Reading: memory (131k tokens: 125 us = 5.6 TB/s, 0.86 of the copy
+// rate).
 #include "oxq_kv4.cuh"
 
 namespace oxq {

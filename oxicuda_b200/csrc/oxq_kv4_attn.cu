@@ -32,7 +32,8 @@
 //
 // What bounds it: about 300 instructions per 16 keys at 16 warps on an SM, half of them on the logic pipe, which issues at
 // half rate (32 sequences of 50 to 16000 keys, 8 kv heads of 128: 77 us, the tiles alone stream in 56, their bytes need 47;
-// 4 x 131072 keys: 111, 87, 80).  A single short call is latency: 3.5 us to find the work, 2 to the first tiles, 4 for the join.
+// 4 x 131072 keys: 111, 87, 80).  f16 queries, with two products for a weight: 88 and 127, at 128 registers and 4 bytes spilled
+// for two groups.  A single short call is latency: 3.5 us to find the work, 2 to the first tiles, 4 for the join.
 #include "oxq_kv4_attn.cuh"
 #include "oxq_tc.cuh"
 

@@ -18,7 +18,8 @@
 // What bounds it: a block's softmax and its products take turns (of 4300 cycles a tile and block: 1900 waiting for products,
 // 1650 exponentials, 450 fetching scores, 400 finding their maximum, before P was handed over in halves) and the two blocks
 // fill each other's gaps in part only; a prompt of 8192 tokens with 32 query heads on 8 takes 558 us = 985 TFLOP/s, 0.58 of
-// cuBLAS's rate (0.52 in a long run under the power cap), the products alone 401.  A CTA's set-up is 10 us.
+// cuBLAS's rate (0.52 in a long run under the power cap), the products alone 401.  A CTA's set-up is 10 us.  At 96 registers a
+// thread before the split the compiler spills 70 to 86 bytes.
 #include "oxq_kv4_attn.cuh"
 #include "oxq_tc.cuh"
 
